@@ -460,6 +460,73 @@ int kbn_fp8_block_requant(const void* w_in, int in_f32, const float* s_in, int64
                           int64_t s_out_e, int64_t s_out_ld, int use_ue8m0, float eps, void* stream);
 
 /*
+ * MXFP4 quantization (no counterpart in the reference): groups of 32 values
+ * along K share a power-of-two scale, each value is a 4-bit e2m1 code (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 and their negatives).
+ *   x       [M, K] of x_dtype (0 bf16, 1 fp16, 2 fp32), K % 32 == 0, rows
+ *           16-byte aligned, ld_x % 8 == 0
+ *   codes   uint8 [M, K/2], two codes a byte, even k in the low nibble; row
+ *           stride in bytes, a multiple of 4
+ *   scales  uint8 [M, K/32], E8M0: the group's scale is 2^(byte - 127)
+ *   Per group: a = max|x| rounded to one mantissa bit (ties up); byte =
+ *   exponent(a) - 2, biased, at least 1; codes = x / scale to the nearest, ties to
+ *   even, at most 6 in magnitude.  A group that holds an infinity or a NaN gets
+ *   byte 255 (it reads back as NaN).
+ */
+int kbn_mxfp4_quant(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                    void* scales, int64_t ld_scales, void* stream);
+
+/* The values of MXFP4 rows in out_dtype (0 bf16, 1 fp16, 2 fp32; exact in bf16
+ * and fp32 but for bytes above 252, where 4 and 6 exceed the types' range).
+ * Any scale bytes, 0 (2^-127) and 255 (NaN) too; sizes, strides and alignment
+ * as above. */
+int kbn_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                      void* out, int out_dtype, int64_t ld_out, void* stream);
+
+/*
+ * Product of two MXFP4 operands (no counterpart in the reference):
+ *   D[m, n] = bf16_rne( sum_g sA[m,g] sW[n,g] sum_{k in g} A[m,k] W[n,k] ), fp32 sums
+ *   A codes [M, K/2] and scales [M, K/32], W codes [N, K/2] and scales
+ *   [N, K/32], K % 128 == 0; code rows 16-byte, scale rows 4-byte aligned
+ *   (strides in bytes, multiples of 16 and 4); D bf16 [M, N], row stride ldd.
+ * The workspace (bytes as asked for the shape, may be 0) is 16-byte aligned.
+ */
+int64_t kbn_mxfp4_gemm_nt_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int64_t ld_sa, const void* W, int64_t ldw, const void* sW,
+                      int64_t ld_sw, void* D, int64_t ldd, int64_t M, int64_t N, int64_t K, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* kbn_mxfp4_quant of x [M, K], then kbn_mxfp4_gemm_nt with W: the same bits.
+ * x as for the quant, with K % 128 == 0. */
+int64_t kbn_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype);
+int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const void* W, int64_t ldw, const void* sW, int64_t ld_sw,
+                     void* D, int64_t ldd, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/*
+ * A whole experts layer for few tokens in two launches: the role of
+ * VllmFusedExperts (tasks/baseline/L2/vllm_fused_experts.py:100-237) at decode
+ * batches, with activations that are not quantized.
+ *   out[t] = sum_e c[t,e] W2_e (silu(G_e x_t) * (U_e x_t)),  w13[e] = [G_e | U_e]
+ *   c[t,e] = sum of topk_weights[t, j] over the slots j with topk_ids[t, j] == e;
+ *   ids outside [0, E) count for nothing (a token with none gets zeros).
+ *   x            [T, H] of x_dtype (0 bf16, 1 fp16), rows 16-byte aligned; T <= 64
+ *   w_format     0: w13 fp8 [E, 2I, H], w2 fp8 [E, H, I], fp32 scales
+ *                   [E, 2I/128, H/128] and [E, H/128, I/128], used as given
+ *                1: MXFP4 codes [E, 2I, H/2] and [E, H, I/2], scales
+ *                   [E, 2I, H/32] and [E, H, I/32]; all contiguous
+ *   topk_weights fp32 [T, topk], topk_ids int32 or int64 (id_bytes 4, 8) [T, topk];
+ *                topk <= 32, E <= 1024
+ *   out          [T, H] of x_dtype, row stride ld_out; H and I multiples of 128
+ * The workspace holds h (bytes as asked), 16-byte aligned.
+ */
+int64_t kbn_few_token_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I);
+int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* w13, const void* s13, const void* w2,
+                          const void* s2, int w_format, const float* topk_weights, const void* topk_ids, int id_bytes,
+                          int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, void* out, int64_t ld_out,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Split-K arrival counters (no counterpart in the reference; DeepGEMM has no
  * split-K).  The small-M split launches of the 64-row tiles sum their fp32
  * slabs themselves, counting arrivals in a region of a library-held device

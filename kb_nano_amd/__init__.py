@@ -14,10 +14,16 @@ sorted-token counterpart ``VllmFusedExperts`` (``MoeAlign``,
 fused ``RMSNormFP8Quant`` / ``FusedAddRMSNormFP8Quant`` that produce the
 quantized activations of a decoder layer's first linear.
 
+Beside them, without a kb_nano counterpart: MXFP4 (``Mxfp4Quant``,
+``dequantize_mxfp4`` and ``Mxfp4Linear``, 4-bit codes with a scale per 32
+values) and ``FewTokenExperts``, the experts layer of a decode batch in two
+launches, over FP8 or MXFP4 weights.
+
 The compute runs in hand-written gfx950 HIP kernels (``csrc/``) behind the
 C-ABI of ``libkbn_fp8.so`` (declared in ``include/kbn_fp8.h``); this package
 is the PyTorch-side host layer.
 """
+from .few_token_experts import FewTokenExperts
 from .fp8_grouped_gemm_contiguous import Fp8GroupedGemmContiguous
 from .fused_experts import FusedExperts
 from .fp8_linear import (
@@ -31,6 +37,7 @@ from .fp8_linear import (
 from .moe_align import MoeAlign
 from .moe_grouped_gemm import MoeGroupedGemm, m_grouped_fp8_gemm_nt_contiguous
 from .moe_sum import MoeSum
+from .mxfp4 import Mxfp4Linear, Mxfp4Quant, dequantize_mxfp4
 from .rmsnorm_quant import FusedAddRMSNormFP8Quant, RMSNormFP8Quant
 from .silu_mul_quant_fp8 import SiluMulQuantFp8
 from .vllm_fused_experts import VllmFusedExperts
@@ -48,6 +55,10 @@ __all__ = [
     "MoeSum",
     "RMSNormFP8Quant",
     "FusedAddRMSNormFP8Quant",
+    "Mxfp4Quant",
+    "dequantize_mxfp4",
+    "Mxfp4Linear",
+    "FewTokenExperts",
     "postprocess_model_fp8_weights",
     "warmup_fp8_linear",
     "m_grouped_fp8_gemm_nt_contiguous",

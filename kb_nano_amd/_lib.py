@@ -58,6 +58,15 @@ SIGNATURES = {
     "kbn_fp8_fused_moe_gemm_workspace_bytes": ([_I64, _I64], _I64),
     "kbn_moe_sum": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "kbn_fp8_block_requant": ([_P, _I, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I, _F, _P], _I),
+    "kbn_mxfp4_quant": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _P], _I),
+    "kbn_mxfp4_dequant": ([_P, _I64, _P, _I64, _I64, _I64, _P, _I, _I64, _P], _I),
+    "kbn_mxfp4_gemm_nt_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "kbn_mxfp4_gemm_nt": ([_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "kbn_mxfp4_linear_workspace_bytes": ([_I64, _I64, _I64, _I], _I64),
+    "kbn_mxfp4_linear": ([_P, _I, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "kbn_few_token_experts_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "kbn_few_token_experts": ([_P, _I, _I64, _P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P,
+                               _I64, _P], _I),
     "kbn_splitk_counter_stats": ([_P, _P, _P], _I),
     "kbn_debug_splitk_regions": ([_I64, _P, _P], _I),
     "kbn_debug_gemm_plan": ([_I64, _I64, _I64, _I, _I, _P], _I),

@@ -45,6 +45,10 @@ _BF16 = torch.bfloat16
 _F32 = torch.float32
 # input dtype codes of kbn_per_token_group_quant_fp8_typed
 _QUANT_IN = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# MXFP4 operands: packed codes, scale bytes and values a scale
+MX_CODES = (torch.uint8, torch.float4_e2m1fn_x2)
+MX_SCALES = (torch.float8_e8m0fnu, torch.uint8)
+MX_GROUP = 32
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -890,6 +894,178 @@ def moe_sum(x: torch.Tensor, out: torch.Tensor) -> None:
           what)
 
 
+def _mx_rows(what: str, name: str, t: torch.Tensor, shape: tuple) -> None:
+    if tuple(t.shape) != shape or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{what}: {name} must be {shape} with contiguous rows, got {tuple(t.shape)}, strides "
+                         f"{t.stride()}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor (a single row's own says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _mx_types(what: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
+    if codes.dtype not in MX_CODES:
+        raise TypeError(f"{what}: {name} codes must be uint8 or float4_e2m1fn_x2 (two a byte), got {codes.dtype}")
+    if scales.dtype not in MX_SCALES:
+        raise TypeError(f"{what}: {name} scales must be float8_e8m0fnu or uint8, got {scales.dtype}")
+
+
+def _mx_quant_args(what: str, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> tuple:
+    _dev_check(what, x, codes, scales)
+    if x.dtype not in _QUANT_IN:
+        raise TypeError(f"{what}: values must be bfloat16, float16 or float32, got {x.dtype}")
+    _mx_types(what, codes, scales, "its")
+    if x.dim() != 2:
+        raise ValueError(f"{what}: 2-D values expected, got {tuple(x.shape)}")
+    M, K = x.shape
+    if K % MX_GROUP:
+        raise ValueError(f"{what}: K={K} must be a multiple of {MX_GROUP}")
+    _mx_rows(what, "values", x, (M, K))
+    _mx_rows(what, "codes", codes, (M, K // 2))
+    _mx_rows(what, "scales", scales, (M, K // MX_GROUP))
+    return M, K
+
+
+def mxfp4_quant(x: torch.Tensor, out_codes: torch.Tensor, out_scales: torch.Tensor) -> None:
+    """MXFP4 codes and scales of ``x [M, K]`` (bf16, fp16 or fp32, K % 32 == 0)
+    into ``out_codes [M, K/2]`` and ``out_scales [M, K/32]``."""
+    what = "mxfp4_quant"
+    M, K = _mx_quant_args(what, x, out_codes, out_scales)
+    check(lib().kbn_mxfp4_quant(x.data_ptr(), _QUANT_IN[x.dtype], M, K, _ld(x), out_codes.data_ptr(),
+                                _ld(out_codes), out_scales.data_ptr(), _ld(out_scales), _stream(x)), what)
+
+
+def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor) -> None:
+    """The values of MXFP4 rows into ``out [M, K]`` (bf16, fp16 or fp32)."""
+    what = "mxfp4_dequant"
+    M, K = _mx_quant_args(what, out, codes, scales)
+    check(lib().kbn_mxfp4_dequant(codes.data_ptr(), _ld(codes), scales.data_ptr(), _ld(scales), M, K,
+                                  out.data_ptr(), _QUANT_IN[out.dtype], _ld(out), _stream(out)), what)
+
+
+def _mx_weight_args(what: str, w: torch.Tensor, ws: torch.Tensor, out: torch.Tensor, M: int, K: int) -> int:
+    _mx_types(what, w, ws, "weight")
+    _dtype_check(what, out, _BF16, "output")
+    if K % GROUP or K == 0:
+        raise ValueError(f"{what}: K={K} must be a multiple of {GROUP}")
+    if w.dim() != 2:
+        raise ValueError(f"{what}: 2-D weight codes expected, got {tuple(w.shape)}")
+    N = w.shape[0]
+    _mx_rows(what, "weight codes", w, (N, K // 2))
+    _mx_rows(what, "weight scales", ws, (N, K // MX_GROUP))
+    _mx_rows(what, "output", out, (M, N))
+    return N
+
+
+def mxfp4_gemm_nt(a: torch.Tensor, a_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                  output: torch.Tensor) -> None:
+    """``output[M, N]`` (bf16) = MXFP4 ``a [M, K]`` x MXFP4 ``weight [N, K]``^T
+    (codes two a byte, one scale per 32 K; fp32 sums)."""
+    what = "mxfp4_gemm_nt"
+    _dev_check(what, a, a_scale, weight, weight_scale, output)
+    _mx_types(what, a, a_scale, "a")
+    if a.dim() != 2:
+        raise ValueError(f"{what}: 2-D codes expected, got {tuple(a.shape)}")
+    M, K = a.shape[0], 2 * a.shape[1]
+    N = _mx_weight_args(what, weight, weight_scale, output, M, K)
+    _mx_rows(what, "a codes", a, (M, K // 2))
+    _mx_rows(what, "a scales", a_scale, (M, K // MX_GROUP))
+    if M == 0 or N == 0:
+        return
+    L = lib()
+    nbytes = L.kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    check(L.kbn_mxfp4_gemm_nt(a.data_ptr(), _ld(a), a_scale.data_ptr(), _ld(a_scale), weight.data_ptr(),
+                              _ld(weight), weight_scale.data_ptr(), _ld(weight_scale), output.data_ptr(),
+                              _ld(output), M, N, K, buf.data_ptr() if nbytes else None, nbytes, _stream(a)), what)
+
+
+def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, output: torch.Tensor) -> None:
+    """``mxfp4_quant`` of ``x [M, K]`` and ``mxfp4_gemm_nt`` with ``weight`` in one
+    library call (the same bits).  The codes and scales of ``x`` live in a
+    buffer of the call's own: calls at the same time, on one stream or several,
+    share nothing."""
+    what = "mxfp4_linear"
+    _dev_check(what, x, weight, weight_scale, output)
+    if x.dtype not in _QUANT_IN:
+        raise TypeError(f"{what}: input must be bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"{what}: 2-D input expected, got {tuple(x.shape)}")
+    M, K = x.shape
+    N = _mx_weight_args(what, weight, weight_scale, output, M, K)
+    _mx_rows(what, "input", x, (M, K))
+    if M == 0 or N == 0:
+        return
+    L = lib()
+    code = _QUANT_IN[x.dtype]
+    nbytes = L.kbn_mxfp4_linear_workspace_bytes(M, N, K, code)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    check(L.kbn_mxfp4_linear(x.data_ptr(), code, _ld(x), weight.data_ptr(), _ld(weight),
+                             weight_scale.data_ptr(), _ld(weight_scale), output.data_ptr(), _ld(output),
+                             M, N, K, buf.data_ptr() if nbytes else None, nbytes, _stream(x)), what)
+
+
+FEW_TOKENS = 64   # rows few_token_experts covers
+
+
+def few_token_experts(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor,
+                      w2_scale: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
+                      out: torch.Tensor) -> None:
+    """A whole experts layer for at most 64 tokens in two launches:
+    ``out[t] = sum_j topk_weights[t, j] * W2_e (silu(G_e x_t) * (U_e x_t))`` with
+    ``e = topk_ids[t, j]`` and ``w13[e] = [G_e | U_e]``; ids outside [0, E) count
+    for nothing.  ``x`` and ``out`` [T, H], bf16 or fp16; weights fp8 [E, 2I, H]
+    and [E, H, I] with fp32 128x128 block scales (used as given), or MXFP4 codes
+    [E, 2I, H/2] and [E, H, I/2] with a scale per 32 K."""
+    what = "few_token_experts"
+    _dev_check(what, x, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids, out)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: hidden states must be bfloat16 or float16, got {x.dtype}")
+    _dtype_check(what, out, x.dtype, "output")
+    _dtype_check(what, topk_weights, torch.float32, "topk_weights")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: topk_ids must be int32 or int64, got {topk_ids.dtype}")
+    if x.dim() != 2 or topk_ids.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+        raise ValueError(f"{what}: hidden states [T, H], routing [T, top_k], w13 [E, 2I, H] and w2 [E, H, I] expected")
+    T, H = x.shape
+    topk = topk_ids.shape[1]
+    E, N2 = w13.shape[:2]
+    inter = N2 // 2
+    if T > FEW_TOKENS:
+        raise ValueError(f"{what}: {T} tokens, at most {FEW_TOKENS}; VllmFusedExperts and FusedExperts take more")
+    if H % GROUP or N2 % (2 * GROUP) or H == 0 or N2 == 0:
+        raise ValueError(f"{what}: H={H} and I={N2 / 2:g} must be multiples of {GROUP}")
+    fp8 = w13.dtype is FP8
+    if fp8:
+        _dtype_check(what, w2, FP8, "w2")
+        _dtype_check(what, w13_scale, torch.float32, "w13_scale")
+        _dtype_check(what, w2_scale, torch.float32, "w2_scale")
+        shapes = ((E, N2, H), (E, H, inter), (E, N2 // GROUP, H // GROUP), (E, H // GROUP, inter // GROUP))
+    else:
+        _mx_types(what, w13, w13_scale, "w13")
+        _mx_types(what, w2, w2_scale, "w2")
+        shapes = ((E, N2, H // 2), (E, H, inter // 2), (E, N2, H // MX_GROUP), (E, H, inter // MX_GROUP))
+    for t, name, shape in zip((w13, w2, w13_scale, w2_scale), ("w13", "w2", "w13_scale", "w2_scale"), shapes):
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous {shape}, got {tuple(t.shape)}")
+    for t, name in ((topk_weights, "topk_weights"), (topk_ids, "topk_ids")):
+        if tuple(t.shape) != (T, topk) or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous {(T, topk)}, got {tuple(t.shape)}")
+    _mx_rows(what, "hidden states", x, (T, H))
+    _mx_rows(what, "output", out, (T, H))
+    if T == 0:
+        return
+    L = lib()
+    nbytes = L.kbn_few_token_experts_workspace_bytes(T, topk, inter)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    check(L.kbn_few_token_experts(
+        x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(),
+        w2_scale.data_ptr(), 0 if fp8 else 1, topk_weights.data_ptr(), topk_ids.data_ptr(), topk_ids.element_size(),
+        T, topk, E, H, inter, out.data_ptr(), _ld(out), buf.data_ptr(), nbytes, _stream(x)), what)
+
+
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the storage byte ranges spanned by two tensors intersect."""
     def span(t):
@@ -964,6 +1140,7 @@ def debug_silu_bf16(g_bits: torch.Tensor, out_bits: torch.Tensor, path: int = 0)
 _fp8_lib = torch.library.Library("kb_nano_fp8", "FRAGMENT")
 _moe_lib = torch.library.Library("kb_nano_fp8_moe", "FRAGMENT")
 _norm_lib = torch.library.Library("kb_nano_norm", "FRAGMENT")
+_mx_lib = torch.library.Library("kb_nano_mxfp4", "FRAGMENT")
 
 
 def _has_op(ns: str, name: str) -> bool:
@@ -1026,6 +1203,21 @@ def _register():
         _norm_lib.impl("fused_add_rmsnorm_fp8_quant",
                        lambda q, s, x, r, w, eps: rmsnorm_fp8_quant(q, s, x, w, eps, residual=r), "CUDA")
         _norm_lib.impl("fused_add_rmsnorm_fp8_quant", _meta_noop, "Meta")
+    # this package's own operators (no reference counterpart)
+    for ns, ops, schema, fn in (
+            ("kb_nano_mxfp4", _mx_lib, "quant(Tensor x, Tensor! out_codes, Tensor! out_scales) -> ()", mxfp4_quant),
+            ("kb_nano_mxfp4", _mx_lib, "dequant(Tensor codes, Tensor scales, Tensor! out) -> ()", mxfp4_dequant),
+            ("kb_nano_mxfp4", _mx_lib, "gemm_nt(Tensor a, Tensor a_scale, Tensor weight, Tensor weight_scale, "
+             "Tensor! output) -> ()", mxfp4_gemm_nt),
+            ("kb_nano_mxfp4", _mx_lib, "linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor! output) -> ()",
+             mxfp4_linear),
+            ("kb_nano_fp8_moe", _moe_lib, "few_token_experts(Tensor x, Tensor w13, Tensor w13_scale, Tensor w2, "
+             "Tensor w2_scale, Tensor topk_weights, Tensor topk_ids, Tensor! out) -> ()", few_token_experts)):
+        name = schema[:schema.index("(")]
+        if not _has_op(ns, name):
+            ops.define(schema)
+            ops.impl(name, fn, "CUDA")
+            ops.impl(name, _meta_noop, "Meta")
 
 
 _register()

@@ -1,0 +1,230 @@
+// MXFP4 quantization and back, and the product of two MXFP4 operands
+//   D[m, n] = bf16( sum_g 2^(ea[m,g] + ew[n,g] - 254) sum_{k in g} a[m,k] w[n,k] ),
+// sums in fp32.
+#include "mxfp4.h"
+
+#include <algorithm>
+
+namespace kbn {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ quant ---
+
+constexpr int kQuantThreads = 256;
+
+// One lane per eight values, four lanes a group.
+template <int kIn>
+__global__ __launch_bounds__(kQuantThreads) void mxfp4_quant_kernel(const void* x, int64_t ld_x, int64_t M, int64_t K,
+                                                                   uint8_t* codes, int64_t ld_c, uint8_t* scales,
+                                                                   int64_t ld_s) {
+    const int64_t k = ((int64_t)blockIdx.x * kQuantThreads + threadIdx.x) * 8;
+    if (k >= K) return;   // whole groups: K is a multiple of 32
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+        uint32_t w[kIn == kMxF32 ? 8 : 4];
+        mx_load8<kIn>(x, m * ld_x + k, w);
+        const uint32_t byte = mx_scale_byte(quad_max_u32(mx_absmax8<kIn>(w)));
+        *reinterpret_cast<uint32_t*>(codes + m * ld_c + k / 2) = mx_codes8<kIn>(w, byte);
+        if ((threadIdx.x & 3) == 0) scales[m * ld_s + k / kMxGroup] = (uint8_t)byte;
+    }
+}
+
+template <int kOut>
+__global__ __launch_bounds__(kQuantThreads) void mxfp4_dequant_kernel(const uint8_t* codes, int64_t ld_c,
+                                                                     const uint8_t* scales, int64_t ld_s, int64_t M,
+                                                                     int64_t K, void* out, int64_t ld_o) {
+    const int64_t k = ((int64_t)blockIdx.x * kQuantThreads + threadIdx.x) * 8;
+    if (k >= K) return;
+    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+        const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + m * ld_c + k / 2);
+        const uint32_t byte = scales[m * ld_s + k / kMxGroup];
+        // byte 0 stands for 2^-127: the conversion reads the exponent field
+        // alone, and 0 there means just that; 255 gives NaN
+        const float sc = __uint_as_float(byte << 23);
+        if constexpr (kOut == kMxF32) {
+            const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 1),
+                        c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 3);
+            v4f* p = reinterpret_cast<v4f*>(static_cast<float*>(out) + m * ld_o + k);
+            p[0] = v4f{a.x, a.y, b.x, b.y};
+            p[1] = v4f{c.x, c.y, d.x, d.y};
+        } else {
+            u32x4 o;
+            if constexpr (kOut == kMxBf16) {
+                o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 0));
+                o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 1));
+                o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 2));
+                o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 3));
+            } else {
+                o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, sc, 0));
+                o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, sc, 1));
+                o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, sc, 2));
+                o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, sc, 3));
+            }
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + m * ld_o + k) = o;
+        }
+    }
+}
+
+static dim3 quant_grid(int64_t M, int64_t K) {
+    return dim3((unsigned)((K / 8 + kQuantThreads - 1) / kQuantThreads), (unsigned)std::min<int64_t>(M, 32768));
+}
+
+// ---------------------------------------------------------------- product ---
+
+struct MxGemmArgs {
+    const uint8_t* A;    // codes [M, K/2]
+    int64_t lda;
+    const uint8_t* sA;   // scale bytes [M, K/32]
+    int64_t ld_sa;
+    const uint8_t* W;
+    int64_t ldw;
+    const uint8_t* sW;
+    int64_t ld_sw;
+    uint16_t* D;
+    int64_t ldd;
+    int M, N, K;
+};
+
+// One wavefront per 16 x 16 outputs.  Lane l holds one group of row l & 15:
+// the weight rows are the matrix instruction's first operand, so that a lane's
+// four results are neighbours in an output row.
+__global__ __launch_bounds__(64) void mxfp4_gemm_simple_kernel(const MxGemmArgs p) {
+    const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+    // rows past the end repeat the last one; their results are not stored
+    const int64_t n = min(n0 + r, p.N - 1), m = min(m0 + r, p.M - 1);
+    const uint8_t *w = p.W + n * p.ldw + g * 16, *a = p.A + m * p.lda + g * 16;
+    const uint8_t *sw = p.sW + n * p.ld_sw + g, *sa = p.sA + m * p.ld_sa + g;
+    v4f acc = {};
+    for (int k = 0; k < p.K; k += 128) {
+        const u32x4 wq = *reinterpret_cast<const u32x4*>(w + k / 2), aq = *reinterpret_cast<const u32x4*>(a + k / 2);
+        const v8i wv = {(int)wq.x, (int)wq.y, (int)wq.z, (int)wq.w}, av = {(int)aq.x, (int)aq.y, (int)aq.z, (int)aq.w};
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc, 4, 4, 0, (int)sw[k / 32], 0, (int)sa[k / 32]);
+    }
+    if (m0 + r >= p.M) return;
+    uint16_t* d = p.D + (int64_t)(m0 + r) * p.ldd;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int col = n0 + g * 4 + i;
+        if (col < p.N) d[col] = __builtin_bit_cast(uint16_t, (__bf16)acc[i]);
+    }
+}
+
+static int gemm_launch(const MxGemmArgs& p, hipStream_t st) {
+    mxfp4_gemm_simple_kernel<<<dim3((p.N + 15) / 16, (p.M + 15) / 16), 64, 0, st>>>(p);
+    KBN_CHECK_LAUNCH("mxfp4_gemm_nt");
+    return 0;
+}
+
+static int check_rows(const char* what, const char* name, int64_t ld, int64_t least, int64_t multiple, const void* ptr,
+                      int64_t align) {
+    KBN_CHECK_ARG(ld >= least && ld % multiple == 0, "%s: %s row stride %lld must be a multiple of %lld and at least %lld", what,
+                  name, (long long)ld, (long long)multiple, (long long)least);
+    KBN_CHECK_ARG(ptr && reinterpret_cast<uintptr_t>(ptr) % align == 0, "%s: %s must be %lld-byte aligned", what, name,
+                  (long long)align);
+    return 0;
+}
+
+static int quant_args(const char* what, int dtype, int64_t M, int64_t K) {
+    KBN_CHECK_ARG(dtype >= 0 && dtype <= 2, "%s: unknown dtype code %d", what, dtype);
+    KBN_CHECK_ARG(M >= 0 && K >= 0 && M < (1LL << 31) && K < (1LL << 31), "%s: bad size M=%lld K=%lld", what, (long long)M,
+                  (long long)K);
+    KBN_CHECK_ARG(K % kMxGroup == 0, "%s: K=%lld must be a multiple of %d", what, (long long)K, kMxGroup);
+    return 0;
+}
+
+static int quant_launch(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_c,
+                        void* scales, int64_t ld_s, hipStream_t st) {
+    auto* const kernel = x_dtype == kMxBf16 ? mxfp4_quant_kernel<kMxBf16>
+                         : x_dtype == kMxF16 ? mxfp4_quant_kernel<kMxF16> : mxfp4_quant_kernel<kMxF32>;
+    kernel<<<quant_grid(M, K), kQuantThreads, 0, st>>>(x, ld_x, M, K, (uint8_t*)codes, ld_c, (uint8_t*)scales, ld_s);
+    KBN_CHECK_LAUNCH("mxfp4_quant");
+    return 0;
+}
+
+static int gemm_args(const char* what, int64_t M, int64_t N, int64_t K) {
+    KBN_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31),
+                  "%s: bad size M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+    KBN_CHECK_ARG(K % 128 == 0, "%s: K=%lld must be a multiple of 128", what, (long long)K);
+    return 0;
+}
+
+}  // namespace kbn
+
+using namespace kbn;
+
+extern "C" int kbn_mxfp4_quant(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_codes,
+                               void* scales, int64_t ld_scales, void* stream) {
+    const char* what = "mxfp4_quant";
+    if (quant_args(what, x_dtype, M, K)) return 1;
+    if (M == 0 || K == 0) return 0;
+    if (check_rows(what, "input", ld_x, K, 8, x, 16) || check_rows(what, "codes", ld_codes, K / 2, 4, codes, 4) ||
+        check_rows(what, "scales", ld_scales, K / kMxGroup, 1, scales, 1))
+        return 1;
+    return quant_launch(x, x_dtype, M, K, ld_x, codes, ld_codes, scales, ld_scales, (hipStream_t)stream);
+}
+
+extern "C" int kbn_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t M, int64_t K,
+                                 void* out, int out_dtype, int64_t ld_out, void* stream) {
+    const char* what = "mxfp4_dequant";
+    if (quant_args(what, out_dtype, M, K)) return 1;
+    if (M == 0 || K == 0) return 0;
+    if (check_rows(what, "codes", ld_codes, K / 2, 4, codes, 4) ||
+        check_rows(what, "scales", ld_scales, K / kMxGroup, 1, scales, 1) || check_rows(what, "output", ld_out, K, 8, out, 16))
+        return 1;
+    auto* const kernel = out_dtype == kMxBf16 ? mxfp4_dequant_kernel<kMxBf16>
+                         : out_dtype == kMxF16 ? mxfp4_dequant_kernel<kMxF16> : mxfp4_dequant_kernel<kMxF32>;
+    kernel<<<quant_grid(M, K), kQuantThreads, 0, (hipStream_t)stream>>>((const uint8_t*)codes, ld_codes, (const uint8_t*)scales,
+                                                                       ld_scales, M, K, out, ld_out);
+    KBN_CHECK_LAUNCH(what);
+    return 0;
+}
+
+extern "C" int64_t kbn_mxfp4_gemm_nt_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+
+extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int64_t ld_sa, const void* W, int64_t ldw,
+                                 const void* sW, int64_t ld_sw, void* D, int64_t ldd, int64_t M, int64_t N, int64_t K,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* what = "mxfp4_gemm_nt";
+    if (gemm_args(what, M, N, K)) return 1;
+    if (M == 0 || N == 0) return 0;
+    if (check_rows(what, "A", lda, K / 2, 16, A, 16) || check_rows(what, "A scales", ld_sa, K / kMxGroup, 4, sA, 4) ||
+        check_rows(what, "W", ldw, K / 2, 16, W, 16) || check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4) ||
+        check_rows(what, "output", ldd, N, 1, D, 2))
+        return 1;
+    const int64_t need = kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
+    KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
+                  what, (long long)need, (long long)workspace_bytes);
+    const MxGemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)sA, ld_sa, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw,
+                       (uint16_t*)D, ldd, (int)M, (int)N, (int)K};
+    return gemm_launch(p, (hipStream_t)stream);
+}
+
+// x -> codes and scales in the workspace -> product
+static int64_t linear_operand_bytes(int64_t M, int64_t K) { return (M * (K / 2 + K / kMxGroup) + 255) / 256 * 256; }
+
+extern "C" int64_t kbn_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype) {
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
+    return linear_operand_bytes(M, K) + kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
+}
+
+extern "C" int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const void* W, int64_t ldw, const void* sW,
+                                int64_t ld_sw, void* D, int64_t ldd, int64_t M, int64_t N, int64_t K, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+    const char* what = "mxfp4_linear";
+    if (quant_args(what, x_dtype, M, K) || gemm_args(what, M, N, K)) return 1;
+    if (M == 0 || N == 0) return 0;
+    if (check_rows(what, "input", ld_x, K, 8, x, 16) || check_rows(what, "W", ldw, K / 2, 16, W, 16) ||
+        check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4) || check_rows(what, "output", ldd, N, 1, D, 2))
+        return 1;
+    const int64_t need = kbn_mxfp4_linear_workspace_bytes(M, N, K, x_dtype);
+    KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
+                  what, (long long)need, (long long)workspace_bytes);
+    uint8_t *codes = (uint8_t*)workspace, *scales = codes + M * (K / 2), *rest = codes + linear_operand_bytes(M, K);
+    (void)rest;
+    if (const int rc = quant_launch(x, x_dtype, M, K, ld_x, codes, K / 2, scales, K / kMxGroup, (hipStream_t)stream)) return rc;
+    const MxGemmArgs p{codes, K / 2, scales, K / kMxGroup, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw, (uint16_t*)D, ldd,
+                       (int)M, (int)N, (int)K};
+    return gemm_launch(p, (hipStream_t)stream);
+}
