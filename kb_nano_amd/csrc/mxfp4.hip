@@ -1,13 +1,11 @@
-// MXFP4 quantization and back, and the product of two MXFP4 operands
-//   D[m, n] = bf16( sum_g 2^(ea[m,g] + ew[n,g] - 254) sum_{k in g} a[m,k] w[n,k] ),
-// sums in fp32.
-#include "mxfp4.h"
+// MXFP4 quantization and back, and the C entries of the format: these two, the
+// product (mxfp4_gemm.hip) and the linear that chains them.
+#include "mxfp4_gemm.h"
 
 #include <algorithm>
 
 namespace kbn {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------ quant ---
@@ -70,57 +68,12 @@ static dim3 quant_grid(int64_t M, int64_t K) {
     return dim3((unsigned)((K / 8 + kQuantThreads - 1) / kQuantThreads), (unsigned)std::min<int64_t>(M, 32768));
 }
 
-// ---------------------------------------------------------------- product ---
-
-struct MxGemmArgs {
-    const uint8_t* A;    // codes [M, K/2]
-    int64_t lda;
-    const uint8_t* sA;   // scale bytes [M, K/32]
-    int64_t ld_sa;
-    const uint8_t* W;
-    int64_t ldw;
-    const uint8_t* sW;
-    int64_t ld_sw;
-    uint16_t* D;
-    int64_t ldd;
-    int M, N, K;
-};
-
-// One wavefront per 16 x 16 outputs.  Lane l holds one group of row l & 15:
-// the weight rows are the matrix instruction's first operand, so that a lane's
-// four results are neighbours in an output row.
-__global__ __launch_bounds__(64) void mxfp4_gemm_simple_kernel(const MxGemmArgs p) {
-    const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-    // rows past the end repeat the last one; their results are not stored
-    const int64_t n = min(n0 + r, p.N - 1), m = min(m0 + r, p.M - 1);
-    const uint8_t *w = p.W + n * p.ldw + g * 16, *a = p.A + m * p.lda + g * 16;
-    const uint8_t *sw = p.sW + n * p.ld_sw + g, *sa = p.sA + m * p.ld_sa + g;
-    v4f acc = {};
-    for (int k = 0; k < p.K; k += 128) {
-        const u32x4 wq = *reinterpret_cast<const u32x4*>(w + k / 2), aq = *reinterpret_cast<const u32x4*>(a + k / 2);
-        const v8i wv = {(int)wq.x, (int)wq.y, (int)wq.z, (int)wq.w}, av = {(int)aq.x, (int)aq.y, (int)aq.z, (int)aq.w};
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, acc, 4, 4, 0, (int)sw[k / 32], 0, (int)sa[k / 32]);
-    }
-    if (m0 + r >= p.M) return;
-    uint16_t* d = p.D + (int64_t)(m0 + r) * p.ldd;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int col = n0 + g * 4 + i;
-        if (col < p.N) d[col] = __builtin_bit_cast(uint16_t, (__bf16)acc[i]);
-    }
-}
-
-static int gemm_launch(const MxGemmArgs& p, hipStream_t st) {
-    mxfp4_gemm_simple_kernel<<<dim3((p.N + 15) / 16, (p.M + 15) / 16), 64, 0, st>>>(p);
-    KBN_CHECK_LAUNCH("mxfp4_gemm_nt");
-    return 0;
-}
-
 static int check_rows(const char* what, const char* name, int64_t ld, int64_t least, int64_t multiple, const void* ptr,
                       int64_t align) {
     KBN_CHECK_ARG(ld >= least && ld % multiple == 0, "%s: %s row stride %lld must be a multiple of %lld and at least %lld", what,
                   name, (long long)ld, (long long)multiple, (long long)least);
+    // a tile's row offsets are 32-bit
+    KBN_CHECK_ARG(ld < (1LL << 31) / 256, "%s: %s row stride %lld is too large", what, name, (long long)ld);
     KBN_CHECK_ARG(ptr && reinterpret_cast<uintptr_t>(ptr) % align == 0, "%s: %s must be %lld-byte aligned", what, name,
                   (long long)align);
     return 0;
@@ -181,7 +134,10 @@ extern "C" int kbn_mxfp4_dequant(const void* codes, int64_t ld_codes, const void
     return 0;
 }
 
-extern "C" int64_t kbn_mxfp4_gemm_nt_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+extern "C" int64_t kbn_mxfp4_gemm_nt_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
+    return mxfp4_plan_bytes(mxfp4_plan(M, N, K), M, N);
+}
 
 extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int64_t ld_sa, const void* W, int64_t ldw,
                                  const void* sW, int64_t ld_sw, void* D, int64_t ldd, int64_t M, int64_t N, int64_t K,
@@ -196,16 +152,18 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int
     const int64_t need = kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
     KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
                   what, (long long)need, (long long)workspace_bytes);
-    const MxGemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)sA, ld_sa, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw,
-                       (uint16_t*)D, ldd, (int)M, (int)N, (int)K};
-    return gemm_launch(p, (hipStream_t)stream);
+    MxGemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)sA, ld_sa, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw,
+                 (uint16_t*)D, ldd, (int)M, (int)N, (int)K};
+    return mxfp4_gemm_launch(p, (float*)workspace, (hipStream_t)stream);
 }
 
-// x -> codes and scales in the workspace -> product
+// x -> codes and scales in the workspace -> product; one or two rows of 16-bit
+// values: in one launch, without them (1 x 10240 x 8192 12.7 us against 13.6)
+static bool linear_fused(int64_t M, int x_dtype) { return M <= kMxFusedRows && x_dtype != kMxF32; }
 static int64_t linear_operand_bytes(int64_t M, int64_t K) { return (M * (K / 2 + K / kMxGroup) + 255) / 256 * 256; }
 
 extern "C" int64_t kbn_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || linear_fused(M, x_dtype)) return 0;
     return linear_operand_bytes(M, K) + kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
 }
 
@@ -221,10 +179,15 @@ extern "C" int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const 
     const int64_t need = kbn_mxfp4_linear_workspace_bytes(M, N, K, x_dtype);
     KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
                   what, (long long)need, (long long)workspace_bytes);
+    if (linear_fused(M, x_dtype)) {
+        MxGemmArgs p{nullptr, ld_x, nullptr, 0, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw, (uint16_t*)D, ldd,
+                     (int)M, (int)N, (int)K};
+        p.X = x;
+        return mxfp4_rows_launch(p, mxfp4_plan(M, N, K).rf, x_dtype, (hipStream_t)stream);
+    }
     uint8_t *codes = (uint8_t*)workspace, *scales = codes + M * (K / 2), *rest = codes + linear_operand_bytes(M, K);
-    (void)rest;
     if (const int rc = quant_launch(x, x_dtype, M, K, ld_x, codes, K / 2, scales, K / kMxGroup, (hipStream_t)stream)) return rc;
-    const MxGemmArgs p{codes, K / 2, scales, K / kMxGroup, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw, (uint16_t*)D, ldd,
-                       (int)M, (int)N, (int)K};
-    return gemm_launch(p, (hipStream_t)stream);
+    MxGemmArgs p{codes, K / 2, scales, K / kMxGroup, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw, (uint16_t*)D, ldd,
+                 (int)M, (int)N, (int)K};
+    return mxfp4_gemm_launch(p, (float*)rest, (hipStream_t)stream);
 }

@@ -1,0 +1,358 @@
+// Product of two MXFP4 operands,
+//   D[m, n] = bf16( sum_g 2^(ea[m,g] + ew[n,g] - 254) sum_{k in g} a[m,k] w[n,k] ),
+// on v_mfma_scale_f32_32x32x64_f8f6f4: a lane's operand is one scale group (32
+// codes, 16 bytes) of one row and the instruction takes the group's scale byte,
+// so scales cost no arithmetic.
+//
+// Tiled kernel: four wavefronts compute a BM x BN tile, (BM/2) x (BN/2) each.
+// Codes go from memory to LDS by direct loads in a ring of kStages stages of
+// 256 K (128 bytes a row: whole lines, as the L2 serves a half line in the time
+// of a whole one, 67 against 133 B/ns for each CU when all read shared data).
+// Scale bytes have two buffers of 512 K, one 16-byte load per row.  A stage is
+// four steps of 64 K: while one is multiplied the fragments of the next are
+// read, in the first slots, so that they have landed when they are needed; the
+// one barrier of a stage comes after its third step, where all of the stage
+// has been read: it frees the stage for the loads of the one kStages ahead, one
+// in each MFMA slot of the fourth step.
+#include "mxfp4_gemm.h"
+
+#include "gemm_kernel.h"
+
+namespace kbn {
+
+constexpr int kMxStageK = 256, kMxScaleK = 512;
+
+template <int BM, int BN, int kStages, int kPerCu>
+__global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArgs p) {
+    constexpr int kRows = BM + BN, kStage = kRows * 128, kScale = kRows * 16, kScaleAt = kStages * kStage;
+    constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 32, FN = TN / 32;
+    constexpr int kDma = kRows / 32;                            // loads of a wavefront per stage: 8 rows each
+    constexpr int kScaleDma = kRows >= 256 ? kRows / 256 : 1;   // and per 512 K of scales: 64 rows each
+    static_assert(BM % 64 == 0 && BN % 64 == 0 && BM * BN * 2 <= kScaleAt, "epilogue");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kScaleAt + 2 * kScale];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+
+    int tm, tn, trel, split;
+    tile_coords<8>(p.tiles_m, p.tiles_n, 0, p.splits, tm, tn, trel, split);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int k_from = split * p.groups_per_split * kMxScaleK;
+    const int k_len = min(p.K, k_from + p.groups_per_split * kMxScaleK) - k_from;
+    // The loop has no branches (with one the 256x256 tile's accumulators move
+    // between register files): it runs pairs of stages, and what lies past
+    // k_len reads as codes and scale bytes of 0, which add nothing.
+    const int pairs = (k_len + kMxScaleK - 1) / kMxScaleK, whole = k_len / kMxStageK;
+
+    // rows past the operand's last read as zeros
+    const int rows_a = min(p.M - m0, BM), rows_w = min(p.N - n0, BN);
+    const v4i dA = make_desc(p.A + (int64_t)m0 * p.lda + k_from / 2, (rows_a - 1) * p.lda + k_len / 2);
+    const v4i dW = make_desc(p.W + (int64_t)n0 * p.ldw + k_from / 2, (rows_w - 1) * p.ldw + k_len / 2);
+    const v4i dsA = make_desc(p.sA + (int64_t)m0 * p.ld_sa + k_from / 32, (rows_a - 1) * p.ld_sa + k_len / 32);
+    const v4i dsW = make_desc(p.sW + (int64_t)n0 * p.ld_sw + k_from / 32, (rows_w - 1) * p.ld_sw + k_len / 32);
+
+    // Load j of this wavefront: rows 8 q .. 8 q + 7 of the stage, q = 4 j + wave.
+    // 16-byte chunk c of row r lies in slot c ^ swz(r) (the swizzle is applied
+    // to the address read, a load's LDS side is contiguous).
+    int voff[kDma];
+#pragma unroll
+    for (int j = 0; j < kDma; ++j) {
+        const int r = (4 * j + wave) * 8 + (lane >> 3), chunk = (lane & 7) ^ swz(r);
+        voff[j] = (j < BM / 32 ? r * (int)p.lda : (r - BM) * (int)p.ldw) + chunk * 16;
+    }
+    int svoff[kScaleDma];
+#pragma unroll
+    for (int j = 0; j < kScaleDma; ++j) {
+        const int r = ((4 * j + wave) * 64 + lane) % kRows;   // 128 or 192 rows: some load the same as another wavefront
+        svoff[j] = r < BM ? r * (int)p.ld_sa : (r - BM) * (int)p.ld_sw;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem, lds = lds0 + (uint32_t)wave * 1024u;
+
+    // Loads of stages past the last fall outside an empty range; in a half stage
+    // the lanes of the chunks behind k_len (the same for every j, whose rows
+    // differ by multiples of 32) fall outside as well.
+    const int behind = ((lane & 7) ^ swz(wave * 8 + (lane >> 3))) >= 4 ? kOob : 0;
+    auto issue = [&](uint32_t base, auto j_, int s) {
+        constexpr int j = decltype(j_)::value;
+        v4i d = j < BM / 32 ? dA : dW;
+        if (s * kMxStageK >= k_len) d[2] = 0;
+        dma_b128<j * 4096, false>(d, base, voff[j] | (s == whole ? behind : 0), s * 128);
+    };
+    auto issue_scales = [&](int o) {
+        static_for<kScaleDma>([&](auto j_) {
+            constexpr int j = decltype(j_)::value;
+            // the 64 rows of one load lie in one operand (BM is a multiple of 64)
+            const int q = (4 * j + wave) % (kRows / 64);
+            v4i d = q < BM / 64 ? dsA : dsW;
+            if (o * kMxScaleK >= k_len) d[2] = 0;
+            dma_b128<kScaleAt, false>(d, lds0 + (uint32_t)(o & 1) * kScale + (uint32_t)q * 1024u, svoff[j], o * 16);
+        });
+    };
+
+    // fragment f (A: f < FM, W: f - FM) of step ks of the stage at LDS offset `at`
+    const int half = lane >> 5, ra = wm * TM + (lane & 31), rw = BM + wn * TN + (lane & 31);
+    auto read_frag = [&](int at, int ks, int f) -> u32x4 {
+        const int r = f < FM ? ra : rw;   // the swizzle is the same 32 rows on
+        return *reinterpret_cast<const u32x4*>(smem + at + r * 128 + (((2 * ks + half) ^ swz(r)) << 4) + (f < FM ? f : f - FM) * 4096);
+    };
+    auto read_scale = [&](int o, int f) -> u32x4 {
+        return *reinterpret_cast<const u32x4*>(smem + kScaleAt + (o & 1) * kScale + (f < FM ? ra : rw) * 16 + (f < FM ? f : f - FM) * 512);
+    };
+
+    v16f acc[FM][FN] = {};
+    constexpr int kR = FM + FN, kT = FM * FN;
+    u32x4 f0[kR], f1[kR], raw[kR];
+    uint32_t sc[kR][4];   // dword: 128 K of the 512; byte 0 for the first 64 of them, byte 2 for the second
+    auto mfma_at = [&](int t, const u32x4 (&f)[kR], auto step_) {   // step of 64 K within the 512
+        constexpr int step = decltype(step_)::value, op = (step & 1) * 2;
+        const int i = t / FN, j = t % FN;
+        const v8i a = {(int)f[i].x, (int)f[i].y, (int)f[i].z, (int)f[i].w}, w = {(int)f[FM + j].x, (int)f[FM + j].y, (int)f[FM + j].z, (int)f[FM + j].w};
+        // W as the first operand: a lane then holds runs of four columns of one row
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, acc[i][j], 4, 4, op, (int)sc[FM + j][step >> 1], op,
+                                                                      (int)sc[i][step >> 1]);
+        keep_here<BM + BN == 512>(acc[i][j][0]);
+    };
+
+    // in the loop's order: an odd stage issues the next but one scales ahead of its codes
+    issue_scales(0);
+    static_for<kStages>([&](auto b_) {
+        if constexpr (decltype(b_)::value == kStages - 1) issue_scales(1);
+        static_for<kDma>([&](auto j_) { issue(lds + decltype(b_)::value * kStage, j_, decltype(b_)::value); });
+    });
+    wait_dma_n<(kStages - 1) * kDma + kScaleDma>();
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < kR; ++f) {
+        f0[f] = read_frag(0, 0, f);
+        raw[f] = read_scale(0, f);
+    }
+    constexpr int kAt = kT >= 2 * kR ? 1 : (2 * kR + kT - 1) / kT;   // reads in a slot
+    // step ks (0 .. 2) of a stage at `at`, and the next one's reads
+    auto step = [&](auto par_, auto ks_, int at) {
+        constexpr int ks = decltype(ks_)::value;
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            mfma_at(t, ks & 1 ? f1 : f0, std::integral_constant<int, 4 * decltype(par_)::value + ks>{});
+#pragma unroll
+            for (int f = t * kAt; f < (t + 1) * kAt && f < kR; ++f) (ks & 1 ? f0 : f1)[f] = read_frag(at, ks + 1, f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int at = 0;   // LDS offset of the current stage
+    auto stage = [&](auto par_, int s) {
+        constexpr int par = decltype(par_)::value;
+        step(par_, std::integral_constant<int, 0>{}, at);
+        step(par_, std::integral_constant<int, 1>{}, at);
+        step(par_, std::integral_constant<int, 2>{}, at);
+        // stage s + 1 has landed, for odd s the next scales too; in flight
+        // behind it: kStages - 2 stages and, for even s, the scales issued
+        // just before the last of them
+        wait_dma_n<(kStages - 2) * kDma + (par == 0 && kStages > 2 ? kScaleDma : 0)>();
+        wait_lds();
+        __syncthreads();
+        if constexpr (par == 1) issue_scales(s / 2 + 2);
+        const int here = at;
+        at = at == (kStages - 1) * kStage ? 0 : at + kStage;
+        const uint32_t base = lds + (uint32_t)here;
+        static_for<kT>([&](auto t_) {
+            constexpr int t = decltype(t_)::value;
+            mfma_at(t, f1, std::integral_constant<int, 4 * par + 3>{});
+#pragma unroll
+            for (int f = t * kAt; f < (t + 1) * kAt && f < kR; ++f) {
+                f0[f] = read_frag(at, 0, f);
+                if constexpr (par == 1) raw[f] = read_scale(s / 2 + 1, f);
+            }
+            constexpr int u0 = t * kDma / kT, u1 = (t + 1) * kDma / kT;
+            static_for<u1 - u0>([&](auto u_) { issue(base, std::integral_constant<int, u0 + decltype(u_)::value>{}, s + kStages); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    for (int o = 0; o < pairs; ++o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // bytes behind k_len are another row's, perhaps a NaN's
+            const uint32_t m = o * kMxScaleK + i * 128 < k_len ? ~0u : 0u;
+#pragma unroll
+            for (int f = 0; f < kR; ++f) sc[f][i] = (raw[f][i] & m) >> (8 * half);
+        }
+        stage(std::integral_constant<int, 0>{}, 2 * o);
+        stage(std::integral_constant<int, 1>{}, 2 * o + 1);
+    }
+    wait_dma();        // the loads past the end still write to this workgroup's LDS
+    __syncthreads();
+
+    if (p.splits > 1) {
+        float* slab = p.P + ((int64_t)split * p.tiles_m * p.tiles_n + trel) * (BM * BN);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int r = wm * TM + i * 32 + (lane & 31);
+            if (m0 + r >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = wn * TN + j * 32 + 8 * q + 4 * half;
+                    *reinterpret_cast<u32x4*>(slab + r * BN + c) =
+                        u32x4{__float_as_uint(acc[i][j][4 * q]), __float_as_uint(acc[i][j][4 * q + 1]),
+                              __float_as_uint(acc[i][j][4 * q + 2]), __float_as_uint(acc[i][j][4 * q + 3])};
+                }
+        }
+        return;
+    }
+    // bf16 through LDS, so that rows leave as whole lines: each wavefront parks
+    // its block row-major, 16-byte chunks rotated by the row (no two of the 32
+    // rows written at once then share more than their fair share of banks)
+    constexpr int kCh = TN / 8, kRowsPer = 64 / kCh;
+    uint8_t* reg = smem + wave * (TM * TN * 2);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int r = i * 32 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<u32x2*>(reg + r * (TN * 2) + ((4 * j + q + r) % kCh) * 16 + 8 * half) =
+                    u32x2{pack_bf16(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+        __builtin_amdgcn_sched_barrier(0);   // one fragment row's registers at a time
+    }
+    wait_lds();
+    const bool lines = p.N % 8 == 0 && p.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(p.D) & 15) == 0;
+    const int cl = lane % kCh, n = n0 + wn * TN + cl * 8;
+#pragma unroll 4
+    for (int it = 0; it < TM / kRowsPer; ++it) {
+        const int r = it * kRowsPer + lane / kCh, m = m0 + wm * TM + r;
+        if (m >= p.M) continue;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(reg + r * (TN * 2) + ((cl + r) % kCh) * 16);
+        uint16_t* d = p.D + (int64_t)m * p.ldd + n;
+        if (lines) {
+            if (n < p.N) *reinterpret_cast<u32x4*>(d) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < p.N) d[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+}
+
+// D = bf16 of the splits' partial sums, added in their order; a lane takes four columns.
+template <int BM, int BN>
+__global__ __launch_bounds__(256) void mxfp4_sum_kernel(const MxGemmArgs p) {
+    const int tiles = p.tiles_m * p.tiles_n;
+    constexpr int kRuns = BN / 4;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;   // (tile row of a tile, run of four columns)
+    const int run = (int)(at % kRuns), r = (int)(at / kRuns % BM);
+    const int64_t t = at / (kRuns * BM);
+    if (t >= tiles) return;
+    // the tile order of the product's workgroups, without their XCD placement
+    const int group = 8 * p.tiles_n, g = (int)t / group, first = g * 8, gm = min(p.tiles_m - first, 8), w = (int)t - g * group;
+    const int m = (first + w % gm) * BM + r, n = (w / gm) * BN + run * 4;
+    if (m >= p.M || n >= p.N) return;
+    const float* s = p.P + (t * BM + r) * BN + run * 4;
+    float v[4] = {};
+    for (int i = 0; i < p.splits; ++i) {
+        const u32x4 q = *reinterpret_cast<const u32x4*>(s + (int64_t)i * tiles * (BM * BN));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += __uint_as_float(q[e]);
+    }
+    uint16_t* d = p.D + (int64_t)m * p.ldd + n;
+    if (n + 4 <= p.N && p.ldd % 4 == 0 && (reinterpret_cast<uintptr_t>(p.D) & 7) == 0) {
+        *reinterpret_cast<u32x2*>(d) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < p.N) d[e] = (uint16_t)pack_bf16(v[e], 0.0f);
+    }
+}
+
+template <int BM, int BN, int kStages, int kPerCu>
+static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStream_t st) {
+    p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = (p.N + BN - 1) / BN;
+    const int groups = (p.K + kMxScaleK - 1) / kMxScaleK;
+    p.groups_per_split = (groups + plan.splits - 1) / plan.splits;
+    p.splits = (groups + p.groups_per_split - 1) / p.groups_per_split;
+    p.P = slabs;
+    mxfp4_gemm_kernel<BM, BN, kStages, kPerCu><<<p.tiles_m * p.tiles_n * p.splits, 256, 0, st>>>(p);
+    KBN_CHECK_LAUNCH("mxfp4_gemm_nt");
+    if (p.splits > 1) {
+        const int64_t lanes = (int64_t)p.tiles_m * p.tiles_n * BM * (BN / 4);
+        mxfp4_sum_kernel<BM, BN><<<(unsigned)((lanes + 255) / 256), 256, 0, st>>>(p);
+        KBN_CHECK_LAUNCH("mxfp4_gemm_nt");
+    }
+    return 0;
+}
+
+// Prices, in us, of the tiles: fixed cost, a further round of workgroups, a
+// stage of 256 K where each CU has one workgroup, one where it has several (a
+// workgroup's share), fitted to 252 shapes (M 40 .. 2048, seven weights) and
+// split counts timed in graphs; 10% off, and the tile picked is 2% slower than
+// the best one, on average.  Each tile carries shapes: 777 x 4608 x 7168 takes
+// 24.5 us with 128x128 against 26.4 and 49, 4096 x 36864 x 7168 579 with 256x256
+// against 719 and 985, 320 x 1000 x 4096 8.2 with 64x64 against 9.5 and 15,
+// 65 x 24576 x 1536 8.9 with 64x128 against 10.4 with 64x64.
+struct TilePrice {
+    int bm, bn, per_cu;
+    double fixed, round, stage_one, stage_many;
+};
+static const TilePrice kTiles[] = {
+    {64, 64, 2, 3.2, 1.1, 0.33, 0.30},
+    {64, 128, 2, 2.7, 0.6, 0.49, 0.47},
+    {128, 128, 2, 2.3, 0.36, 0.76, 0.69},
+    {256, 256, 1, 6.8, 8.1, 1.47, 1.75},
+};
+constexpr double kSplitFixed = 3.0, kSplitMb = 0.35;   // the sum's launch, and each MB of partial sums
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t groups = ceil_div(K, kMxScaleK), cus = cu_count();
+    MxPlan best{};
+    double price = 1e30;
+    if (M <= 64) {
+        // The few-rows kernel is bound by what each CU reads: 16 (rf + cg) rows
+        // of codes a workgroup, about 33 B/ns a CU; K in pairs of stages of
+        // each wavefront.  M = 64: 2048 x 2048 4.7 / 5.3 / 7.0 us with rf 1 / 2 / 4,
+        // 8192 x 8192 18.9 / 13.3 / 17.0, 10240 x 8192 26.1 / 21.1 / 18.4.
+        const int64_t cg = ceil_div(M, 16), stages = 8 * ceil_div(ceil_div(K, 256), 8);
+        for (int rf = 1; rf <= 4; rf *= 2) {
+            const int64_t rounds = ceil_div(ceil_div(N, 16 * rf), cus);
+            const double t = 2.7 + 1.5 * (rounds - 1) + 0.0039 * 16 * (rf + cg) * stages * rounds;
+            if (t < price) {
+                price = t;
+                best = {0, 0, 1, rf};
+            }
+        }
+        if (M <= 16) return best;
+    }
+    for (const TilePrice& t : kTiles) {
+        const int64_t tiles_m = ceil_div(M, t.bm), tiles = tiles_m * ceil_div(N, t.bn);
+        for (int splits = 1; splits <= 4 && splits <= groups; ++splits) {
+            const int64_t per = ceil_div(groups, splits), used = ceil_div(groups, per);
+            if (used != splits) continue;
+            const int64_t q = ceil_div(tiles * splits, cus), stages = 2 * per;
+            // one row of tiles: every weight line comes from memory
+            const double cold = tiles_m == 1 ? 1.4 : 1.0;
+            double us = t.fixed + t.round * (ceil_div(q, t.per_cu) - 1) +
+                        cold * (q == 1 ? t.stage_one * stages : t.stage_many * stages * q);
+            if (splits > 1) us += kSplitFixed + kSplitMb * 4e-6 * (double)(tiles * t.bm * t.bn * splits);
+            if (us < price) {
+                price = us;
+                best = {t.bm, t.bn, splits, 0};
+            }
+        }
+    }
+    return best;
+}
+
+int64_t mxfp4_plan_bytes(const MxPlan& p, int64_t M, int64_t N) {
+    return p.rf || p.splits == 1 ? 0 : ceil_div(M, p.bm) * ceil_div(N, p.bn) * p.bm * p.bn * 4 * p.splits;
+}
+
+int mxfp4_gemm_launch(MxGemmArgs& p, float* slabs, hipStream_t st) {
+    const MxPlan plan = mxfp4_plan(p.M, p.N, p.K);
+    if (plan.rf) return mxfp4_rows_launch(p, plan.rf, kMxBf16, st);
+    if (plan.bm == 256) return launch_tiled<256, 256, 2, 1>(p, plan, slabs, st);
+    if (plan.bm == 128) return launch_tiled<128, 128, 2, 2>(p, plan, slabs, st);
+    if (plan.bn == 128) return launch_tiled<64, 128, 3, 2>(p, plan, slabs, st);
+    return launch_tiled<64, 64, 4, 2>(p, plan, slabs, st);
+}
+
+}  // namespace kbn
