@@ -8,21 +8,22 @@
 // At these sizes the layer is the time to stream each named expert's weights
 // once, so the activations are not quantized: weight codes widen exactly to
 // bf16 (an MXFP4 code with its power-of-two scale too) and run through the
-// bf16 matrix instruction, 16 weight rows by 16 tokens, sums in fp32.  FP8
-// block scales multiply each 128-K block's fp32 sum.  An operand with more
+// bf16 matrix instruction, 16 weight rows by 16 activation rows, sums in fp32.
+// FP8 block scales multiply each 128-K block's fp32 sum.  An operand with more
 // than bf16's 8 significant bits (fp16 activations, and h, which has fp32's)
 // goes as a pair of bf16 values, x = hi + lo, hi the nearest and lo the
 // nearest to the rest: 16 bits and more, for one more matrix instruction on
-// operands that are there already.
+// weights that are there already.
 //
-// A token is a column: lane l of a 16-column group serves token 16 group +
-// (l & 15), and an expert's columns of other tokens read as zeros.  The down
-// kernel owns 16 output columns of every token over all experts, so the sum
-// over experts stays in registers, in a fixed order.
+// Both kernels stream like the few-rows MXFP4 product: each wavefront has a
+// private LDS ring filled by direct loads of whole 128-byte weight lines (a
+// stage: 128 K of FP8, 256 K of MXFP4, and the activations of that K), no
+// barrier in the loop.  An expert's tokens are taken kR at a time, a pass; one
+// pass is the rule (2 tokens an expert at 64 tokens and 256 experts with 8 a
+// token), and further ones find the weights in L2.
 #include "mxfp4.h"
 
-#include <algorithm>
-#include <type_traits>
+#include "gemm_kernel.h"
 
 namespace kbn {
 
@@ -33,6 +34,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kMaxTokens = 64, kMaxTopk = 32, kMaxExperts = 1024;
 enum WFormat : int { kWFp8 = 0, kWMxfp4 = 1 };
 
+// A pass of an expert, and a row of one: what the gate/up launch writes down
+// for the down launch.
+struct Pass {
+    uint16_t expert, rows;
+    int first_row;
+};
+struct Row {
+    uint16_t pair, token;   // pair: token * topk + slot
+    float weight;
+};
+
 struct ExpertsArgs {
     const void* x;
     int64_t ld_x;
@@ -42,7 +54,10 @@ struct ExpertsArgs {
     int id64;
     const float* weights;
     int T, H, I, E, topk;
-    uint16_t* h;               // hi then lo, each [T * topk, I]; row t * topk + first slot of the expert
+    int* count;                // passes
+    Pass* passes;              // [T * topk]
+    Row* rows;                 // [T * topk]
+    uint16_t* h;               // [T * topk][I / 128][hi 128, lo 128]; row t * topk + first slot of the expert
     void* out;
     int64_t ld_out;
 };
@@ -52,64 +67,26 @@ __device__ __forceinline__ int expert_of(const ExpertsArgs& p, int pair) {
     return e >= 0 && e < p.E ? (int)e : -1;
 }
 
-// First slot of token t that names expert e (-1: none), and the sum of the
-// weights of all that do.
-__device__ __forceinline__ int find_slot(const int* ids, const float* weights, int topk, int t, int e, float& c) {
-    int slot = -1;
-    c = 0.0f;
-    for (int j = 0; j < topk; ++j)
-        if (ids[t * topk + j] == e) {
-            c += weights[t * topk + j];
-            if (slot < 0) slot = j;
-        }
-    return slot;
-}
-
-// 128 K of 16 weight rows: lane (row l & 15, part l >> 4).
-//   FP8: the lane holds k = 64 j + 16 part .. + 15 for j = 0, 1;
-//   MXFP4: k = 32 part .. + 31, one scale group.
+// The i-th eight values of a lane's 16 bytes of weight codes (FP8: i < 2,
+// MXFP4: i < 4), in bf16 (exact); byte: the MXFP4 group's scale.
 template <int kW>
-struct WFrag {
-    u32x4 q[kW == kWFp8 ? 2 : 1];
-    uint32_t byte;   // MXFP4
-};
-template <int kW>
-__device__ __forceinline__ WFrag<kW> load_w(const uint8_t* row, const uint8_t* srow, int k, int part) {
-    WFrag<kW> f;
-    if constexpr (kW == kWFp8) {
-        f.q[0] = *reinterpret_cast<const u32x4*>(row + k + 16 * part);
-        f.q[1] = *reinterpret_cast<const u32x4*>(row + k + 64 + 16 * part);
-        f.byte = 0;
-    } else {
-        f.q[0] = *reinterpret_cast<const u32x4*>(row + k / 2 + 16 * part);
-        f.byte = srow[k / 32 + part];
-    }
-    return f;
-}
-// The i-th (of four) eight values of a fragment, in bf16 (exact).
-template <int kW>
-__device__ __forceinline__ bf16x8 widen_w(const WFrag<kW>& f, int i) {
+__device__ __forceinline__ bf16x8 widen_w(const u32x4& q, int i, uint32_t byte) {
     u32x4 r;
     if constexpr (kW == kWFp8) {
-        const uint32_t a = i & 1 ? f.q[i >> 1].z : f.q[i >> 1].x, b = i & 1 ? f.q[i >> 1].w : f.q[i >> 1].y;
+        const uint32_t a = i ? q.z : q.x, b = i ? q.w : q.y;
         r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
         r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
         r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
         r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
     } else {
-        const float sc = __uint_as_float(f.byte << 23);
-        const uint32_t a = f.q[0][i];
+        const float sc = __uint_as_float(byte << 23);
+        const uint32_t a = q[i];
         r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(a, sc, 0));
         r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(a, sc, 1));
         r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(a, sc, 2));
         r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(a, sc, 3));
     }
     return __builtin_bit_cast(bf16x8, r);
-}
-// K offset, within the 128, of a lane's i-th eight values.
-template <int kW>
-__device__ __forceinline__ int k_of(int i, int part) {
-    return kW == kWFp8 ? 64 * (i >> 1) + 16 * part + 8 * (i & 1) : 32 * part + 8 * i;
 }
 
 __device__ __forceinline__ v4f mfma(bf16x8 a, bf16x8 b, v4f c) {
@@ -131,220 +108,470 @@ __device__ __forceinline__ void split8(f16x8 x, bf16x8& hi, bf16x8& lo) {
     }
 }
 
-// The token ids in LDS: -1 for those that name no expert.
-__device__ __forceinline__ void load_ids(const ExpertsArgs& p, int* ids, float* weights, int tid, int n) {
-    for (int i = tid; i < p.T * p.topk; i += n) {
-        ids[i] = expert_of(p, i);
-        if (weights) weights[i] = p.weights[i];
-    }
+// A uniform load through the scalar cache: it leaves the count of vector loads
+// in flight alone.
+__device__ __forceinline__ float scalar_load(const float* p, int64_t i) {
+    typedef const float __attribute__((address_space(4))) * Const;
+    return ((Const)(uintptr_t)p)[i];
 }
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kDepth = 2;
 
-// Workgroup: 16 rows of h (16 gate and 16 up rows) of one expert, K split over
-// the wavefronts.  slot: a routed pair whose expert no earlier pair names
-// (by_pair), or an expert.
-template <int kW, bool kF16, int kGroups>
-__global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs p, int by_pair) {
-    __shared__ int ids[kMaxTokens * kMaxTopk];
-    __shared__ float red[kWaves][2][kGroups][4][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = lane >> 4, col = lane & 15;
-    const int e = by_pair ? expert_of(p, blockIdx.y) : (int)blockIdx.y;
-    if (e < 0) return;
-    load_ids(p, ids, nullptr, tid, kWaves * 64);
-    __syncthreads();
-    if (by_pair)
-        for (int i = 0; i < (int)blockIdx.y; ++i)
-            if (ids[i] == e) return;   // an earlier pair's workgroup has this expert
-    int slot[kGroups];
-    bool any = false;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        const int t = 16 * g + col;
-        slot[g] = -1;
-        if (t < p.T)
-            for (int j = p.topk - 1; j >= 0; --j)
-                if (ids[t * p.topk + j] == e) slot[g] = j;
-        any |= __ballot(slot[g] >= 0) != 0;
-    }
-    if (!any) return;
-    const int i0 = blockIdx.x * 16, KB = p.H / 128;
-    const int64_t rows = (int64_t)e * 2 * p.I, gr = rows + i0 + col, ur = gr + p.I;
-    const int64_t ldw = kW == kWFp8 ? p.H : p.H / 2, lds = p.H / 32;
-    const uint8_t* const w[2] = {p.w13 + gr * ldw, p.w13 + ur * ldw};
-    const uint8_t* sb[2] = {nullptr, nullptr};
-    const float* sf[2] = {nullptr, nullptr};
-    if constexpr (kW == kWFp8) {
-        const float* s = static_cast<const float*>(p.s13) + (rows / 128) * KB;
-        sf[0] = s + (int64_t)(i0 / 128) * KB;
-        sf[1] = s + (int64_t)((p.I + i0) / 128) * KB;
-    } else {
-        sb[0] = static_cast<const uint8_t*>(p.s13) + gr * lds;
-        sb[1] = static_cast<const uint8_t*>(p.s13) + ur * lds;
-    }
-    v4f acc[2][kGroups] = {};
-    for (int kb = wave; kb < KB; kb += kWaves) {
-        const int k = kb * 128;
-        WFrag<kW> f[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) f[h] = load_w<kW>(w[h], sb[h], k, part);
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            if (__ballot(slot[g] >= 0) == 0) continue;
-            bf16x8 hi[4] = {}, lo[4] = {};
-            if (slot[g] >= 0) {
-                const uint16_t* x = static_cast<const uint16_t*>(p.x) + (int64_t)(16 * g + col) * p.ld_x + k;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(x + k_of<kW>(i, part));
-                    if constexpr (kF16) split8(__builtin_bit_cast(f16x8, v), hi[i], lo[i]);
-                    else hi[i] = __builtin_bit_cast(bf16x8, v);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v4f s = kW == kWFp8 ? v4f{} : acc[h][g];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bf16x8 a = widen_w<kW>(f[h], i);
-                    s = mfma(a, hi[i], s);
-                    if constexpr (kF16) s = mfma(a, lo[i], s);
-                }
-                if constexpr (kW == kWFp8) acc[h][g] += s * sf[h][kb];
-                else acc[h][g] = s;
-            }
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[wave][h][g][i][lane] = acc[h][g][i];
-    __syncthreads();
-    const int64_t pairs = (int64_t)p.T * p.topk;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {   // lane (part, col), register i = wave: row i0 + 4 part + wave of token 16 g + col
-        if (slot[g] < 0) continue;
-        float gate = 0.0f, up = 0.0f;
-#pragma unroll
-        for (int v = 0; v < kWaves; ++v) {
-            gate += red[v][0][g][wave][lane];
-            up += red[v][1][g][wave][lane];
-        }
-        const float y = gate / (1.0f + __expf(-gate)) * up;
-        const int64_t at = ((int64_t)(16 * g + col) * p.topk + slot[g]) * p.I + i0 + 4 * part + wave;
-        const __bf16 hi = (__bf16)y;
-        p.h[at] = __builtin_bit_cast(uint16_t, hi);
-        p.h[pairs * p.I + at] = __builtin_bit_cast(uint16_t, low_part(y, hi));
-    }
-}
+// What a wavefront's stage holds: 16 RF weight rows of 128 bytes, kR activation
+// rows (kRowBytes each) and, for MXFP4, 8 scale bytes a weight row.  Sixteen-byte
+// chunk c of a weight row q lies in slot c ^ swz(q), that of activation row r in
+// slot c ^ (r & 15): no two lanes that read together share a bank.
+template <int kW, int RF, int kR, int kRowBytes>
+struct StageOf {
+    static constexpr int kK = kW == kWFp8 ? 128 : 256;
+    static constexpr int kWLoads = 2 * RF, kXLoads = kR * kRowBytes / 1024, kScaleLoads = kW == kWMxfp4;
+    static constexpr int kLoads = kWLoads + kXLoads + kScaleLoads;
+    static constexpr int kXAt = kWLoads * 1024, kScaleAt = kXAt + kXLoads * 1024, kBytes = kScaleAt + kScaleLoads * 256;
+    static constexpr int kParts = kW == kWFp8 ? 2 : 4;   // matrix instructions per 16 bytes of codes
 
-// Workgroup: 16 output columns of every token; the (expert, 128 K) blocks of
-// the named experts are split into one run for each wavefront.
-template <int kW, bool kF16, int kGroups>
-__global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) {
-    __shared__ int ids[kMaxTokens * kMaxTopk];
-    __shared__ float weights[kMaxTokens * kMaxTopk];
+    // fragment f's codes, half j of the stage's K
+    static __device__ __forceinline__ u32x4 w(const uint8_t* at, int f, int j, int r, int part) {
+        return *reinterpret_cast<const u32x4*>(at + (16 * f + r) * 128 + (((4 * j + part) ^ swz(r)) << 4));
+    }
+    static __device__ __forceinline__ uint32_t scale(const uint8_t* at, int f, int j, int r, int part) {
+        if constexpr (kW == kWFp8) return 0;
+        else return *reinterpret_cast<const uint32_t*>(at + kScaleAt + (16 * f + r) * 8 + 4 * j) >> (8 * part) & 0xFFu;
+    }
+    // chunk c of activation row r (rows past kR: any other, their results go nowhere)
+    static __device__ __forceinline__ u32x4 x(const uint8_t* at, int r, int c) {
+        return *reinterpret_cast<const u32x4*>(at + kXAt + (r % kR) * kRowBytes + ((c ^ (r % kR)) << 4));
+    }
+};
+
+// The routing written down for the down launch: the named experts in order,
+// each one's tokens in order, kR rows a pass.  One workgroup.
+__device__ void write_passes(const ExpertsArgs& p, int kR, int* ids, float* weights) {
     __shared__ uint32_t named[kMaxExperts / 32];
-    __shared__ uint16_t list[kMaxExperts];
-    __shared__ int count;
-    __shared__ float red[kWaves][kGroups][4][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = lane >> 4, col = lane & 15;
-    if (tid < kMaxExperts / 32) named[tid] = 0;
-    load_ids(p, ids, weights, tid, kWaves * 64);
+    __shared__ int list[kMaxExperts], total, sums[2][kWaves];
+    const int tid = threadIdx.x, n = kWaves * 64, pairs = p.T * p.topk;
+    for (int i = tid; i < kMaxExperts / 32; i += n) named[i] = 0;
+    for (int i = tid; i < pairs; i += n) {
+        ids[i] = expert_of(p, i);
+        weights[i] = p.weights[i];
+    }
     __syncthreads();
-    for (int i = tid; i < p.T * p.topk; i += kWaves * 64)
+    for (int i = tid; i < pairs; i += n)
         if (ids[i] >= 0) atomicOr(&named[ids[i] >> 5], 1u << (ids[i] & 31));
     __syncthreads();
-    if (tid == 0) {
-        int n = 0;
-        for (int i = 0; i < kMaxExperts / 32; ++i)
-            for (uint32_t b = named[i]; b; b &= b - 1) list[n++] = (uint16_t)(32 * i + __ffs((int)b) - 1);
-        count = n;
+    if (tid < 64) {   // the named experts' numbers, in order
+        uint32_t w = tid < kMaxExperts / 32 ? named[tid] : 0;
+        int at = __popc(w);
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(at, d);
+            if (tid >= d) at += o;
+        }
+        if (tid == 63) total = at;
+        at -= __popc(w);
+        for (; w; w &= w - 1) list[at++] = 32 * tid + __ffs((int)w) - 1;
     }
     __syncthreads();
-    const int KB = p.I / 128, n0 = blockIdx.x * 16;
-    const int units = count * KB, from = (int)((int64_t)units * wave / kWaves), to = (int)((int64_t)units * (wave + 1) / kWaves);
-    const int64_t ldw = kW == kWFp8 ? p.I : p.I / 2, lds = p.I / 32, pairs = (int64_t)p.T * p.topk;
-    v4f acc[kGroups] = {};
-    int slot[kGroups], have = -1;
-    float c[kGroups];
-    const uint8_t *w = nullptr, *sb = nullptr;
-    const float* sf = nullptr;
-    for (int u = from; u < to; ++u) {
-        const int a = u / KB, kb = u - a * KB, k = kb * 128;
-        if (a != have) {
-            have = a;
-            const int e = list[a];
-            const int64_t row = (int64_t)e * p.H + n0 + col;
-            w = p.w2 + row * ldw;
-            if constexpr (kW == kWFp8) sf = static_cast<const float*>(p.s2) + ((int64_t)e * (p.H / 128) + n0 / 128) * KB;
-            else sb = static_cast<const uint8_t*>(p.s2) + row * lds;
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                slot[g] = -1;
-                c[g] = 0.0f;
-                if (16 * g + col < p.T) slot[g] = find_slot(ids, weights, p.topk, 16 * g + col, e, c[g]);
+    int pass0 = 0, row0 = 0;
+    for (int from = 0; from < total; from += n) {
+        const int e = from + tid < total ? list[from + tid] : -1;
+        int rows = 0;
+        if (e >= 0)
+            for (int t = 0; t < p.T; ++t) {
+                bool hit = false;
+                for (int j = 0; j < p.topk; ++j) hit |= ids[t * p.topk + j] == e;
+                rows += hit;
+            }
+        int np = (rows + kR - 1) / kR, ends_p = np, ends_r = rows;
+        for (int d = 1; d < 64; d *= 2) {
+            const int a = __shfl_up(ends_p, d), b = __shfl_up(ends_r, d);
+            if ((tid & 63) >= d) {
+                ends_p += a;
+                ends_r += b;
             }
         }
-        const WFrag<kW> f = load_w<kW>(w, sb, k, part);
+        if ((tid & 63) == 63) {
+            sums[0][tid >> 6] = ends_p;
+            sums[1][tid >> 6] = ends_r;
+        }
+        __syncthreads();
+        int ps = pass0 + ends_p - np, rs = row0 + ends_r - rows;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < (tid >> 6)) {
+                ps += sums[0][w];
+                rs += sums[1][w];
+            }
+            pass0 += sums[0][w];
+            row0 += sums[1][w];
+        }
+        __syncthreads();
+        for (int q = 0; q < np; ++q) p.passes[ps + q] = Pass{(uint16_t)e, (uint16_t)min(kR, rows - q * kR), rs + q * kR};
+        if (e >= 0)
+            for (int t = 0; t < p.T; ++t) {
+                int slot = -1;
+                float c = 0.0f;
+                for (int j = 0; j < p.topk; ++j)
+                    if (ids[t * p.topk + j] == e) {
+                        c += weights[t * p.topk + j];
+                        if (slot < 0) slot = j;
+                    }
+                if (slot >= 0) p.rows[rs++] = Row{(uint16_t)(t * p.topk + slot), (uint16_t)t, c};
+            }
+    }
+    if (tid == 0) *p.count = pass0;
+}
+
+// Workgroup 0 writes the passes.  The others own 8 RF rows of h (as many gate
+// and up rows) of one expert, K split over the wavefronts: that of a routed
+// pair that is the first to name it (by_pair), or expert blockIdx / tiles.
+// RF = 1: fragment rows 0 .. 7 are gate rows, 8 .. 15 up rows; RF = 2: one
+// fragment each.
+template <int kW, bool kF16, int kR, int RF>
+__global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs p, int by_pair) {
+    typedef StageOf<kW, RF, kR, (kW == kWFp8 ? 256 : 512)> St;
+    constexpr int kRing = kDepth * St::kBytes, kSums = RF * 1024;
+    constexpr int kSmem = kWaves * (kRing > kSums ? kRing : kSums), kIds = kMaxTokens * kMaxTopk * 8;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kSmem > kIds ? kSmem : kIds];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = lane >> 4, r = lane & 15;
+    if (blockIdx.x == 0) {
+        write_passes(p, kR, reinterpret_cast<int*>(smem), reinterpret_cast<float*>(smem) + kMaxTokens * kMaxTopk);
+        return;
+    }
+    const int tiles = p.I / (8 * RF), at = (int)blockIdx.x - 1, owner = at / tiles, i0 = (at - owner * tiles) * 8 * RF;
+    const int e = __builtin_amdgcn_readfirstlane(by_pair ? expert_of(p, owner) : owner);
+    if (e < 0) return;
+    // lane t: token t's first slot that names e
+    int slot = -1;
+    if (lane < p.T)
+        for (int j = p.topk - 1; j >= 0; --j)
+            if (expert_of(p, lane * p.topk + j) == e) slot = j;
+    const uint64_t mask = __ballot(slot >= 0);
+    if (mask == 0) return;
+    if (by_pair) {   // only the first pair's workgroup stays
+        const int first = __ffsll((unsigned long long)mask) - 1;
+        if (first * p.topk + __shfl(slot, first) != owner) return;
+    }
+    const int rows = __popcll(mask);
+    // lane c: the token and slot of the expert's c-th row
+    int token = 0;
+    {
+        uint64_t m = mask;
+        for (int c = 0; c < lane && c < rows - 1; ++c) m &= m - 1;
+        token = __ffsll((unsigned long long)m) - 1;
+    }
+    const int pair = token * p.topk + __shfl(slot, token);
+
+    // the expert's rows from the first gate row to the last up row
+    const int ldw = kW == kWFp8 ? p.H : p.H / 2, lds = p.H / 32;
+    const int units = (p.H + St::kK - 1) / St::kK, from = units * wave / kWaves, S = units * (wave + 1) / kWaves - from;
+    const int64_t row0 = (int64_t)e * 2 * p.I + i0;
+    const v4i dW = make_desc(p.w13 + row0 * ldw, (int64_t)(p.I + 8 * RF) * ldw);
+    const v4i dS = make_desc(static_cast<const uint8_t*>(p.s13) + row0 * lds, (int64_t)(p.I + 8 * RF) * lds);
+    const v4i dX = make_desc(p.x, ((int64_t)(p.T - 1) * p.ld_x + p.H) * 2);
+    const float* const s_gate = static_cast<const float*>(p.s13) + ((int64_t)e * 2 * p.I + i0) / 128 * (p.H / 128);
+    const float* const s_up = s_gate + (int64_t)p.I / 128 * (p.H / 128);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * kRing;
+    const uint8_t* const ring = smem + wave * kRing;
+
+    // weight load j: rows 8 j .. 8 j + 7 of the stage's 16 RF, the gate's then the up's
+    int voff[St::kWLoads];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            if (__ballot(slot[g] >= 0) == 0) continue;
-            bf16x8 hi[4] = {}, lo[4] = {};
-            if (slot[g] >= 0) {
-                const uint16_t* h = p.h + ((int64_t)(16 * g + col) * p.topk + slot[g]) * p.I + k;
+    for (int j = 0; j < St::kWLoads; ++j) {
+        const int q = 8 * j + (lane >> 3);
+        voff[j] = (q < 8 * RF ? q : p.I + q - 8 * RF) * ldw + (((lane & 7) ^ swz(q)) << 4);
+    }
+    const int sq = lane >> 1;   // scale bytes: two lanes a row
+    const int svoff = sq >= 16 * RF ? kOob : (sq < 8 * RF ? sq : p.I + sq - 8 * RF) * lds + (lane & 1) * 4;
+    // this lane's chunks lie in the upper half of the stage: behind H at the end
+    // of an H that is an odd multiple of 128 (MXFP4)
+    const bool behind0 = ((lane & 7) ^ swz(lane >> 3)) >= 4, behind1 = ((lane & 7) ^ swz(8 + (lane >> 3))) >= 4;
+
+    for (int r0 = 0; r0 < rows; r0 += kR) {
+        const int n = min(kR, rows - r0);
+        constexpr int kChunks = St::kK / 8;   // 16-byte chunks of an activation row
+        int xoff[St::kXLoads];
+        bool xbehind[St::kXLoads];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    hi[i] = *reinterpret_cast<const bf16x8*>(h + k_of<kW>(i, part));
-                    lo[i] = *reinterpret_cast<const bf16x8*>(h + pairs * p.I + k_of<kW>(i, part));
+        for (int j = 0; j < St::kXLoads; ++j) {
+            const int i = 64 * j + lane, q = i / kChunks, c = (i % kChunks) ^ q;
+            const int t = __shfl(token, r0 + q < rows ? r0 + q : 0);
+            xoff[j] = q < n ? t * (int)p.ld_x * 2 + c * 16 : kOob;
+            xbehind[j] = c >= kChunks / 2;
+        }
+        auto issue = [&](auto buf_, int s) {
+            constexpr int b = decltype(buf_)::value * St::kBytes;
+            v4i w = dW, x = dX, sc = dS;
+            if (s >= S) w[2] = x[2] = sc[2] = 0;   // keeps the count of loads in flight
+            const int k = (from + s) * St::kK;
+            const bool half = kW == kWMxfp4 && k + St::kK > p.H;
+            static_for<St::kWLoads>([&](auto j_) {
+                constexpr int j = decltype(j_)::value;
+                dma_b128<b + j * 1024, true>(w, lds0, half && (j & 1 ? behind1 : behind0) ? kOob : voff[j], (from + s) * 128);
+            });
+            static_for<St::kXLoads>([&](auto j_) {
+                constexpr int j = decltype(j_)::value;
+                dma_b128<b + St::kXAt + j * 1024, false>(x, lds0, half && xbehind[j] ? kOob : xoff[j], k * 2);
+            });
+            if constexpr (St::kScaleLoads) dma_b32<b + St::kScaleAt>(sc, lds0, svoff, (from + s) * 8);
+        };
+        v4f acc[RF] = {};
+        auto use = [&](auto buf_, int s) {
+            constexpr int b = decltype(buf_)::value * St::kBytes;
+            if (s >= S) return;
+            const uint8_t* const at = ring + b;
+            u32x4 w[RF][2], x[2][St::kParts];
+            uint32_t byte[RF][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int f = 0; f < RF; ++f) {
+                    w[f][j] = St::w(at, f, j, r, part);
+                    byte[f][j] = St::scale(at, f, j, r, part);
+                    // bytes behind H are another row's, perhaps a NaN's
+                    if (kW == kWMxfp4 && j == 1 && (from + s + 1) * St::kK > p.H) byte[f][j] = 0;
                 }
-            }
-            v4f s = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bf16x8 x = widen_w<kW>(f, i);
-                s = mfma(x, hi[i], s);
-                s = mfma(x, lo[i], s);
+                for (int i = 0; i < St::kParts; ++i)   // k = 64 j + 16 part + 8 i, MXFP4 128 j + 32 part + 8 i
+                    x[j][i] = St::x(at, r, (kW == kWFp8 ? 8 * j + 2 * part : 16 * j + 4 * part) + i);
             }
-            // other tokens' columns stay as they are: zeros times an expert's
-            // NaN weight would not be zeros
-            if (slot[g] >= 0) acc[g] += s * (kW == kWFp8 ? c[g] * sf[kb] : c[g]);
+            const float f0 = kW == kWFp8 ? scalar_load(s_gate, from + s) : 0.0f, f1 = kW == kWFp8 ? scalar_load(s_up, from + s) : 0.0f;
+            wait_lds();   // all of the stage is read: its buffer may be filled again
+            issue(buf_, s + kDepth);
+            bf16x8 hi[2][St::kParts], lo[2][St::kParts];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < St::kParts; ++i) {
+                    if constexpr (kF16) split8(__builtin_bit_cast(f16x8, x[j][i]), hi[j][i], lo[j][i]);
+                    else hi[j][i] = __builtin_bit_cast(bf16x8, x[j][i]);
+                }
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                v4f t = kW == kWFp8 ? v4f{} : acc[f];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < St::kParts; ++i) {
+                        const bf16x8 a = widen_w<kW>(w[f][j], i, byte[f][j]);
+                        t = mfma(a, hi[j][i], t);
+                        if constexpr (kF16) t = mfma(a, lo[j][i], t);
+                    }
+                if constexpr (kW == kWFp8) acc[f] += t * (RF == 1 ? (part < 2 ? f0 : f1) : f ? f1 : f0);
+                else acc[f] = t;
+            }
+        };
+        __syncthreads();   // the last pass's sums are read
+        static_for<kDepth>([&](auto b_) { issue(b_, decltype(b_)::value); });
+        for (int s = 0; s < S; s += kDepth)
+            static_for<kDepth>([&](auto b_) {
+                wait_dma_n<(kDepth - 1) * St::kLoads>();
+                use(b_, s + decltype(b_)::value);
+            });
+        wait_dma();
+        __syncthreads();
+        v4f* sums = reinterpret_cast<v4f*>(smem);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) sums[(wave * RF + f) * 64 + lane] = acc[f];
+        __syncthreads();
+        // thread: column c, row q of h; a lane of the sums holds rows 4 part .. 4 part + 3
+        const int c = tid & 15, q = tid >> 4, row = __shfl(pair, min(r0 + c, 63));
+        if (q < 8 * RF && c < n) {
+            const float* f = reinterpret_cast<const float*>(smem);
+            const int g_at = (q / 4 * 16 + c) * 4 + q % 4, u_at = RF == 1 ? g_at + 128 : g_at + 256;
+            float gate = 0.0f, up = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                gate += f[v * RF * 256 + g_at];
+                up += f[v * RF * 256 + u_at];
+            }
+            const float y = gate / (1.0f + __expf(-gate)) * up;
+            const __bf16 hi = (__bf16)y;
+            const int i = i0 + q;
+            uint16_t* h = p.h + ((int64_t)row * (p.I / 128) + i / 128) * 256 + i % 128;
+            h[0] = __builtin_bit_cast(uint16_t, hi);
+            h[128] = __builtin_bit_cast(uint16_t, low_part(y, hi));
         }
     }
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][g][i][lane] = acc[g][i];
+}
+
+// Workgroup: 16 output columns of every token.  The stages of all passes form
+// one sequence, cut into a run for each wavefront; a pass's sums are weighted
+// and added to the wavefront's [T][16] sums in LDS when the run leaves it, and
+// the wavefronts' are added in their order at the end.
+template <int kW, bool kF16, int kR>
+__global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) {
+    typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
+    constexpr int kRing = kDepth * St::kBytes;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // rings, sums [kWaves][T][16], passes, rows
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = lane >> 4, r = lane & 15;
+    float* const sums = reinterpret_cast<float*>(smem + kWaves * kRing);
+    Pass* const passes = reinterpret_cast<Pass*>(sums + kWaves * p.T * 16);
+    Row* const rows = reinterpret_cast<Row*>(passes + p.T * p.topk);
+    const int count = *p.count;
+    for (int i = tid; i < p.T * p.topk; i += kWaves * 64) {
+        if (i < count) passes[i] = p.passes[i];
+        rows[i] = p.rows[i];   // those behind the last are not read
+    }
+    for (int i = tid; i < kWaves * p.T * 16; i += kWaves * 64) sums[i] = 0.0f;
     __syncthreads();
+    float* const own = sums + wave * p.T * 16;
+
+    const int n0 = blockIdx.x * 16, units = (p.I + St::kK - 1) / St::kK;   // stages of a pass
+    const int total = count * units;
+    const int from = (int)((int64_t)total * wave / kWaves), S = (int)((int64_t)total * (wave + 1) / kWaves) - from;
+    const int ldw = kW == kWFp8 ? p.I : p.I / 2, lds = p.I / 32;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * kRing;
+    const uint8_t* const ring = smem + wave * kRing;
+    const v4i dH = make_desc(p.h, (int64_t)p.T * p.topk * p.I * 4);
+    int voff[2];
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        const int t = 16 * g + col;
-        if (t >= p.T) continue;
+    for (int j = 0; j < 2; ++j) {
+        const int q = 8 * j + (lane >> 3);
+        voff[j] = q * ldw + (((lane & 7) ^ swz(q)) << 4);
+    }
+    const int svoff = lane < 32 ? (lane >> 1) * lds + (lane & 1) * 4 : kOob;
+    const bool behind0 = ((lane & 7) ^ swz(lane >> 3)) >= 4, behind1 = ((lane & 7) ^ swz(8 + (lane >> 3))) >= 4;
+
+    // the stage that is loaded next: pass lp, stage lk of it
+    int lp = from / units, lk = from - lp * units;
+    v4i dW = {}, dS = {};
+    int hoff[St::kXLoads];
+    bool hbehind[St::kXLoads];
+    constexpr int kChunks = St::kXLoads * 64 / kR;   // 16-byte chunks of an h row's stage
+    auto enter = [&]() {
+        const Pass v = passes[lp < count ? lp : count - 1];
+        const int e = __builtin_amdgcn_readfirstlane(v.expert);
+        const int64_t row0 = (int64_t)e * p.H + n0;
+        dW = make_desc(p.w2 + row0 * ldw, (int64_t)16 * ldw);
+        if constexpr (kW == kWMxfp4) dS = make_desc(static_cast<const uint8_t*>(p.s2) + row0 * lds, (int64_t)16 * lds);
+#pragma unroll
+        for (int j = 0; j < St::kXLoads; ++j) {
+            const int i = 64 * j + lane, q = i / kChunks, c = (i % kChunks) ^ q;
+            hoff[j] = q < v.rows ? rows[v.first_row + (q < v.rows ? q : 0)].pair * p.I * 4 + c * 16 : kOob;
+            hbehind[j] = c >= kChunks / 2;
+        }
+    };
+    auto issue = [&](auto buf_, int s) {
+        constexpr int b = decltype(buf_)::value * St::kBytes;
+        v4i w = dW, x = dH, sc = dS;
+        if (s >= S) w[2] = x[2] = sc[2] = 0;
+        const bool half = kW == kWMxfp4 && (lk + 1) * St::kK > p.I;
+        dma_b128<b, true>(w, lds0, half && behind0 ? kOob : voff[0], lk * 128);
+        dma_b128<b + 1024, true>(w, lds0, half && behind1 ? kOob : voff[1], lk * 128);
+        static_for<St::kXLoads>([&](auto j_) {
+            constexpr int j = decltype(j_)::value;
+            dma_b128<b + St::kXAt + j * 1024, false>(x, lds0, half && hbehind[j] ? kOob : hoff[j], lk * St::kK * 4);
+        });
+        if constexpr (St::kScaleLoads) dma_b32<b + St::kScaleAt>(sc, lds0, svoff, lk * 8);
+        if (s >= S) return;
+        if (++lk == units) {
+            lk = 0;
+            ++lp;
+            if (s + 1 < S) enter();
+        }
+    };
+
+    // the stage in use: pass up, stage uk of it
+    int up = lp, uk = lk;
+    v4f acc = {};
+    auto leave = [&]() {   // the pass's sums, weighted, to their tokens
+        const Pass v = passes[up];
+        if (r < v.rows) {
+            const Row row = rows[v.first_row + r];
+            v4f* o = reinterpret_cast<v4f*>(own + row.token * 16 + 4 * part);
+            *o += acc * row.weight;
+        }
+        acc = v4f{};
+    };
+    auto use = [&](auto buf_, int s) {
+        constexpr int b = decltype(buf_)::value * St::kBytes;
+        if (s >= S) return;
+        const uint8_t* const at = ring + b;
+        u32x4 w[2], hi[2][St::kParts], lo[2][St::kParts];
+        uint32_t byte[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            w[j] = St::w(at, 0, j, r, part);
+            byte[j] = St::scale(at, 0, j, r, part);
+            if (kW == kWMxfp4 && j == 1 && (uk + 1) * St::kK > p.I) byte[j] = 0;
+#pragma unroll
+            for (int i = 0; i < St::kParts; ++i) {
+                // 128 K of h: 16 chunks of high parts, then 16 of low ones
+                const int c = kW == kWFp8 ? 8 * j + 2 * part + i : 32 * j + 4 * part + i;
+                hi[j][i] = St::x(at, r, c);
+                lo[j][i] = St::x(at, r, c + 16);
+            }
+        }
+        float f = 1.0f;
+        if constexpr (kW == kWFp8) {
+            const int e = __builtin_amdgcn_readfirstlane(passes[up].expert);
+            f = scalar_load(static_cast<const float*>(p.s2), ((int64_t)e * (p.H / 128) + n0 / 128) * units + uk);
+        }
+        wait_lds();
+        issue(buf_, s + kDepth);
+        v4f t = kW == kWFp8 ? v4f{} : acc;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < St::kParts; ++i) {
+                const bf16x8 a = widen_w<kW>(w[j], i, byte[j]);
+                t = mfma(a, __builtin_bit_cast(bf16x8, hi[j][i]), t);
+                t = mfma(a, __builtin_bit_cast(bf16x8, lo[j][i]), t);
+            }
+        if constexpr (kW == kWFp8) acc += t * f;
+        else acc = t;
+        if (++uk == units) {
+            leave();
+            uk = 0;
+            ++up;
+        }
+    };
+    if (S > 0) {
+        enter();
+        static_for<kDepth>([&](auto b_) { issue(b_, decltype(b_)::value); });
+        for (int s = 0; s < S; s += kDepth)
+            static_for<kDepth>([&](auto b_) {
+                wait_dma_n<(kDepth - 1) * St::kLoads>();
+                use(b_, s + decltype(b_)::value);
+            });
+        if (uk) leave();
+    }
+    wait_dma();
+    __syncthreads();
+    for (int i = tid; i < p.T * 16; i += kWaves * 64) {
         float y = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) y += red[v][g][wave][lane];
-        uint16_t* o = static_cast<uint16_t*>(p.out) + (int64_t)t * p.ld_out + n0 + 4 * part + wave;
+        for (int v = 0; v < kWaves; ++v) y += sums[v * p.T * 16 + i];
+        uint16_t* o = static_cast<uint16_t*>(p.out) + (int64_t)(i / 16) * p.ld_out + n0 + i % 16;
         if constexpr (kF16) *o = __builtin_bit_cast(uint16_t, (_Float16)y);
         else *o = __builtin_bit_cast(uint16_t, (__bf16)y);
     }
 }
 
-template <int kW, bool kF16, int kGroups>
+template <int kW, bool kF16, int kR>
 static int launch(const ExpertsArgs& p, hipStream_t st) {
-    const int pairs = p.T * p.topk, by_pair = pairs <= p.E;
-    gate_up_kernel<kW, kF16, kGroups><<<dim3(p.I / 16, by_pair ? pairs : p.E), kWaves * 64, 0, st>>>(p, by_pair);
+    const int pairs = p.T * p.topk, by_pair = pairs <= p.E, owners = by_pair ? pairs : p.E;
+    if (owners * (p.I / 16) >= 2 * cu_count())
+        gate_up_kernel<kW, kF16, kR, 2><<<1 + owners * (p.I / 16), kWaves * 64, 0, st>>>(p, by_pair);
+    else
+        gate_up_kernel<kW, kF16, kR, 1><<<1 + owners * (p.I / 8), kWaves * 64, 0, st>>>(p, by_pair);
     KBN_CHECK_LAUNCH("few_token_experts");
-    down_kernel<kW, kF16, kGroups><<<p.H / 16, kWaves * 64, 0, st>>>(p);
+    typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
+    const size_t smem = kWaves * (kDepth * St::kBytes + p.T * 64) + pairs * (sizeof(Pass) + sizeof(Row));
+    auto* const down = down_kernel<kW, kF16, kR>;
+    if (smem > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(down), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != hipSuccess) (void)hipGetLastError();
+    }
+    down<<<p.H / 16, kWaves * 64, smem, st>>>(p);
     KBN_CHECK_LAUNCH("few_token_experts");
     return 0;
 }
 
 template <int kW, bool kF16>
 static int launch_for(const ExpertsArgs& p, hipStream_t st) {
-    return p.T <= 16 ? launch<kW, kF16, 1>(p, st) : p.T <= 32 ? launch<kW, kF16, 2>(p, st) : launch<kW, kF16, 4>(p, st);
+    return (int64_t)p.T * p.topk > 2 * p.E && p.T > 4 ? launch<kW, kF16, 8>(p, st) : launch<kW, kF16, 4>(p, st);
 }
+
+static int64_t list_bytes(int64_t T, int64_t topk) { return 256 + T * topk * (int64_t)(sizeof(Pass) + sizeof(Row)); }
 
 }  // namespace kbn
 
@@ -352,7 +579,7 @@ using namespace kbn;
 
 extern "C" int64_t kbn_few_token_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I) {
     if (T < 0 || T > kMaxTokens || topk < 1 || topk > kMaxTopk || I < 0 || I >= (1LL << 31)) return 0;
-    return T * topk * I * 4;
+    return list_bytes(T, topk) + T * topk * I * 4;
 }
 
 extern "C" int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* w13, const void* s13, const void* w2,
@@ -366,10 +593,14 @@ extern "C" int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, c
     KBN_CHECK_ARG(T >= 0 && T <= kMaxTokens, "%s: T=%lld tokens, at most %d", what, (long long)T, kMaxTokens);
     KBN_CHECK_ARG(topk >= 1 && topk <= kMaxTopk, "%s: top_k=%lld outside [1, %d]", what, (long long)topk, kMaxTopk);
     KBN_CHECK_ARG(E >= 1 && E <= kMaxExperts, "%s: num_experts=%lld outside [1, %d]", what, (long long)E, kMaxExperts);
-    KBN_CHECK_ARG(H > 0 && I > 0 && H % 128 == 0 && I % 128 == 0 && H < (1 << 24) && I < (1 << 24),
-                  "%s: H=%lld and I=%lld must be multiples of 128", what, (long long)H, (long long)I);
+    KBN_CHECK_ARG(H > 0 && I > 0 && H % 128 == 0 && I % 128 == 0, "%s: H=%lld and I=%lld must be multiples of 128", what,
+                  (long long)H, (long long)I);
+    // offsets within an expert, within the activations and within h are 32-bit
+    KBN_CHECK_ARG(H < (1 << 24) && I < (1 << 24) && (I + 128) * H < (1LL << 31) && T * topk * I * 4 < (1LL << 31) &&
+                      E * (I / 8) < (1LL << 31),
+                  "%s: H=%lld and I=%lld are too large", what, (long long)H, (long long)I);
     if (T == 0) return 0;
-    KBN_CHECK_ARG(ld_x >= H && ld_x % 8 == 0 && x && aligned16(x), "%s: input rows must be 16-byte aligned", what);
+    KBN_CHECK_ARG(ld_x >= H && ld_x % 8 == 0 && ld_x < (1 << 24) && x && aligned16(x), "%s: input rows must be 16-byte aligned", what);
     KBN_CHECK_ARG(ld_out >= H && out && reinterpret_cast<uintptr_t>(out) % 2 == 0, "%s: output row stride %lld below H=%lld", what,
                   (long long)ld_out, (long long)H);
     KBN_CHECK_ARG(w13 && w2 && s13 && s2 && topk_weights && topk_ids, "%s: null pointer", what);
@@ -379,8 +610,10 @@ extern "C" int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, c
     const int64_t need = kbn_few_token_experts_workspace_bytes(T, topk, I);
     KBN_CHECK_ARG(workspace_bytes >= need && aligned16(workspace) && workspace, "%s: workspace of %lld bytes needed, got %lld",
                   what, (long long)need, (long long)workspace_bytes);
+    uint8_t* const ws = (uint8_t*)workspace;
     const ExpertsArgs p{x, ld_x, (const uint8_t*)w13, (const uint8_t*)w2, s13, s2, topk_ids, id_bytes == 8, topk_weights,
-                        (int)T, (int)H, (int)I, (int)E, (int)topk, (uint16_t*)workspace, out, ld_out};
+                        (int)T, (int)H, (int)I, (int)E, (int)topk, (int*)ws, (Pass*)(ws + 256),
+                        (Row*)(ws + 256 + T * topk * sizeof(Pass)), (uint16_t*)(ws + list_bytes(T, topk)), out, ld_out};
     const hipStream_t st = (hipStream_t)stream;
     if (w_format == kWFp8) return x_dtype == kMxF16 ? launch_for<kWFp8, true>(p, st) : launch_for<kWFp8, false>(p, st);
     return x_dtype == kMxF16 ? launch_for<kWMxfp4, true>(p, st) : launch_for<kWMxfp4, false>(p, st);
