@@ -25,6 +25,8 @@
 
 #include "gemm_kernel.h"
 
+#include <cmath>
+
 namespace kbn {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -115,7 +117,6 @@ __device__ __forceinline__ float scalar_load(const float* p, int64_t i) {
     return ((Const)(uintptr_t)p)[i];
 }
 
-constexpr int kWaves = 4, kDepth = 2;
 
 // What a wavefront's stage holds: 16 RF weight rows of 128 bytes, kR activation
 // rows (kRowBytes each) and, for MXFP4, 8 scale bytes a weight row.  Sixteen-byte
@@ -145,6 +146,7 @@ struct StageOf {
 
 // The routing written down for the down launch: the named experts in order,
 // each one's tokens in order, kR rows a pass.  One workgroup.
+template <int kWaves>
 __device__ void write_passes(const ExpertsArgs& p, int kR, int* ids, float* weights) {
     __shared__ uint32_t named[kMaxExperts / 32];
     __shared__ int list[kMaxExperts], total, sums[2][kWaves];
@@ -219,55 +221,36 @@ __device__ void write_passes(const ExpertsArgs& p, int kR, int* ids, float* weig
     if (tid == 0) *p.count = pass0;
 }
 
-// Workgroup 0 writes the passes.  The others own 8 RF rows of h (as many gate
-// and up rows) of one expert, K split over the wavefronts: that of a routed
-// pair that is the first to name it (by_pair), or expert blockIdx / tiles.
-// RF = 1: fragment rows 0 .. 7 are gate rows, 8 .. 15 up rows; RF = 2: one
-// fragment each.
-template <int kW, bool kF16, int kR, int RF>
-__global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs p, int by_pair) {
+// Workgroup 0 writes the passes.  The others own `run` tiles of 8 RF rows of h
+// (as many gate and up rows) of one expert, K split over the wavefronts: the
+// expert of a routed pair that is the first to name it (by_pair), or every
+// expert in turn.  RF = 1: fragment rows 0 .. 7 are gate rows, 8 .. 15 up rows;
+// RF = 2: one fragment each.  A wavefront's stages of all tiles and passes form
+// one sequence, so the ring stays full while a tile's sums meet in LDS; the
+// first stages' weights are asked for before the routing is looked at.
+template <int kW, bool kF16, int kR, int RF, int kWaves, int kDepth>
+__global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs p, int by_pair, int run, int down_rows) {
     typedef StageOf<kW, RF, kR, (kW == kWFp8 ? 256 : 512)> St;
-    constexpr int kRing = kDepth * St::kBytes, kSums = RF * 1024;
-    constexpr int kSmem = kWaves * (kRing > kSums ? kRing : kSums), kIds = kMaxTokens * kMaxTopk * 8;
+    constexpr int kRing = kDepth * St::kBytes, kSums = kWaves * RF * kR * 64;
+    constexpr int kSmem = kWaves * kRing + kSums, kIds = kMaxTokens * kMaxTopk * 8;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kSmem > kIds ? kSmem : kIds];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = lane >> 4, r = lane & 15;
     if (blockIdx.x == 0) {
-        write_passes(p, kR, reinterpret_cast<int*>(smem), reinterpret_cast<float*>(smem) + kMaxTokens * kMaxTopk);
+        write_passes<kWaves>(p, down_rows, reinterpret_cast<int*>(smem), reinterpret_cast<float*>(smem) + kMaxTokens * kMaxTopk);
         return;
     }
-    const int tiles = p.I / (8 * RF), at = (int)blockIdx.x - 1, owner = at / tiles, i0 = (at - owner * tiles) * 8 * RF;
+    const int tiles = p.I / (8 * RF), runs = (tiles + run - 1) / run, at = (int)blockIdx.x - 1, owner = at / runs;
+    const int tile0 = (at - owner * runs) * run, ntiles = min(run, tiles - tile0), i0 = tile0 * 8 * RF;
     const int e = __builtin_amdgcn_readfirstlane(by_pair ? expert_of(p, owner) : owner);
     if (e < 0) return;
-    // lane t: token t's first slot that names e
-    int slot = -1;
-    if (lane < p.T)
-        for (int j = p.topk - 1; j >= 0; --j)
-            if (expert_of(p, lane * p.topk + j) == e) slot = j;
-    const uint64_t mask = __ballot(slot >= 0);
-    if (mask == 0) return;
-    if (by_pair) {   // only the first pair's workgroup stays
-        const int first = __ffsll((unsigned long long)mask) - 1;
-        if (first * p.topk + __shfl(slot, first) != owner) return;
-    }
-    const int rows = __popcll(mask);
-    // lane c: the token and slot of the expert's c-th row
-    int token = 0;
-    {
-        uint64_t m = mask;
-        for (int c = 0; c < lane && c < rows - 1; ++c) m &= m - 1;
-        token = __ffsll((unsigned long long)m) - 1;
-    }
-    const int pair = token * p.topk + __shfl(slot, token);
 
     // the expert's rows from the first gate row to the last up row
     const int ldw = kW == kWFp8 ? p.H : p.H / 2, lds = p.H / 32;
     const int units = (p.H + St::kK - 1) / St::kK, from = units * wave / kWaves, S = units * (wave + 1) / kWaves - from;
     const int64_t row0 = (int64_t)e * 2 * p.I + i0;
-    const v4i dW = make_desc(p.w13 + row0 * ldw, (int64_t)(p.I + 8 * RF) * ldw);
-    const v4i dS = make_desc(static_cast<const uint8_t*>(p.s13) + row0 * lds, (int64_t)(p.I + 8 * RF) * lds);
+    const v4i dW = make_desc(p.w13 + row0 * ldw, (int64_t)(p.I + ntiles * 8 * RF) * ldw);
+    const v4i dS = make_desc(static_cast<const uint8_t*>(p.s13) + row0 * lds, (int64_t)(p.I + ntiles * 8 * RF) * lds);
     const v4i dX = make_desc(p.x, ((int64_t)(p.T - 1) * p.ld_x + p.H) * 2);
-    const float* const s_gate = static_cast<const float*>(p.s13) + ((int64_t)e * 2 * p.I + i0) / 128 * (p.H / 128);
-    const float* const s_up = s_gate + (int64_t)p.I / 128 * (p.H / 128);
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * kRing;
     const uint8_t* const ring = smem + wave * kRing;
 
@@ -283,120 +266,181 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
     // this lane's chunks lie in the upper half of the stage: behind H at the end
     // of an H that is an odd multiple of 128 (MXFP4)
     const bool behind0 = ((lane & 7) ^ swz(lane >> 3)) >= 4, behind1 = ((lane & 7) ^ swz(8 + (lane >> 3))) >= 4;
+    auto load_w = [&](uint32_t base, int tile, int s, bool none) {
+        v4i w = dW, sc = dS;
+        if (none) w[2] = sc[2] = 0;   // an empty load keeps the count of loads in flight
+        const bool half = kW == kWMxfp4 && (from + s + 1) * St::kK > p.H;
+        static_for<St::kWLoads>([&](auto j_) {
+            constexpr int j = decltype(j_)::value;
+            dma_b128<j * 1024, true>(w, base, half && (j & 1 ? behind1 : behind0) ? kOob : voff[j],
+                                     tile * 8 * RF * ldw + (from + s) * 128);
+        });
+        if constexpr (St::kScaleLoads) dma_b32<St::kScaleAt>(sc, base, svoff, tile * 8 * RF * lds + (from + s) * 8);
+    };
+    const bool early = S >= kDepth;
+    if (early)
+        for (int s = 0; s < kDepth; ++s) load_w(lds0 + (uint32_t)s * St::kBytes, 0, s, false);
 
-    for (int r0 = 0; r0 < rows; r0 += kR) {
-        const int n = min(kR, rows - r0);
-        constexpr int kChunks = St::kK / 8;   // 16-byte chunks of an activation row
-        int xoff[St::kXLoads];
-        bool xbehind[St::kXLoads];
+    // lane t: token t's first slot that names e
+    int slot = -1;
+    if (lane < p.T)
+        for (int j = p.topk - 1; j >= 0; --j)
+            if (expert_of(p, lane * p.topk + j) == e) slot = j;
+    const uint64_t mask = __ballot(slot >= 0);
+    const int first = mask ? __ffsll((unsigned long long)mask) - 1 : 0;
+    const bool owned = mask != 0 && (!by_pair || first * p.topk + __shfl(slot, first) == owner);
+    if (!owned) {      // nobody names e, or an earlier pair's workgroup has it
+        wait_dma();    // loads in flight write to this workgroup's LDS
+        return;
+    }
+    const int rows = __popcll(mask);
+    // lane c: the token and slot of the expert's c-th row
+    int token = 0;
+    {
+        uint64_t m = mask;
+        for (int c = 0; c < lane && c < rows - 1; ++c) m &= m - 1;
+        token = __ffsll((unsigned long long)m) - 1;
+    }
+    const int pair = token * p.topk + __shfl(slot, token);
+
+    // the stage that is loaded next: tile lt, rows lr .. lr + kR - 1, stage ls
+    int lt = 0, lr = 0, ls = 0;
+    constexpr int kChunks = St::kK / 8;   // 16-byte chunks of an activation row
+    int xoff[St::kXLoads];
+    bool xbehind[St::kXLoads];
+    auto set_rows = [&]() {
 #pragma unroll
         for (int j = 0; j < St::kXLoads; ++j) {
             const int i = 64 * j + lane, q = i / kChunks, c = (i % kChunks) ^ q;
-            const int t = __shfl(token, r0 + q < rows ? r0 + q : 0);
-            xoff[j] = q < n ? t * (int)p.ld_x * 2 + c * 16 : kOob;
+            const int t = __shfl(token, lr + q < rows ? lr + q : 0);
+            xoff[j] = lr + q < rows ? t * (int)p.ld_x * 2 + c * 16 : kOob;
             xbehind[j] = c >= kChunks / 2;
         }
-        auto issue = [&](auto buf_, int s) {
-            constexpr int b = decltype(buf_)::value * St::kBytes;
-            v4i w = dW, x = dX, sc = dS;
-            if (s >= S) w[2] = x[2] = sc[2] = 0;   // keeps the count of loads in flight
-            const int k = (from + s) * St::kK;
-            const bool half = kW == kWMxfp4 && k + St::kK > p.H;
-            static_for<St::kWLoads>([&](auto j_) {
-                constexpr int j = decltype(j_)::value;
-                dma_b128<b + j * 1024, true>(w, lds0, half && (j & 1 ? behind1 : behind0) ? kOob : voff[j], (from + s) * 128);
-            });
-            static_for<St::kXLoads>([&](auto j_) {
-                constexpr int j = decltype(j_)::value;
-                dma_b128<b + St::kXAt + j * 1024, false>(x, lds0, half && xbehind[j] ? kOob : xoff[j], k * 2);
-            });
-            if constexpr (St::kScaleLoads) dma_b32<b + St::kScaleAt>(sc, lds0, svoff, (from + s) * 8);
-        };
-        v4f acc[RF] = {};
-        auto use = [&](auto buf_, int s) {
-            constexpr int b = decltype(buf_)::value * St::kBytes;
-            if (s >= S) return;
-            const uint8_t* const at = ring + b;
-            u32x4 w[RF][2], x[2][St::kParts];
-            uint32_t byte[RF][2];
+    };
+    auto load_x = [&](uint32_t base, int s, bool none) {
+        v4i x = dX;
+        if (none) x[2] = 0;
+        const int k = (from + s) * St::kK;
+        const bool half = kW == kWMxfp4 && k + St::kK > p.H;
+        static_for<St::kXLoads>([&](auto j_) {
+            constexpr int j = decltype(j_)::value;
+            dma_b128<St::kXAt + j * 1024, false>(x, base, half && xbehind[j] ? kOob : xoff[j], k * 2);
+        });
+    };
+    auto advance = [&]() {
+        if (++ls < S) return;
+        ls = 0;
+        lr += kR;
+        if (lr >= rows) {
+            lr = 0;
+            ++lt;
+        }
+        if (rows > kR) set_rows();
+    };
+    auto issue = [&](int buf) {
+        const uint32_t base = lds0 + (uint32_t)buf * St::kBytes;
+        load_w(base, lt, ls, lt >= ntiles);
+        load_x(base, ls, lt >= ntiles);
+        advance();
+    };
+    set_rows();
+    if (early) {
+        for (int s = 0; s < kDepth; ++s) {
+            load_x(lds0 + (uint32_t)s * St::kBytes, s, false);
+            advance();
+        }
+    } else if (S) {
+        for (int s = 0; s < kDepth; ++s) issue(s);
+    }
+    wait_dma_n<(kDepth - 1) * St::kXLoads>();   // the first stage, in either order
+
+    int buf = 0, sums_at = 0;
+    for (int tile = 0; tile < ntiles; ++tile) {
+        const int i = i0 + tile * 8 * RF;
+        const float* const s_gate = static_cast<const float*>(p.s13) + ((int64_t)e * 2 * p.I + i) / 128 * (p.H / 128);
+        const float* const s_up = static_cast<const float*>(p.s13) + ((int64_t)e * 2 * p.I + p.I + i) / 128 * (p.H / 128);
+        for (int r0 = 0; r0 < rows; r0 += kR) {
+            v4f acc[RF] = {};
+            for (int s = 0; s < S; ++s, buf = buf == kDepth - 1 ? 0 : buf + 1) {
+                wait_dma_n<(kDepth - 1) * St::kLoads>();
+                const uint8_t* const at = ring + buf * St::kBytes;
+                u32x4 w[RF][2], x[2][St::kParts];
+                uint32_t byte[RF][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                for (int f = 0; f < RF; ++f) {
-                    w[f][j] = St::w(at, f, j, r, part);
-                    byte[f][j] = St::scale(at, f, j, r, part);
-                    // bytes behind H are another row's, perhaps a NaN's
-                    if (kW == kWMxfp4 && j == 1 && (from + s + 1) * St::kK > p.H) byte[f][j] = 0;
+                    for (int f = 0; f < RF; ++f) {
+                        w[f][j] = St::w(at, f, j, r, part);
+                        byte[f][j] = St::scale(at, f, j, r, part);
+                        // bytes behind H are another row's, perhaps a NaN's
+                        if (kW == kWMxfp4 && j == 1 && (from + s + 1) * St::kK > p.H) byte[f][j] = 0;
+                    }
+#pragma unroll
+                    for (int q = 0; q < St::kParts; ++q)   // k = 64 j + 16 part + 8 q, MXFP4 128 j + 32 part + 8 q
+                        x[j][q] = St::x(at, r, (kW == kWFp8 ? 8 * j + 2 * part : 16 * j + 4 * part) + q);
                 }
-#pragma unroll
-                for (int i = 0; i < St::kParts; ++i)   // k = 64 j + 16 part + 8 i, MXFP4 128 j + 32 part + 8 i
-                    x[j][i] = St::x(at, r, (kW == kWFp8 ? 8 * j + 2 * part : 16 * j + 4 * part) + i);
-            }
-            const float f0 = kW == kWFp8 ? scalar_load(s_gate, from + s) : 0.0f, f1 = kW == kWFp8 ? scalar_load(s_up, from + s) : 0.0f;
-            wait_lds();   // all of the stage is read: its buffer may be filled again
-            issue(buf_, s + kDepth);
-            bf16x8 hi[2][St::kParts], lo[2][St::kParts];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int i = 0; i < St::kParts; ++i) {
-                    if constexpr (kF16) split8(__builtin_bit_cast(f16x8, x[j][i]), hi[j][i], lo[j][i]);
-                    else hi[j][i] = __builtin_bit_cast(bf16x8, x[j][i]);
-                }
-#pragma unroll
-            for (int f = 0; f < RF; ++f) {
-                v4f t = kW == kWFp8 ? v4f{} : acc[f];
+                const float f0 = kW == kWFp8 ? scalar_load(s_gate, from + s) : 0.0f, f1 = kW == kWFp8 ? scalar_load(s_up, from + s) : 0.0f;
+                wait_lds();   // all of the stage is read: its buffer may be filled again
+                issue(buf);
+                bf16x8 hi[2][St::kParts], lo[2][St::kParts];
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < St::kParts; ++i) {
-                        const bf16x8 a = widen_w<kW>(w[f][j], i, byte[f][j]);
-                        t = mfma(a, hi[j][i], t);
-                        if constexpr (kF16) t = mfma(a, lo[j][i], t);
+                    for (int q = 0; q < St::kParts; ++q) {
+                        if constexpr (kF16) split8(__builtin_bit_cast(f16x8, x[j][q]), hi[j][q], lo[j][q]);
+                        else hi[j][q] = __builtin_bit_cast(bf16x8, x[j][q]);
                     }
-                if constexpr (kW == kWFp8) acc[f] += t * (RF == 1 ? (part < 2 ? f0 : f1) : f ? f1 : f0);
-                else acc[f] = t;
-            }
-        };
-        __syncthreads();   // the last pass's sums are read
-        static_for<kDepth>([&](auto b_) { issue(b_, decltype(b_)::value); });
-        for (int s = 0; s < S; s += kDepth)
-            static_for<kDepth>([&](auto b_) {
-                wait_dma_n<(kDepth - 1) * St::kLoads>();
-                use(b_, s + decltype(b_)::value);
-            });
-        wait_dma();
-        __syncthreads();
-        v4f* sums = reinterpret_cast<v4f*>(smem);
 #pragma unroll
-        for (int f = 0; f < RF; ++f) sums[(wave * RF + f) * 64 + lane] = acc[f];
-        __syncthreads();
-        // thread: column c, row q of h; a lane of the sums holds rows 4 part .. 4 part + 3
-        const int c = tid & 15, q = tid >> 4, row = __shfl(pair, min(r0 + c, 63));
-        if (q < 8 * RF && c < n) {
-            const float* f = reinterpret_cast<const float*>(smem);
-            const int g_at = (q / 4 * 16 + c) * 4 + q % 4, u_at = RF == 1 ? g_at + 128 : g_at + 256;
-            float gate = 0.0f, up = 0.0f;
+                for (int f = 0; f < RF; ++f) {
+                    v4f t = kW == kWFp8 ? v4f{} : acc[f];
 #pragma unroll
-            for (int v = 0; v < kWaves; ++v) {
-                gate += f[v * RF * 256 + g_at];
-                up += f[v * RF * 256 + u_at];
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int q = 0; q < St::kParts; ++q) {
+                            const bf16x8 a = widen_w<kW>(w[f][j], q, byte[f][j]);
+                            t = mfma(a, hi[j][q], t);
+                            if constexpr (kF16) t = mfma(a, lo[j][q], t);
+                        }
+                    if constexpr (kW == kWFp8) acc[f] += t * (RF == 1 ? (part < 2 ? f0 : f1) : f ? f1 : f0);
+                    else acc[f] = t;
+                }
             }
-            const float y = gate / (1.0f + __expf(-gate)) * up;
-            const __bf16 hi = (__bf16)y;
-            const int i = i0 + q;
-            uint16_t* h = p.h + ((int64_t)row * (p.I / 128) + i / 128) * 256 + i % 128;
-            h[0] = __builtin_bit_cast(uint16_t, hi);
-            h[128] = __builtin_bit_cast(uint16_t, low_part(y, hi));
+            // the wavefronts' sums meet: [wavefront][fragment][part][column] of
+            // four rows each
+            float* const sums = reinterpret_cast<float*>(smem + kWaves * kRing);
+            if (r < kR) {
+#pragma unroll
+                for (int f = 0; f < RF; ++f)
+                    *reinterpret_cast<v4f*>(sums + (((wave * RF + f) * 4 + part) * kR + r) * 4) = acc[f];
+            }
+            __syncthreads();
+            // thread: column c, row q of h
+            const int c = tid & 15, q = tid >> 4, row = __shfl(pair, min(r0 + c, 63));
+            if (q < 8 * RF && r0 + c < rows && c < kR) {
+                const int g_at = (q / 4 * kR + c) * 4 + q % 4, u_at = g_at + (RF == 1 ? 2 : 4) * kR * 4;
+                float gate = 0.0f, up = 0.0f;
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) {
+                    gate += sums[v * RF * kR * 16 + g_at];
+                    up += sums[v * RF * kR * 16 + u_at];
+                }
+                const float y = gate / (1.0f + __expf(-gate)) * up;
+                const __bf16 hi = (__bf16)y;
+                uint16_t* h = p.h + ((int64_t)row * (p.I / 128) + (i + q) / 128) * 256 + (i + q) % 128;
+                h[0] = __builtin_bit_cast(uint16_t, hi);
+                h[128] = __builtin_bit_cast(uint16_t, low_part(y, hi));
+            }
+            __syncthreads();   // the sums are read
         }
     }
+    wait_dma();
 }
 
 // Workgroup: 16 output columns of every token.  The stages of all passes form
 // one sequence, cut into a run for each wavefront; a pass's sums are weighted
 // and added to the wavefront's [T][16] sums in LDS when the run leaves it, and
 // the wavefronts' are added in their order at the end.
-template <int kW, bool kF16, int kR>
+template <int kW, bool kF16, int kR, int kWaves, int kDepth>
 __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) {
     typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
     constexpr int kRing = kDepth * St::kBytes;
@@ -407,8 +451,8 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
     Row* const rows = reinterpret_cast<Row*>(passes + p.T * p.topk);
     const int count = *p.count;
     for (int i = tid; i < p.T * p.topk; i += kWaves * 64) {
-        if (i < count) passes[i] = p.passes[i];
-        rows[i] = p.rows[i];   // those behind the last are not read
+        passes[i] = p.passes[i];   // those behind the last hold anything and are not read
+        rows[i] = p.rows[i];
     }
     for (int i = tid; i < kWaves * p.T * 16; i += kWaves * 64) sums[i] = 0.0f;
     __syncthreads();
@@ -546,29 +590,58 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
     }
 }
 
-template <int kW, bool kF16, int kR>
-static int launch(const ExpertsArgs& p, hipStream_t st) {
-    const int pairs = p.T * p.topk, by_pair = pairs <= p.E, owners = by_pair ? pairs : p.E;
-    if (owners * (p.I / 16) >= 2 * cu_count())
-        gate_up_kernel<kW, kF16, kR, 2><<<1 + owners * (p.I / 16), kWaves * 64, 0, st>>>(p, by_pair);
-    else
-        gate_up_kernel<kW, kF16, kR, 1><<<1 + owners * (p.I / 8), kWaves * 64, 0, st>>>(p, by_pair);
-    KBN_CHECK_LAUNCH("few_token_experts");
+constexpr int kDepth = 2;   // stages in flight: more takes LDS that further workgroups use better (T = 16: 317 -> 407 us with 3)
+
+template <int kW, bool kF16, int kR, int kWaves>
+static size_t down_smem(const ExpertsArgs& p) {
     typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
-    const size_t smem = kWaves * (kDepth * St::kBytes + p.T * 64) + pairs * (sizeof(Pass) + sizeof(Row));
-    auto* const down = down_kernel<kW, kF16, kR>;
-    if (smem > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(down), hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != hipSuccess) (void)hipGetLastError();
-    }
-    down<<<p.H / 16, kWaves * 64, smem, st>>>(p);
+    return kWaves * (kDepth * St::kBytes + p.T * 64) + p.T * p.topk * (sizeof(Pass) + sizeof(Row));
+}
+template <int kW, bool kF16, int kR, int kWaves>
+static int launch_down(const ExpertsArgs& p, hipStream_t st) {
+    down_kernel<kW, kF16, kR, kWaves, kDepth><<<p.H / 16, kWaves * 64, down_smem<kW, kF16, kR, kWaves>(p), st>>>(p);
     KBN_CHECK_LAUNCH("few_token_experts");
     return 0;
 }
 
+// active: experts named, on average over uniform routing.  Sixteen gate and
+// sixteen up rows a workgroup, in runs of up to four such tiles where that
+// leaves five workgroups a CU (a run's stages stream without a break: T = 5,
+// MXFP4, 82 us against 96 with single tiles); eight and eight where there would
+// be fewer workgroups than 1.5 a CU, then with eight wavefronts if there is at
+// most one a CU (T = 1 on an eighth 16.2 -> 15.3 us).
+template <int kW, bool kF16, int kR>
+static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hipStream_t st) {
+    const int pairs = p.T * p.topk, by_pair = pairs <= p.E, owners = by_pair ? pairs : p.E, cus = cu_count();
+    if (active * (p.I / 16) >= 1.5 * cus) {
+        const int run = (int)std::max(1.0, std::min(4.0, std::round(active * (p.I / 16) / (5.0 * cus))));
+        gate_up_kernel<kW, kF16, kR, 2, 4, kDepth><<<1 + owners * ((p.I / 16 + run - 1) / run), 256, 0, st>>>(p, by_pair, run, down_rows);
+    } else if (owners * (p.I / 8) > cus) {
+        gate_up_kernel<kW, kF16, kR, 1, 4, kDepth><<<1 + owners * (p.I / 8), 256, 0, st>>>(p, by_pair, 1, down_rows);
+    } else {
+        gate_up_kernel<kW, kF16, kR, 1, 8, kDepth><<<1 + owners * (p.I / 8), 512, 0, st>>>(p, by_pair, 1, down_rows);
+    }
+    KBN_CHECK_LAUNCH("few_token_experts");
+    return 0;
+}
+
+// Rows of a pass: more hold more tokens of an expert, fewer leave LDS for more
+// workgroups.  us, gate/up with 2 / 4 / 8 (MXFP4) and 4 / 8 (FP8): rows an expert
+// 1.1 72 / 76 / 78, 1.6 174 / 169 / 174 and 282 / 294, 2.3 (FP8) 1692 / 1613, 4
+// 449 / 339 / 293.  Down with 2, 4 and 8: 1.1 rows 72 / 74 / 81, 1.6 (FP8) 290 / 280 /
+// 312, 2.3 (FP8) 1660 / 1516 / 1548, 4 360 / 309 / 294, 16 (FP8) 118 / 97 / 89.
 template <int kW, bool kF16>
 static int launch_for(const ExpertsArgs& p, hipStream_t st) {
-    return (int64_t)p.T * p.topk > 2 * p.E && p.T > 4 ? launch<kW, kF16, 8>(p, st) : launch<kW, kF16, 4>(p, st);
+    const double active = p.E * (1.0 - pow(1.0 - std::min(1.0, (double)p.topk / p.E), p.T)), rows = p.T * p.topk / active;
+    int down = rows < 1.5 ? 2 : rows < 3.0 ? 4 : 8;
+    if (down == 4 && down_smem<kW, kF16, 4, 8>(p) > 160 * 1024) down = 8;
+    const int rc = rows < 2.0 ? launch_gate_up<kW, kF16, (kW == kWMxfp4 ? 2 : 4)>(p, active, down, st)
+                              : launch_gate_up<kW, kF16, 8>(p, active, down, st);
+    if (rc) return rc;
+    if (down == 8) return launch_down<kW, kF16, 8, 4>(p, st);
+    if (down == 4) return launch_down<kW, kF16, 4, 8>(p, st);
+    // eight wavefronts on a CU, in one workgroup or two
+    return p.H / 16 < 1.5 * cu_count() ? launch_down<kW, kF16, 2, 8>(p, st) : launch_down<kW, kF16, 2, 4>(p, st);
 }
 
 static int64_t list_bytes(int64_t T, int64_t topk) { return 256 + T * topk * (int64_t)(sizeof(Pass) + sizeof(Row)); }
