@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <utility>
+#include <vector>
 
 #include "kbn_fp8.h"
 
@@ -290,7 +291,179 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- MXFP4 and the experts layer for few tokens
+
+// The C entries' code of a value type; -1 for another type.
+int value_code(at::ScalarType t) {
+    return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1;
+}
+bool is_mx_scales(const at::Tensor& t, int64_t dev) {
+    return (t.scalar_type() == at::kFloat8_e8m0fnu || t.scalar_type() == at::kByte) && t.get_device() == dev;
+}
+
+// A tensor as rows: contiguous, or two dimensions with contiguous rows.
+struct Rows {
+    int64_t n = 0, k = 0, ld = 0;
+    bool ok = false;
+};
+Rows rows_of(const at::Tensor& t) {
+    Rows r;
+    if (t.dim() < 1 || t.numel() == 0) return r;
+    r.k = t.size(-1);
+    r.n = t.numel() / r.k;
+    r.ok = t.is_contiguous() || (t.dim() == 2 && t.stride(1) == 1);
+    r.ld = t.dim() == 2 && r.n > 1 ? t.stride(0) : r.k;
+    return r;
+}
+std::vector<int64_t> with_last(const at::Tensor& like, int64_t last) {
+    std::vector<int64_t> s = like.sizes().vec();
+    s.back() = last;
+    return s;
+}
+at::Tensor empty_like_rows(const at::Tensor& like, int64_t last, at::ScalarType type) {
+    return at::empty(with_last(like, last), like.options().dtype(type).requires_grad(false));
+}
+
+// mx_quant(x) -> (codes, scales) | None
+PyObject* mx_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 1) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor* x = plain_tensor(args[0]);
+        if (!x || !plain_thread()) Py_RETURN_NONE;
+        const int code = value_code(x->scalar_type());
+        const Rows r = rows_of(*x);
+        hipStream_t st;
+        if (code < 0 || !r.ok || r.k % 32 || !launch_stream(x->get_device(), st)) Py_RETURN_NONE;
+        const at::Tensor q = empty_like_rows(*x, r.k / 2, at::kByte), s = empty_like_rows(*x, r.k / 32, at::kFloat8_e8m0fnu);
+        Ref out{pair(q, s)};
+        if (!out.p) return nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_mxfp4_quant(x->data_ptr(), code, r.n, r.k, r.ld, q.data_ptr(), r.k / 2, s.data_ptr(), r.k / 32, (void*)st);
+        }
+        if (rc) return failed(rc, "mxfp4_quant");
+        return out.take();
+    });
+}
+
+// mx_dequant(codes, scales, value code) -> values | None
+PyObject* mx_dequant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 3) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *q = plain_tensor(args[0]), *s = plain_tensor(args[1]);
+        if (!q || !s || !PyLong_CheckExact(args[2]) || !plain_thread()) Py_RETURN_NONE;
+        const long code = PyLong_AsLong(args[2]);
+        const int64_t dev = q->get_device();
+        const Rows r = rows_of(*q), t = rows_of(*s);
+        hipStream_t st;
+        if (code < 0 || code > 2 || q->scalar_type() != at::kByte || !is_mx_scales(*s, dev) || !r.ok || !t.ok || r.k % 16 ||
+            t.k != r.k / 16 || s->dim() != q->dim() || s->sizes().slice(0, s->dim() - 1) != q->sizes().slice(0, q->dim() - 1) ||
+            !launch_stream(dev, st))
+            Py_RETURN_NONE;
+        const at::Tensor out = empty_like_rows(*q, 2 * r.k, code == 0 ? at::kBFloat16 : code == 1 ? at::kHalf : at::kFloat);
+        Ref o{THPVariable_Wrap(out)};
+        if (!o.p) return nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_mxfp4_dequant(q->data_ptr(), r.ld, s->data_ptr(), t.ld, r.n, 2 * r.k, out.data_ptr(), (int)code, 2 * r.k, (void*)st);
+        }
+        if (rc) return failed(rc, "mxfp4_dequant");
+        return o.take();
+    });
+}
+
+// mx_linear(x, codes, scales) -> output | None
+PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 3) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x = plain_tensor(args[0]), *w = plain_tensor(args[1]), *s = plain_tensor(args[2]);
+        if (!x || !w || !s || !plain_thread()) Py_RETURN_NONE;
+        const int code = value_code(x->scalar_type());
+        const int64_t dev = x->get_device();
+        const Rows r = rows_of(*x);
+        hipStream_t st;
+        if (code < 0 || !r.ok || r.k % kGroup || !is(*w, at::kByte, dev, 2) || w->numel() == 0 || w->size(1) * 2 != r.k ||
+            w->stride(1) != 1 || !is_mx_scales(*s, dev) || s->dim() != 2 || s->size(0) != w->size(0) || s->size(1) != r.k / 32 ||
+            s->stride(1) != 1 || !launch_stream(dev, st))
+            Py_RETURN_NONE;
+        const int64_t N = w->size(0), ldw = N > 1 ? w->stride(0) : r.k / 2, lds = N > 1 ? s->stride(0) : r.k / 32;
+        const at::Tensor out = empty_like_rows(*x, N, at::kBFloat16);
+        Ref o{THPVariable_Wrap(out)};
+        if (!o.p) return nullptr;
+        // a buffer of the call's own: calls at once on one stream share nothing
+        const int64_t bytes = kbn_mxfp4_linear_workspace_bytes(r.n, N, r.k, code);
+        const at::Tensor ws = bytes ? at::empty({bytes}, w->options().requires_grad(false)) : at::Tensor();
+        void* const wsp = bytes ? ws.data_ptr() : nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_mxfp4_linear(x->data_ptr(), code, r.ld, w->data_ptr(), ldw, s->data_ptr(), lds, out.data_ptr(), N, r.n, N, r.k,
+                                  wsp, bytes, (void*)st);
+        }
+        if (rc) return failed(rc, "mxfp4_linear");
+        return o.take();
+    });
+}
+
+// few_experts(x, w13, w13 scales, w2, w2 scales, topk weights, topk ids) -> output | None
+PyObject* few_experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 7) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor* t[7];
+        for (int i = 0; i < 7; ++i)
+            if (!(t[i] = plain_tensor(args[i])) || t[i]->numel() == 0) Py_RETURN_NONE;
+        const at::Tensor &x = *t[0], &w13 = *t[1], &s13 = *t[2], &w2 = *t[3], &s2 = *t[4], &tw = *t[5], &ids = *t[6];
+        const int64_t dev = x.get_device();
+        hipStream_t st;
+        if (!plain_thread() || x.dim() != 2 || w13.dim() != 3 || ids.dim() != 2) Py_RETURN_NONE;
+        const int code = value_code(x.scalar_type());
+        const bool fp8 = w13.scalar_type() == at::kFloat8_e4m3fn;
+        const int64_t T = x.size(0), H = x.size(1), E = w13.size(0), N2 = w13.size(1), I = N2 / 2, topk = ids.size(1);
+        const Rows r = rows_of(x);
+        if ((code != 0 && code != 1) || !r.ok || T > 64 || H % kGroup || N2 % (2 * kGroup) ||
+            (!fp8 && w13.scalar_type() != at::kByte) || w13.get_device() != dev || !is(w2, w13.scalar_type(), dev, 3) ||
+            !is(tw, at::kFloat, dev, 2) || (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) ||
+            ids.get_device() != dev || ids.size(0) != T || tw.sizes() != ids.sizes())
+            Py_RETURN_NONE;
+        const int64_t per = fp8 ? 1 : 2;   // values a byte
+        auto shape = [](const at::Tensor& a, int64_t p, int64_t q, int64_t s) {
+            return a.dim() == 3 && a.size(0) == p && a.size(1) == q && a.size(2) == s && a.is_contiguous();
+        };
+        if (!shape(w13, E, N2, H / per) || !shape(w2, E, H, I / per) || !tw.is_contiguous() || !ids.is_contiguous()) Py_RETURN_NONE;
+        if (fp8) {
+            if (!is(s13, at::kFloat, dev, 3) || !is(s2, at::kFloat, dev, 3) || !shape(s13, E, N2 / kGroup, H / kGroup) ||
+                !shape(s2, E, H / kGroup, I / kGroup))
+                Py_RETURN_NONE;
+        } else if (!is_mx_scales(s13, dev) || !is_mx_scales(s2, dev) || !shape(s13, E, N2, H / 32) || !shape(s2, E, H, I / 32)) {
+            Py_RETURN_NONE;
+        }
+        if (!launch_stream(dev, st)) Py_RETURN_NONE;
+        const at::Tensor out = at::empty({T, H}, x.options().requires_grad(false));
+        Ref o{THPVariable_Wrap(out)};
+        if (!o.p) return nullptr;
+        const int64_t bytes = kbn_few_token_experts_workspace_bytes(T, topk, I);
+        if (bytes <= 0) Py_RETURN_NONE;
+        const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte).requires_grad(false));
+        void* const wsp = ws.data_ptr();
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_few_token_experts(x.data_ptr(), code, r.ld, w13.data_ptr(), s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), fp8 ? 0 : 1,
+                                       (const float*)tw.data_ptr(), ids.data_ptr(), (int)ids.element_size(), T, topk, E, H, I,
+                                       out.data_ptr(), H, wsp, bytes, (void*)st);
+        }
+        if (rc) return failed(rc, "few_token_experts");
+        return o.take();
+    });
+}
+
 PyMethodDef kMethods[] = {
+    {"mx_quant", (PyCFunction)(void (*)())mx_quant, METH_FASTCALL, "MXFP4 quantization"},
+    {"mx_dequant", (PyCFunction)(void (*)())mx_dequant, METH_FASTCALL, "the values of MXFP4 codes"},
+    {"mx_linear", (PyCFunction)(void (*)())mx_linear, METH_FASTCALL, "rows through an MXFP4 weight"},
+    {"few_experts", (PyCFunction)(void (*)())few_experts, METH_FASTCALL, "experts layer for few tokens"},
     {"norm", (PyCFunction)(void (*)())norm, METH_FASTCALL, "RMSNorm (+ residual add) + 1x128 quant"},
     {"silu", (PyCFunction)(void (*)())silu, METH_FASTCALL, "SiLU*Mul + 1x128 quant"},
     {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "bf16 activations through an FP8 weight"},

@@ -37,6 +37,10 @@ class FewTokenExperts(nn.Module):
             raise ValueError(f"FewTokenExperts: block_shape must be {expected} for {w13.dtype} weights, got {block_shape}")
         if num_experts != w13.shape[0]:
             raise ValueError(f"FewTokenExperts: num_experts={num_experts}, but w13 holds {w13.shape[0]}")
+        if _ops._host is not None and not torch.compiler.is_compiling():
+            out = _ops._host.few_experts(hidden_states, w13, w13_scale, w2, w2_scale, topk_weights, topk_ids)
+            if out is not None:
+                return out
         out = torch.empty(hidden_states.shape, dtype=hidden_states.dtype, device=hidden_states.device)
         args = (hidden_states, w13, w13_scale, w2, w2_scale, topk_weights.contiguous(), topk_ids.contiguous(), out)
         if torch.compiler.is_compiling():

@@ -27,6 +27,10 @@ class Mxfp4Quant(nn.Module):
     ``[..., K/2]`` and scales float8_e8m0fnu ``[..., K/32]``."""
 
     def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        if _ops._host is not None and not torch.compiler.is_compiling():
+            out = _ops._host.mx_quant(x)   # the plain case in one native step
+            if out is not None:
+                return out
         K = x.shape[-1]
         codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
         scales = torch.empty(*x.shape[:-1], K // MX_GROUP, dtype=torch.float8_e8m0fnu, device=x.device)
@@ -49,6 +53,10 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
     """The values of ``codes [..., K/2]`` with ``scales [..., K/32]`` as ``dtype``
     (bf16, fp16 or fp32) ``[..., K]``: a weight checked or used without the MXFP4
     product."""
+    if _ops._host is not None and not torch.compiler.is_compiling():
+        out = _ops._host.mx_dequant(codes, scales, _ops._QUANT_IN.get(dtype, -1))
+        if out is not None:
+            return out
     out = torch.empty(*codes.shape[:-1], 2 * codes.shape[-1], dtype=dtype, device=codes.device)
     c2, s2, o2 = (codes, scales, out) if codes.dim() == 2 else (_rows(codes), _rows(scales), _rows(out))
     if torch.compiler.is_compiling():
@@ -68,6 +76,10 @@ class Mxfp4Linear(nn.Module):
 
     def forward(self, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                 bias: torch.Tensor | None = None) -> torch.Tensor:
+        if _ops._host is not None and not torch.compiler.is_compiling():
+            output = _ops._host.mx_linear(x, weight, weight_scale)
+            if output is not None:
+                return output if bias is None else output + bias
         N = weight.shape[0]
         flat = x.dim() == 2
         x2 = x if flat else _rows(x)
