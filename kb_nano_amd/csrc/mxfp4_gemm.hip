@@ -97,9 +97,13 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         return *reinterpret_cast<const u32x4*>(smem + kScaleAt + (o & 1) * kScale + (f < FM ? ra : rw) * 16 + (f < FM ? f : f - FM) * 512);
     };
 
+    // The large tile reads the fragments of one step ahead, under the 16 MFMAs
+    // (512 cycles) of a step.  A smaller one's step is over before the reads of
+    // the next are back, so it reads a whole stage ahead.
+    constexpr bool kWhole = BM + BN <= 256;
     v16f acc[FM][FN] = {};
     constexpr int kR = FM + FN, kT = FM * FN;
-    u32x4 f0[kR], f1[kR], raw[kR];
+    u32x4 f[kWhole ? 8 : 2][kR], raw[kR];
     uint32_t sc[kR][4];   // dword: 128 K of the 512; byte 0 for the first 64 of them, byte 2 for the second
     auto mfma_at = [&](int t, const u32x4 (&f)[kR], auto step_) {   // step of 64 K within the 512
         constexpr int step = decltype(step_)::value, op = (step & 1) * 2;
@@ -120,50 +124,71 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
     wait_dma_n<(kStages - 1) * kDma + kScaleDma>();
     __syncthreads();
 #pragma unroll
-    for (int f = 0; f < kR; ++f) {
-        f0[f] = read_frag(0, 0, f);
-        raw[f] = read_scale(0, f);
+    for (int q = 0; q < kR; ++q) {
+#pragma unroll
+        for (int ks = 0; ks < (kWhole ? 4 : 1); ++ks) f[ks][q] = read_frag(0, ks, q);
+        raw[q] = read_scale(0, q);
     }
-    constexpr int kAt = kT >= 2 * kR ? 1 : (2 * kR + kT - 1) / kT;   // reads in a slot
-    // step ks (0 .. 2) of a stage at `at`, and the next one's reads
-    auto step = [&](auto par_, auto ks_, int at) {
-        constexpr int ks = decltype(ks_)::value;
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            mfma_at(t, ks & 1 ? f1 : f0, std::integral_constant<int, 4 * decltype(par_)::value + ks>{});
-#pragma unroll
-            for (int f = t * kAt; f < (t + 1) * kAt && f < kR; ++f) (ks & 1 ? f0 : f1)[f] = read_frag(at, ks + 1, f);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
+
     int at = 0;   // LDS offset of the current stage
-    auto stage = [&](auto par_, int s) {
+    // Stage s + 1 has landed, for odd s the next scales too; in flight behind
+    // it: kStages - 2 stages and, for even s, the scales issued just before the
+    // last of them.  All of stage s is read: its buffer is free.  Returns the
+    // LDS address that the stage kStages ahead goes to.
+    auto turn = [&](auto par_, int s) -> uint32_t {
         constexpr int par = decltype(par_)::value;
-        step(par_, std::integral_constant<int, 0>{}, at);
-        step(par_, std::integral_constant<int, 1>{}, at);
-        step(par_, std::integral_constant<int, 2>{}, at);
-        // stage s + 1 has landed, for odd s the next scales too; in flight
-        // behind it: kStages - 2 stages and, for even s, the scales issued
-        // just before the last of them
         wait_dma_n<(kStages - 2) * kDma + (par == 0 && kStages > 2 ? kScaleDma : 0)>();
         wait_lds();
         __syncthreads();
         if constexpr (par == 1) issue_scales(s / 2 + 2);
-        const int here = at;
+        const uint32_t base = lds + (uint32_t)at;
         at = at == (kStages - 1) * kStage ? 0 : at + kStage;
-        const uint32_t base = lds + (uint32_t)here;
-        static_for<kT>([&](auto t_) {
-            constexpr int t = decltype(t_)::value;
-            mfma_at(t, f1, std::integral_constant<int, 4 * par + 3>{});
+        return base;
+    };
+    // loads of the stage kStages ahead that go to slot t of n
+    auto refill = [&](uint32_t base, auto t_, auto n_, int s) {
+        constexpr int u0 = decltype(t_)::value * kDma / decltype(n_)::value, u1 = (decltype(t_)::value + 1) * kDma / decltype(n_)::value;
+        static_for<u1 - u0>([&](auto u_) { issue(base, std::integral_constant<int, u0 + decltype(u_)::value>{}, s + kStages); });
+    };
+    auto stage = [&](auto par_, int s) {
+        constexpr int par = decltype(par_)::value;
+        if constexpr (kWhole) {
+            const uint32_t base = turn(par_, s);
+            constexpr int kReads = 4 * kR, kAt = (kReads + 3 * kT - 1) / (3 * kT);   // all in the first three steps
+            static_for<4 * kT>([&](auto t_) {
+                constexpr int t = decltype(t_)::value;
+                mfma_at(t % kT, f[4 * par + t / kT], std::integral_constant<int, 4 * par + t / kT>{});
 #pragma unroll
-            for (int f = t * kAt; f < (t + 1) * kAt && f < kR; ++f) {
-                f0[f] = read_frag(at, 0, f);
-                if constexpr (par == 1) raw[f] = read_scale(s / 2 + 1, f);
-            }
-            constexpr int u0 = t * kDma / kT, u1 = (t + 1) * kDma / kT;
-            static_for<u1 - u0>([&](auto u_) { issue(base, std::integral_constant<int, u0 + decltype(u_)::value>{}, s + kStages); });
-            __builtin_amdgcn_sched_barrier(0);
-        });
+                for (int q = t * kAt; q < (t + 1) * kAt && q < kReads; ++q) f[4 * (1 - par) + q / kR][q % kR] = read_frag(at, q / kR, q % kR);
+                if constexpr (par == 1 && t < kR) raw[t] = read_scale(s / 2 + 1, t);
+                refill(base, t_, std::integral_constant<int, 4 * kT>{}, s);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
+            constexpr int kAt = kT >= 2 * kR ? 1 : (2 * kR + kT - 1) / kT;   // reads in a slot
+            static_for<3>([&](auto ks_) {
+                constexpr int ks = decltype(ks_)::value;
+#pragma unroll
+                for (int t = 0; t < kT; ++t) {
+                    mfma_at(t, f[ks & 1], std::integral_constant<int, 4 * par + ks>{});
+#pragma unroll
+                    for (int q = t * kAt; q < (t + 1) * kAt && q < kR; ++q) f[1 - (ks & 1)][q] = read_frag(at, ks + 1, q);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
+            const uint32_t base = turn(par_, s);
+            static_for<kT>([&](auto t_) {
+                constexpr int t = decltype(t_)::value;
+                mfma_at(t, f[1], std::integral_constant<int, 4 * par + 3>{});
+#pragma unroll
+                for (int q = t * kAt; q < (t + 1) * kAt && q < kR; ++q) {
+                    f[0][q] = read_frag(at, 0, q);
+                    if constexpr (par == 1) raw[q] = read_scale(s / 2 + 1, q);
+                }
+                refill(base, t_, std::integral_constant<int, kT>{}, s);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        }
     };
     for (int o = 0; o < pairs; ++o) {
 #pragma unroll
@@ -171,7 +196,7 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
             // bytes behind k_len are another row's, perhaps a NaN's
             const uint32_t m = o * kMxScaleK + i * 128 < k_len ? ~0u : 0u;
 #pragma unroll
-            for (int f = 0; f < kR; ++f) sc[f][i] = (raw[f][i] & m) >> (8 * half);
+            for (int q = 0; q < kR; ++q) sc[q][i] = (raw[q][i] & m) >> (8 * half);
         }
         stage(std::integral_constant<int, 0>{}, 2 * o);
         stage(std::integral_constant<int, 1>{}, 2 * o + 1);
