@@ -8,39 +8,48 @@
 // Codes go from memory to LDS by direct loads in a ring of kStages stages of
 // 256 K (128 bytes a row: whole lines, as the L2 serves a half line in the time
 // of a whole one, 67 against 133 B/ns for each CU when all read shared data).
-// Scale bytes have two buffers of 512 K, one 16-byte load per row.  A stage is
-// four steps of 64 K: while one is multiplied the fragments of the next are
-// read, in the first slots, so that they have landed when they are needed; the
-// one barrier of a stage comes after its third step, where all of the stage
-// has been read: it frees the stage for the loads of the one kStages ahead, one
-// in each MFMA slot of the fourth step.
+// Scale bytes have one buffer of 1024 K, 32 bytes a row: a request takes the L2
+// the same time whatever it fetches of a line, and at 512 K a load the scales
+// were a third of all requests (2 to 8% of the time, 200 x 8192 x 8192 21.3 ->
+// 19.7 us with 64x64 tiles, 4096 x 36864 x 7168 577 -> 571 with 256x256).  A
+// stage is four steps of 64 K.  Its one barrier comes where all of it has been
+// read and frees it for the loads of the stage kStages ahead, which are spread
+// over the MFMA slots behind it.
+//
+// What bounds it.  Large products: power.  4096 x 36864 x 7168 runs at 3.8
+// PFLOP/s with the matrix pipes busy half of the cycles at the 1.6 to 1.8 GHz
+// that the card then holds, and waits for data in 12%; the same instructions
+// alone on random operands reach 5.6 to 6.  Few tiles: the loads, 44 to 55 B/ns
+// a CU where weights come from memory once and from the L2 for the other rows
+// of tiles (200 x 8192 x 8192 19.4 us; more stages in flight change nothing, nor
+// does another row stride).
 #include "mxfp4_gemm.h"
 
 #include "gemm_kernel.h"
 
 namespace kbn {
 
-constexpr int kMxStageK = 256, kMxScaleK = 512;
+constexpr int kMxStageK = 256, kMxPairK = 512, kMxScaleK = 1024;
 
 template <int BM, int BN, int kStages, int kPerCu>
 __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArgs p) {
-    constexpr int kRows = BM + BN, kStage = kRows * 128, kScale = kRows * 16, kScaleAt = kStages * kStage;
+    constexpr int kRows = BM + BN, kStage = kRows * 128, kScaleAt = kStages * kStage;
     constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 32, FN = TN / 32;
     constexpr int kDma = kRows / 32;                            // loads of a wavefront per stage: 8 rows each
-    constexpr int kScaleDma = kRows >= 256 ? kRows / 256 : 1;   // and per 512 K of scales: 64 rows each
+    constexpr int kScaleDma = (kRows + 127) / 128;              // and per 1024 K of scales: 32 rows each
     static_assert(BM % 64 == 0 && BN % 64 == 0 && BM * BN * 2 <= kScaleAt, "epilogue");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kScaleAt + 2 * kScale];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kScaleAt + kRows * 32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
 
     int tm, tn, trel, split;
     tile_coords<8>(p.tiles_m, p.tiles_n, 0, p.splits, tm, tn, trel, split);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int k_from = split * p.groups_per_split * kMxScaleK;
-    const int k_len = min(p.K, k_from + p.groups_per_split * kMxScaleK) - k_from;
+    const int k_from = split * p.groups_per_split * kMxPairK;
+    const int k_len = min(p.K, k_from + p.groups_per_split * kMxPairK) - k_from;
     // The loop has no branches (with one the 256x256 tile's accumulators move
     // between register files): it runs pairs of stages, and what lies past
     // k_len reads as codes and scale bytes of 0, which add nothing.
-    const int pairs = (k_len + kMxScaleK - 1) / kMxScaleK, whole = k_len / kMxStageK;
+    const int pairs = (k_len + kMxPairK - 1) / kMxPairK, whole = k_len / kMxStageK;
 
     // rows past the operand's last read as zeros
     const int rows_a = min(p.M - m0, BM), rows_w = min(p.N - n0, BN);
@@ -61,8 +70,8 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
     int svoff[kScaleDma];
 #pragma unroll
     for (int j = 0; j < kScaleDma; ++j) {
-        const int r = ((4 * j + wave) * 64 + lane) % kRows;   // 128 or 192 rows: some load the same as another wavefront
-        svoff[j] = r < BM ? r * (int)p.ld_sa : (r - BM) * (int)p.ld_sw;
+        const int r = ((4 * j + wave) * 32 + (lane >> 1)) % kRows;   // 192 rows: some load the same as another wavefront
+        svoff[j] = (r < BM ? r * (int)p.ld_sa : (r - BM) * (int)p.ld_sw) + (lane & 1) * 16;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, lds = lds0 + (uint32_t)wave * 1024u;
 
@@ -76,14 +85,14 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         if (s * kMxStageK >= k_len) d[2] = 0;
         dma_b128<j * 4096, false>(d, base, voff[j] | (s == whole ? behind : 0), s * 128);
     };
-    auto issue_scales = [&](int o) {
+    auto issue_scales = [&](int c) {   // 1024 K
         static_for<kScaleDma>([&](auto j_) {
             constexpr int j = decltype(j_)::value;
-            // the 64 rows of one load lie in one operand (BM is a multiple of 64)
-            const int q = (4 * j + wave) % (kRows / 64);
-            v4i d = q < BM / 64 ? dsA : dsW;
-            if (o * kMxScaleK >= k_len) d[2] = 0;
-            dma_b128<kScaleAt, false>(d, lds0 + (uint32_t)(o & 1) * kScale + (uint32_t)q * 1024u, svoff[j], o * 16);
+            // the 32 rows of one load lie in one operand
+            const int q = (4 * j + wave) % (kRows / 32);
+            v4i d = q < BM / 32 ? dsA : dsW;
+            if (c * kMxScaleK >= k_len) d[2] = 0;
+            dma_b128<kScaleAt, false>(d, lds0 + (uint32_t)q * 1024u, svoff[j], c * 32);
         });
     };
 
@@ -94,7 +103,7 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         return *reinterpret_cast<const u32x4*>(smem + at + r * 128 + (((2 * ks + half) ^ swz(r)) << 4) + (f < FM ? f : f - FM) * 4096);
     };
     auto read_scale = [&](int o, int f) -> u32x4 {
-        return *reinterpret_cast<const u32x4*>(smem + kScaleAt + (o & 1) * kScale + (f < FM ? ra : rw) * 16 + (f < FM ? f : f - FM) * 512);
+        return *reinterpret_cast<const u32x4*>(smem + kScaleAt + (f < FM ? ra : rw) * 32 + (o & 1) * 16 + (f < FM ? f : f - FM) * 1024);
     };
 
     // The large tile reads the fragments of one step ahead, under the 16 MFMAs
@@ -115,13 +124,11 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         keep_here<BM + BN == 512>(acc[i][j][0]);
     };
 
-    // in the loop's order: an odd stage issues the next but one scales ahead of its codes
     issue_scales(0);
     static_for<kStages>([&](auto b_) {
-        if constexpr (decltype(b_)::value == kStages - 1) issue_scales(1);
         static_for<kDma>([&](auto j_) { issue(lds + decltype(b_)::value * kStage, j_, decltype(b_)::value); });
     });
-    wait_dma_n<(kStages - 1) * kDma + kScaleDma>();
+    wait_dma_n<(kStages - 1) * kDma>();
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kR; ++q) {
@@ -131,16 +138,18 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
     }
 
     int at = 0;   // LDS offset of the current stage
-    // Stage s + 1 has landed, for odd s the next scales too; in flight behind
-    // it: kStages - 2 stages and, for even s, the scales issued just before the
-    // last of them.  All of stage s is read: its buffer is free.  Returns the
-    // LDS address that the stage kStages ahead goes to.
+    // Stage s + 1 has landed; in flight behind it: kStages - 2 stages.  All of
+    // stage s is read: its buffer is free.  Returns the LDS address that the
+    // stage kStages ahead goes to.  The scales' one buffer is free once the
+    // second pair's bytes are in registers: the next 1024 K are asked for in
+    // the third stage of four and have landed, ahead of that stage's codes, a
+    // stage later.
     auto turn = [&](auto par_, int s) -> uint32_t {
         constexpr int par = decltype(par_)::value;
-        wait_dma_n<(kStages - 2) * kDma + (par == 0 && kStages > 2 ? kScaleDma : 0)>();
+        wait_dma_n<(par == 1 && kStages > 3 ? 1 : kStages - 2) * kDma>();
         wait_lds();
         __syncthreads();
-        if constexpr (par == 1) issue_scales(s / 2 + 2);
+        if (par == 0 && (s & 2)) issue_scales(s / 4 + 1);
         const uint32_t base = lds + (uint32_t)at;
         at = at == (kStages - 1) * kStage ? 0 : at + kStage;
         return base;
@@ -194,7 +203,7 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // bytes behind k_len are another row's, perhaps a NaN's
-            const uint32_t m = o * kMxScaleK + i * 128 < k_len ? ~0u : 0u;
+            const uint32_t m = o * kMxPairK + i * 128 < k_len ? ~0u : 0u;
 #pragma unroll
             for (int q = 0; q < kR; ++q) sc[q][i] = (raw[q][i] & m) >> (8 * half);
         }
@@ -291,7 +300,7 @@ template <int BM, int BN, int kStages, int kPerCu>
 static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStream_t st) {
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
-    const int groups = (p.K + kMxScaleK - 1) / kMxScaleK;
+    const int groups = (p.K + kMxPairK - 1) / kMxPairK;
     p.groups_per_split = (groups + plan.splits - 1) / plan.splits;
     p.splits = (groups + p.groups_per_split - 1) / p.groups_per_split;
     p.P = slabs;
@@ -307,28 +316,29 @@ static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStre
 
 // Prices, in us, of the tiles: fixed cost, a further round of workgroups, a
 // stage of 256 K where each CU has one workgroup, one where it has several (a
-// workgroup's share), fitted to 252 shapes (M 40 .. 2048, seven weights) and
-// split counts timed in graphs; 10% off, and the tile picked is 2% slower than
-// the best one, on average.  Each tile carries shapes: 777 x 4608 x 7168 takes
-// 24.5 us with 128x128 against 26.4 and 49, 4096 x 36864 x 7168 579 with 256x256
-// against 719 and 985, 320 x 1000 x 4096 8.2 with 64x64 against 9.5 and 15,
-// 65 x 24576 x 1536 8.9 with 64x128 against 10.4 with 64x64.
+// workgroup's share), fitted to 72 shapes (M 40 .. 2048, eight weights) and
+// three split counts timed in graphs; 12% off each, but the tile picked is
+// 0.7% slower than the best one on average, 12% at most.  Each tile carries
+// shapes: 777 x 4608 x 7168 takes 24.3 us with 64x128 against 25.7, 29.4 and 47.8,
+// 4096 x 36864 x 7168 571 with 256x256 against 733, 924 and 1167, 320 x 1000 x
+// 4096 7.2 with 64x64 against 8.7 and 12.3, 777 x 7168 x 18432 84 with 128x128
+// against 97 with 64x128.
 struct TilePrice {
     int bm, bn, per_cu;
     double fixed, round, stage_one, stage_many;
 };
 static const TilePrice kTiles[] = {
-    {64, 64, 2, 3.2, 1.1, 0.33, 0.30},
-    {64, 128, 2, 2.7, 0.6, 0.49, 0.47},
-    {128, 128, 2, 2.3, 0.36, 0.76, 0.69},
-    {256, 256, 1, 6.8, 8.1, 1.47, 1.75},
+    {64, 64, 2, 2.8, 1.2, 0.323, 0.272},
+    {64, 128, 2, 3.1, 1.65, 0.466, 0.40},
+    {128, 128, 2, 2.9, 3.0, 0.826, 0.567},
+    {256, 256, 1, 7.5, 8.8, 1.5, 1.7},
 };
 constexpr double kSplitFixed = 3.0, kSplitMb = 0.35;   // the sum's launch, and each MB of partial sums
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
-    const int64_t groups = ceil_div(K, kMxScaleK), cus = cu_count();
+    const int64_t groups = ceil_div(K, kMxPairK), cus = cu_count();
     MxPlan best{};
     double price = 1e30;
     if (M <= 64) {
@@ -348,15 +358,13 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
         if (M <= 16) return best;
     }
     for (const TilePrice& t : kTiles) {
-        const int64_t tiles_m = ceil_div(M, t.bm), tiles = tiles_m * ceil_div(N, t.bn);
+        const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
         for (int splits = 1; splits <= 4 && splits <= groups; ++splits) {
             const int64_t per = ceil_div(groups, splits), used = ceil_div(groups, per);
             if (used != splits) continue;
             const int64_t q = ceil_div(tiles * splits, cus), stages = 2 * per;
-            // one row of tiles: every weight line comes from memory
-            const double cold = tiles_m == 1 ? 1.4 : 1.0;
             double us = t.fixed + t.round * (ceil_div(q, t.per_cu) - 1) +
-                        cold * (q == 1 ? t.stage_one * stages : t.stage_many * stages * q);
+                        (q == 1 ? t.stage_one * stages : t.stage_many * stages * q);
             if (splits > 1) us += kSplitFixed + kSplitMb * 4e-6 * (double)(tiles * t.bm * t.bn * splits);
             if (us < price) {
                 price = us;
