@@ -318,7 +318,7 @@ static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStre
 // stage of 256 K where each CU has one workgroup, one where it has several (a
 // workgroup's share), fitted to 72 shapes (M 40 .. 2048, eight weights) and
 // three split counts timed in graphs; 12% off each, but the tile picked is
-// 0.7% slower than the best one on average, 12% at most.  Each tile carries
+// 0.9% slower than the best one on average, 12% at most.  Each tile carries
 // shapes: 777 x 4608 x 7168 takes 24.3 us with 64x128 against 25.7, 29.4 and 47.8,
 // 4096 x 36864 x 7168 571 with 256x256 against 733, 924 and 1167, 320 x 1000 x
 // 4096 7.2 with 64x64 against 8.7 and 12.3, 777 x 7168 x 18432 84 with 128x128
@@ -343,13 +343,14 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
     double price = 1e30;
     if (M <= 64) {
         // The few-rows kernel is bound by what each CU reads: 16 (rf + cg) rows
-        // of codes a workgroup, about 33 B/ns a CU; K in pairs of stages of
-        // each wavefront.  M = 64: 2048 x 2048 4.7 / 5.3 / 7.0 us with rf 1 / 2 / 4,
-        // 8192 x 8192 18.9 / 13.3 / 17.0, 10240 x 8192 26.1 / 21.1 / 18.4.
+        // a workgroup, K in pairs of stages of each wavefront; fitted to 40
+        // shapes, 11% off.  M = 64: 2048 x 2048 4.4 / 5.2 / 6.8 us with rf 1 / 2 / 4, 8192 x 8192
+        // 18.5 / 13.0 / 16.5, 10240 x 8192 25.7 / 20.8 / 17.1.  Against the tiles, M = 20 and 64: 8192 x 8192 9.7
+        // and 13.0 (12.4 and 13.5), 8192 x 28672 28.6 and 38.3 (28.0 and 30.3).
         const int64_t cg = ceil_div(M, 16), stages = 8 * ceil_div(ceil_div(K, 256), 8);
         for (int rf = 1; rf <= 4; rf *= 2) {
             const int64_t rounds = ceil_div(ceil_div(N, 16 * rf), cus);
-            const double t = 2.7 + 1.5 * (rounds - 1) + 0.0039 * 16 * (rf + cg) * stages * rounds;
+            const double t = 2.6 + 0.7 * (rounds - 1) + (0.064 * rf + 0.039 * cg) * stages * rounds;
             if (t < price) {
                 price = t;
                 best = {0, 0, 1, rf};
@@ -358,13 +359,14 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
         if (M <= 16) return best;
     }
     for (const TilePrice& t : kTiles) {
-        const int64_t tiles = ceil_div(M, t.bm) * ceil_div(N, t.bn);
+        const int64_t tiles_m = ceil_div(M, t.bm), tiles = tiles_m * ceil_div(N, t.bn);
+        const double cold = tiles_m == 1 ? 1.15 : 1.0;   // one row of tiles: every weight line comes from memory
         for (int splits = 1; splits <= 4 && splits <= groups; ++splits) {
             const int64_t per = ceil_div(groups, splits), used = ceil_div(groups, per);
             if (used != splits) continue;
             const int64_t q = ceil_div(tiles * splits, cus), stages = 2 * per;
             double us = t.fixed + t.round * (ceil_div(q, t.per_cu) - 1) +
-                        (q == 1 ? t.stage_one * stages : t.stage_many * stages * q);
+                        cold * (q == 1 ? t.stage_one * stages : t.stage_many * stages * q);
             if (splits > 1) us += kSplitFixed + kSplitMb * 4e-6 * (double)(tiles * t.bm * t.bn * splits);
             if (us < price) {
                 price = us;
