@@ -57,6 +57,8 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
         out = _ops._host.mx_dequant(codes, scales, _ops._QUANT_IN.get(dtype, -1))
         if out is not None:
             return out
+    if scales.shape[:-1] != codes.shape[:-1]:
+        raise ValueError(f"dequantize_mxfp4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} have other rows")
     out = torch.empty(*codes.shape[:-1], 2 * codes.shape[-1], dtype=dtype, device=codes.device)
     c2, s2, o2 = (codes, scales, out) if codes.dim() == 2 else (_rows(codes), _rows(scales), _rows(out))
     if torch.compiler.is_compiling():

@@ -1,0 +1,61 @@
+"""FewTokenExperts where a launch takes several tiles of an expert, several
+passes of its tokens, a wide hidden size, or weights past 32-bit offsets."""
+import pytest
+import torch
+
+from tests.test_gpu_few_token_experts import FP8, call, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("T,E,H,I,topk,spread", [(40, 96, 128, 640, 8, True), (64, 128, 128, 384, 8, True),
+                                                 (64, 128, 256, 384, 8, False), (20, 128, 384, 384, 8, False),
+                                                 (2, 64, 6272, 128, 2, True), (1, 64, 7168, 256, 1, True),
+                                                 (12, 9, 1152, 1920, 4, True), (64, 12, 640, 128, 12, True)])
+def test_tiles_and_passes(gpu_device, T, E, H, I, topk, spread, w):
+    print(f"few-token experts T={T} E={E} H={H} I={I} topk={topk} spread={spread} {w}", flush=True)
+    for dt in (torch.bfloat16, torch.float16):
+        d = make(T, E, H, I, topk, w, dt, T + H, gpu_device, spread)
+        check(d, call(d), f"T={T} {w} {dt}")
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+def test_weights_past_32_bit_offsets(gpu_device, w):
+    """1024 experts, 4.3 and 2.1 GB of FP8 weights (half of that in MXFP4): the last ones and one in between."""
+    print(f"few-token experts past 32 bits {w}", flush=True)
+    T, E, H, I, topk = 6, 1024, 2048, 1024, 3
+    some = torch.tensor([0, 700, E - 1])
+    d = make(T, 3, H, I, topk, w, torch.bfloat16, 9, gpu_device)
+    full = {**d, "E": E, "ids": some.to(torch.int32).to(gpu_device)[d["ids"].long()]}
+    for name in ("w13", "s13", "w2", "s2"):
+        big = torch.zeros(E, *d[name].shape[1:], dtype=torch.uint8 if d[name].dtype is FP8 else d[name].dtype, device=gpu_device)
+        big[some] = d[name].view(big.dtype)
+        full[name] = big.view(d[name].dtype)
+    check(d, call(full), w)
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+def test_weights_of_slots_that_name_nobody_are_not_read(gpu_device, w):
+    print(f"few-token experts NaN routing weights {w}", flush=True)
+    d = make(7, 16, 256, 128, 4, w, torch.bfloat16, 2, gpu_device)
+    d["ids"][::2, 1], d["tw"][::2, 1] = -1, float("nan")
+    d["ids"][3], d["tw"][3] = 16, float("inf")
+    out = call(d)
+    check(d, out, w)
+    assert bool((out[3] == 0).all())
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+def test_the_last_rows_of_the_weights_end_the_buffer(gpu_device, w):
+    """Weights that end where their storage ends, with NaN codes and scales before their start."""
+    print(f"few-token experts at the end of a buffer {w}", flush=True)
+    d = make(3, 5, 384, 128, 2, w, torch.bfloat16, 4, gpu_device)
+    d["ids"][0, 0] = 4
+    d["ids"][0, 1] = 0
+    for name in ("w13", "s13", "w2", "s2"):
+        t = d[name]
+        b = torch.full((256 + t.numel() * t.element_size(),), 0xFF, dtype=torch.uint8, device=gpu_device)
+        b[256:] = t.contiguous().view(torch.uint8).flatten()
+        d[name] = b[256:].view(t.dtype).view(t.shape)
+    check(d, call(d), w)

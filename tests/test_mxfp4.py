@@ -164,3 +164,11 @@ def test_plain_quantization_is_the_nearest():
     best = (x.double().abs().unsqueeze(-1) / s.unsqueeze(-1) - every).abs().amin(-1)
     assert torch.equal((v - x.double()).abs() / s, best)
     assert float(best.max()) <= 1.0
+
+
+def test_dequantize_refuses_other_rows():
+    """As many rows in another arrangement are other rows."""
+    from kb_nano_amd import dequantize_mxfp4
+    for shape in ((3, 2, 2), (6, 2), (2, 4, 2)):
+        with pytest.raises(ValueError, match="other rows"):
+            dequantize_mxfp4(torch.zeros(2, 3, 32, dtype=torch.uint8), torch.zeros(shape, dtype=torch.uint8))
