@@ -343,14 +343,18 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
     double price = 1e30;
     if (M <= 64) {
         // The few-rows kernel is bound by what each CU reads: 16 (rf + cg) rows
-        // a workgroup, K in pairs of stages of each wavefront; fitted to 40
-        // shapes, 11% off.  M = 64: 2048 x 2048 4.4 / 5.2 / 6.8 us with rf 1 / 2 / 4, 8192 x 8192
-        // 18.5 / 13.0 / 16.5, 10240 x 8192 25.7 / 20.8 / 17.1.  Against the tiles, M = 20 and 64: 8192 x 8192 9.7
-        // and 13.0 (12.4 and 13.5), 8192 x 28672 28.6 and 38.3 (28.0 and 30.3).
+        // a workgroup, K in pairs of stages of each wavefront; fitted to 70
+        // shapes, 12% off, the variant picked 0.5% slower than the best one on
+        // average.  us with rf 1 / 2 / 3 / 4: M = 64, 2048 x 2048 4.4 / 5.2 / 6.0 / 6.9,
+        // 8192 x 8192 18.4 / 13.0 / 14.6 / 16.5, 10240 x 8192 25.6 / 20.8 / 15.0 / 17.0;
+        // M = 1, 2.8 / 3.1 / 3.5 / 4.4, 8.3 / 8.5 / 9.8 / 11.4, 11.0 / 11.9 / 10.6 / 10.9,
+        // 36864 x 7168 25.6 / 27.1 / 23.7 / 30.4.  Against the best tile, M = 20 and 64:
+        // 8192 x 8192 9.7 and 13.0 (12.4 and 13.4), 8192 x 28672 29.1 and 38.7
+        // (28.1 and 30.4).
         const int64_t cg = ceil_div(M, 16), stages = 8 * ceil_div(ceil_div(K, 256), 8);
-        for (int rf = 1; rf <= 4; rf *= 2) {
+        for (int rf = 1; rf <= (cg < 4 ? 4 : 3); ++rf) {
             const int64_t rounds = ceil_div(ceil_div(N, 16 * rf), cus);
-            const double t = 2.6 + 0.7 * (rounds - 1) + (0.064 * rf + 0.039 * cg) * stages * rounds;
+            const double t = 2.5 + 0.33 * (rounds - 1) + (0.06 * rf + 0.044 * cg) * stages * rounds;
             if (t < price) {
                 price = t;
                 best = {0, 0, 1, rf};

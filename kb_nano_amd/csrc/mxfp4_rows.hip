@@ -202,7 +202,11 @@ static int launch(const MxGemmArgs& p, hipStream_t st) {
 }
 template <int CG, int kX, int kIn>
 static int launch_for(const MxGemmArgs& p, int rf, hipStream_t st) {
-    return rf == 1 ? launch<1, CG, kX, kIn>(p, st) : rf == 2 ? launch<2, CG, kX, kIn>(p, st) : launch<4, CG, kX, kIn>(p, st);
+    if (rf == 1) return launch<1, CG, kX, kIn>(p, st);
+    if (rf == 2) return launch<2, CG, kX, kIn>(p, st);
+    if constexpr (CG < 4)   // with 64 rows there is always a cheaper tile
+        if (rf == 4) return launch<4, CG, kX, kIn>(p, st);
+    return launch<3, CG, kX, kIn>(p, st);
 }
 
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st) {

@@ -9,10 +9,11 @@ pytestmark = pytest.mark.gpu
 
 # odd widths and K that ends inside a stage (256), a pair (512) or a scale chunk (1024)
 SHAPES = [(17, 67, 640), (33, 65, 640), (51, 67, 1152), (17, 4141, 640), (34, 4183, 1152), (49, 4331, 1152),   # few rows:
-          (18, 8295, 1664), (35, 8213, 1664), (16, 8195, 1408), (1, 8209, 1152), (64, 9001, 2176),   # 16, 32 and 64 wide
+          (18, 8295, 1664), (35, 8213, 1664), (16, 8195, 1408), (1, 8209, 1152), (54, 8235, 1664),   # 16, 32, 48
+          (2, 12305, 640), (17, 12841, 1664), (34, 12677, 1664), (64, 9001, 2176),        # and 64 wide
           (74, 67, 3200), (75, 67, 4352), (2930, 65, 6784), (65, 130, 2176),              # 64 x 64: in 4, 3, 2 splits, 1
-          (2765, 73, 7296), (17, 8227, 8832), (3637, 131, 17280), (65, 16571, 1152),      # 64 x 128
-          (3714, 261, 16256), (65, 16401, 8832), (139, 11375, 12032), (1100, 2050, 2432),  # 128 x 128
+          (2765, 73, 7296), (17, 8227, 18432), (3637, 131, 17280), (65, 16571, 1152),      # 64 x 128
+          (3714, 261, 16256), (65, 16401, 8832), (139, 11375, 12032), (1025, 2051, 640),  # 128 x 128
           (2704, 907, 19072), (3300, 1185, 10368), (816, 5399, 16000), (913, 12331, 640)]  # 256 x 256
 
 
