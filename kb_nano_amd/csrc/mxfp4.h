@@ -77,15 +77,16 @@ __device__ __forceinline__ uint32_t mx_codes8(const uint32_t (&w)[kIn == kMxF32 
 }
 
 // Eight consecutive values of a row (16-byte aligned) as packed words.
-template <int kIn>
+template <int kIn, bool kOnce>
 __device__ __forceinline__ void mx_load8(const void* x, int64_t elem, uint32_t (&w)[kIn == kMxF32 ? 8 : 4]) {
+    auto load = [](const u32x4* p) { return kOnce ? __builtin_nontemporal_load(p) : *p; };
     if constexpr (kIn == kMxF32) {
         const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(x) + elem);
-        const u32x4 a = p[0], b = p[1];
+        const u32x4 a = load(p), b = load(p + 1);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
         w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     } else {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + elem);
+        const u32x4 a = load(reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + elem));
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     }
 }

@@ -243,3 +243,27 @@ def test_linear_graph_and_streams(gpu_device, M):
             outs.append(lin(xs[i % 4], w, sw))
     torch.cuda.synchronize()
     assert all(torch.equal(o, refs[i % 4]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K", [(1153, 8192), (4611, 2080), (131073, 96)])
+def test_quant_of_many_rows(gpu_device, M, K, dtype):
+    """Rows in numbers that no group of rows divides, inside wider buffers, with a NaN in the last row."""
+    from kb_nano_amd import _ops
+    print(f"mxfp4 quant {M}x{K} {dtype}", flush=True)
+    x = torch.zeros(M, K + 64, dtype=dtype, device=gpu_device)
+    x[:, 8:8 + K] = torch.randn(M, K, generator=torch.Generator(gpu_device).manual_seed(M), device=gpu_device)
+    x = x[:, 8:8 + K]
+    x[M - 1, 40] = float("nan")
+    codes = torch.full((M + 1, K // 2 + 8), 7, dtype=torch.uint8, device=gpu_device)
+    scales = torch.full((M + 1, K // 32 + 3), 9, dtype=torch.uint8, device=gpu_device)
+    _ops.mxfp4_quant(x, codes[:M, :K // 2], scales[:M, :K // 32])
+    rows = torch.cat((torch.arange(0, 64), torch.arange(M - 64, M)))
+    _same_quant(x[rows], codes[rows, :K // 2].contiguous(), scales[rows, :K // 32].contiguous())
+    small = [torch.empty(512, n, dtype=torch.uint8, device=gpu_device) for n in (K // 2, K // 32)]
+    for at in range(0, M, 512):   # the same bits as in small calls
+        n = min(512, M - at)
+        _ops.mxfp4_quant(x[at:at + n], small[0][:n], small[1][:n])
+        assert torch.equal(codes[at:at + n, :K // 2], small[0][:n]) and torch.equal(scales[at:at + n, :K // 32], small[1][:n])
+    assert bool((codes[M] == 7).all() and (codes[:, K // 2:] == 7).all())
+    assert bool((scales[M] == 9).all() and (scales[:, K // 32:] == 9).all())
