@@ -9,11 +9,12 @@
 // once, so the activations are not quantized: weight codes widen exactly to
 // bf16 (an MXFP4 code with its power-of-two scale too) and run through the
 // bf16 matrix instruction, 16 weight rows by 16 activation rows, sums in fp32.
-// FP8 block scales multiply each 128-K block's fp32 sum.  An operand with more
-// than bf16's 8 significant bits (fp16 activations, and h, which has fp32's)
-// goes as a pair of bf16 values, x = hi + lo, hi the nearest and lo the
-// nearest to the rest: 16 bits and more, for one more matrix instruction on
-// weights that are there already.
+// FP8 block scales multiply each 128-K block's fp32 sum.  fp16 activations meet
+// FP8 codes in fp16, where those are exact as well.  Another operand with more
+// than bf16's 8 significant bits (fp16 activations of MXFP4 weights, whose
+// scales pass fp16's range, and h, which has fp32's) goes as a pair of bf16
+// values, x = hi + lo, hi the nearest and lo the nearest to the rest: 16 bits
+// and more, for one more matrix instruction on weights that are there already.
 //
 // Both kernels stream like the few-rows MXFP4 product: each wavefront has a
 // private LDS ring filled by direct loads of whole 128-byte weight lines (a
@@ -91,8 +92,22 @@ __device__ __forceinline__ bf16x8 widen_w(const u32x4& q, int i, uint32_t byte) 
     return __builtin_bit_cast(bf16x8, r);
 }
 
+// FP8 codes in fp16 (exact too), for fp16 activations.
+__device__ __forceinline__ f16x8 widen_half(const u32x4& q, int i) {
+    const uint32_t a = i ? q.z : q.x, b = i ? q.w : q.y;
+    u32x4 r;
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true));
+    r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false));
+    r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true));
+    return __builtin_bit_cast(f16x8, r);
+}
+
 __device__ __forceinline__ v4f mfma(bf16x8 a, bf16x8 b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma(f16x8 a, f16x8 b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // The rest of v beside its nearest bf16 (0 beside an infinity).
@@ -382,12 +397,13 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
                 const float f0 = kW == kWFp8 ? scalar_load(s_gate, from + s) : 0.0f, f1 = kW == kWFp8 ? scalar_load(s_up, from + s) : 0.0f;
                 wait_lds();   // all of the stage is read: its buffer may be filled again
                 issue(buf);
+                constexpr bool kHalf = kF16 && kW == kWFp8, kPair = kF16 && !kHalf;
                 bf16x8 hi[2][St::kParts], lo[2][St::kParts];
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int q = 0; q < St::kParts; ++q) {
-                        if constexpr (kF16) split8(__builtin_bit_cast(f16x8, x[j][q]), hi[j][q], lo[j][q]);
+                        if constexpr (kPair) split8(__builtin_bit_cast(f16x8, x[j][q]), hi[j][q], lo[j][q]);
                         else hi[j][q] = __builtin_bit_cast(bf16x8, x[j][q]);
                     }
 #pragma unroll
@@ -397,9 +413,13 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int q = 0; q < St::kParts; ++q) {
-                            const bf16x8 a = widen_w<kW>(w[f][j], q, byte[f][j]);
-                            t = mfma(a, hi[j][q], t);
-                            if constexpr (kF16) t = mfma(a, lo[j][q], t);
+                            if constexpr (kHalf) {
+                                t = mfma(widen_half(w[f][j], q), __builtin_bit_cast(f16x8, x[j][q]), t);
+                            } else {
+                                const bf16x8 a = widen_w<kW>(w[f][j], q, byte[f][j]);
+                                t = mfma(a, hi[j][q], t);
+                                if constexpr (kPair) t = mfma(a, lo[j][q], t);
+                            }
                         }
                     if constexpr (kW == kWFp8) acc[f] += t * (RF == 1 ? (part < 2 ? f0 : f1) : f ? f1 : f0);
                     else acc[f] = t;

@@ -59,3 +59,33 @@ def test_the_last_rows_of_the_weights_end_the_buffer(gpu_device, w):
         b[256:] = t.contiguous().view(torch.uint8).flatten()
         d[name] = b[256:].view(t.dtype).view(t.shape)
     check(d, call(d), w)
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+def test_fp16_subnormal_and_large_activations(gpu_device, w):
+    """fp16 activations from its smallest subnormal number to its largest, a row each; weights of E4M3's
+    smallest subnormals, so that their products show."""
+    print(f"few-token experts fp16 range {w}", flush=True)
+    d = make(8, 6, 256, 128, 2, w, torch.float16, 5, gpu_device)
+    for t, e in enumerate((-24, -20, -15, -14, -10, 0, 8, 12)):
+        d["x"][t] = (d["x"][t].float().clamp(-3, 3) * 2.0 ** e).half()
+    d["x"][0] = torch.where(torch.arange(256, device=gpu_device) % 3 == 0, 2.0 ** -24, 0.0).half()
+    if w == "fp8":
+        small = torch.randint(1, 8, (6, 256, 256), generator=torch.Generator().manual_seed(6), dtype=torch.uint8).to(gpu_device)
+        d["w13"][:, :, ::2] = small.view(FP8)[:, :, ::2]
+        d["s13"][:] = 2.0 ** 18   # sums that reach h from subnormal activations
+        d["s13"][:, :, 1:] = 2.0 ** 17
+        d["v13"] = d["w13"].double() * d["s13"].double().repeat_interleave(128, 1).repeat_interleave(128, 2)
+        d["s2"][:] = 2.0 ** -40
+        d["v2"] = d["w2"].double() * 2.0 ** -40
+    out = call(d)
+    keep = [t for t in range(8) if t < (7 if w == "mxfp4" else 5)]    # the larger rows leave fp16's range with these weights
+    check({**d, "x": d["x"][keep], "ids": d["ids"][keep], "tw": d["tw"][keep]}, out[keep], w)
+    if w == "mxfp4":   # 65520 and more round to infinity: 231 outputs of the last row, of up to 2.3e6
+        x, ref = d["x"][7].double(), torch.zeros(256, dtype=torch.float64, device=gpu_device)
+        for e, c in zip(d["ids"][7].tolist(), d["tw"][7].tolist()):
+            gate, up = (d["v13"][e] @ x).chunk(2)
+            ref += c * (d["v2"][e] @ (gate / (1 + torch.exp(-gate)) * up))
+        over = ref.abs() >= 65520
+        assert int(over.sum()) == 231 and bool((out[7][over].double() == torch.inf * ref[over].sign()).all())
+        assert bool(out[7][~over].isfinite().all())
