@@ -456,42 +456,43 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
     wait_dma();
 }
 
-// Workgroup: 16 output columns of every token.  The stages of all passes form
+// Workgroup: `cols` output columns (at most 16 RF, a multiple of 4) of every
+// token.  The stages of all passes form
 // one sequence, cut into a run for each wavefront; a pass's sums are weighted
 // and added to the wavefront's [T][16] sums in LDS when the run leaves it, and
 // the wavefronts' are added in their order at the end.
-template <int kW, bool kF16, int kR, int kWaves, int kDepth>
-__global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) {
-    typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
-    constexpr int kRing = kDepth * St::kBytes;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // rings, sums [kWaves][T][16], passes, rows
+template <int kW, bool kF16, int kR, int RF, int kWaves, int kDepth>
+__global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, int cols) {
+    typedef StageOf<kW, RF, kR, (kW == kWFp8 ? 512 : 1024)> St;
+    constexpr int kRing = kDepth * St::kBytes, kCols = 16 * RF;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // rings, sums [kWaves][T][kCols], passes, rows
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = lane >> 4, r = lane & 15;
     float* const sums = reinterpret_cast<float*>(smem + kWaves * kRing);
-    Pass* const passes = reinterpret_cast<Pass*>(sums + kWaves * p.T * 16);
+    Pass* const passes = reinterpret_cast<Pass*>(sums + kWaves * p.T * kCols);
     Row* const rows = reinterpret_cast<Row*>(passes + p.T * p.topk);
     const int count = *p.count;
     for (int i = tid; i < p.T * p.topk; i += kWaves * 64) {
         passes[i] = p.passes[i];   // those behind the last hold anything and are not read
         rows[i] = p.rows[i];
     }
-    for (int i = tid; i < kWaves * p.T * 16; i += kWaves * 64) sums[i] = 0.0f;
+    for (int i = tid; i < kWaves * p.T * kCols; i += kWaves * 64) sums[i] = 0.0f;
     __syncthreads();
-    float* const own = sums + wave * p.T * 16;
+    float* const own = sums + wave * p.T * kCols;
 
-    const int n0 = blockIdx.x * 16, units = (p.I + St::kK - 1) / St::kK;   // stages of a pass
+    const int n0 = blockIdx.x * cols, n = min(cols, p.H - n0), units = (p.I + St::kK - 1) / St::kK;   // stages of a pass
     const int total = count * units;
     const int from = (int)((int64_t)total * wave / kWaves), S = (int)((int64_t)total * (wave + 1) / kWaves) - from;
     const int ldw = kW == kWFp8 ? p.I : p.I / 2, lds = p.I / 32;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem + (uint32_t)wave * kRing;
     const uint8_t* const ring = smem + wave * kRing;
     const v4i dH = make_desc(p.h, (int64_t)p.T * p.topk * p.I * 4);
-    int voff[2];
+    int voff[St::kWLoads];   // rows past the last are zeros
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < St::kWLoads; ++j) {
         const int q = 8 * j + (lane >> 3);
-        voff[j] = q * ldw + (((lane & 7) ^ swz(q)) << 4);
+        voff[j] = q < n ? q * ldw + (((lane & 7) ^ swz(q)) << 4) : kOob;
     }
-    const int svoff = lane < 32 ? (lane >> 1) * lds + (lane & 1) * 4 : kOob;
+    const int svoff = (lane >> 1) < n ? (lane >> 1) * lds + (lane & 1) * 4 : kOob;
     const bool behind0 = ((lane & 7) ^ swz(lane >> 3)) >= 4, behind1 = ((lane & 7) ^ swz(8 + (lane >> 3))) >= 4;
 
     // the stage that is loaded next: pass lp, stage lk of it
@@ -504,8 +505,8 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
         const Pass v = passes[lp < count ? lp : count - 1];
         const int e = __builtin_amdgcn_readfirstlane(v.expert);
         const int64_t row0 = (int64_t)e * p.H + n0;
-        dW = make_desc(p.w2 + row0 * ldw, (int64_t)16 * ldw);
-        if constexpr (kW == kWMxfp4) dS = make_desc(static_cast<const uint8_t*>(p.s2) + row0 * lds, (int64_t)16 * lds);
+        dW = make_desc(p.w2 + row0 * ldw, (int64_t)n * ldw);
+        if constexpr (kW == kWMxfp4) dS = make_desc(static_cast<const uint8_t*>(p.s2) + row0 * lds, (int64_t)n * lds);
 #pragma unroll
         for (int j = 0; j < St::kXLoads; ++j) {
             const int i = 64 * j + lane, q = i / kChunks, c = (i % kChunks) ^ q;
@@ -518,8 +519,10 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
         v4i w = dW, x = dH, sc = dS;
         if (s >= S) w[2] = x[2] = sc[2] = 0;
         const bool half = kW == kWMxfp4 && (lk + 1) * St::kK > p.I;
-        dma_b128<b, true>(w, lds0, half && behind0 ? kOob : voff[0], lk * 128);
-        dma_b128<b + 1024, true>(w, lds0, half && behind1 ? kOob : voff[1], lk * 128);
+        static_for<St::kWLoads>([&](auto j_) {
+            constexpr int j = decltype(j_)::value;
+            dma_b128<b + j * 1024, true>(w, lds0, half && (j & 1 ? behind1 : behind0) ? kOob : voff[j], lk * 128);
+        });
         static_for<St::kXLoads>([&](auto j_) {
             constexpr int j = decltype(j_)::value;
             dma_b128<b + St::kXAt + j * 1024, false>(x, lds0, half && hbehind[j] ? kOob : hoff[j], lk * St::kK * 4);
@@ -535,27 +538,31 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
 
     // the stage in use: pass up, stage uk of it
     int up = lp, uk = lk;
-    v4f acc = {};
+    v4f acc[RF] = {};
     auto leave = [&]() {   // the pass's sums, weighted, to their tokens
         const Pass v = passes[up];
         if (r < v.rows) {
             const Row row = rows[v.first_row + r];
-            v4f* o = reinterpret_cast<v4f*>(own + row.token * 16 + 4 * part);
-            *o += acc * row.weight;
+#pragma unroll
+            for (int f = 0; f < RF; ++f) *reinterpret_cast<v4f*>(own + row.token * kCols + 16 * f + 4 * part) += acc[f] * row.weight;
         }
-        acc = v4f{};
+#pragma unroll
+        for (int f = 0; f < RF; ++f) acc[f] = v4f{};
     };
     auto use = [&](auto buf_, int s) {
         constexpr int b = decltype(buf_)::value * St::kBytes;
         if (s >= S) return;
         const uint8_t* const at = ring + b;
-        u32x4 w[2], hi[2][St::kParts], lo[2][St::kParts];
-        uint32_t byte[2];
+        u32x4 w[RF][2], hi[2][St::kParts], lo[2][St::kParts];
+        uint32_t byte[RF][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            w[j] = St::w(at, 0, j, r, part);
-            byte[j] = St::scale(at, 0, j, r, part);
-            if (kW == kWMxfp4 && j == 1 && (uk + 1) * St::kK > p.I) byte[j] = 0;
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                w[f][j] = St::w(at, f, j, r, part);
+                byte[f][j] = St::scale(at, f, j, r, part);
+                if (kW == kWMxfp4 && j == 1 && (uk + 1) * St::kK > p.I) byte[f][j] = 0;
+            }
 #pragma unroll
             for (int i = 0; i < St::kParts; ++i) {
                 // 128 K of h: 16 chunks of high parts, then 16 of low ones
@@ -564,24 +571,28 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
                 lo[j][i] = St::x(at, r, c + 16);
             }
         }
-        float f = 1.0f;
+        float s0 = 1.0f, s1 = 1.0f;   // the scales of the first column's block and the last one's
         if constexpr (kW == kWFp8) {
-            const int e = __builtin_amdgcn_readfirstlane(passes[up].expert);
-            f = scalar_load(static_cast<const float*>(p.s2), ((int64_t)e * (p.H / 128) + n0 / 128) * units + uk);
+            const int64_t row = (int64_t)__builtin_amdgcn_readfirstlane(passes[up].expert) * (p.H / 128);
+            s0 = scalar_load(static_cast<const float*>(p.s2), (row + n0 / 128) * units + uk);
+            if constexpr (RF == 2) s1 = scalar_load(static_cast<const float*>(p.s2), (row + (n0 + n - 1) / 128) * units + uk);
         }
         wait_lds();
         issue(buf_, s + kDepth);
-        v4f t = kW == kWFp8 ? v4f{} : acc;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int f = 0; f < RF; ++f) {
+            v4f t = kW == kWFp8 ? v4f{} : acc[f];
 #pragma unroll
-            for (int i = 0; i < St::kParts; ++i) {
-                const bf16x8 a = widen_w<kW>(w[j], i, byte[j]);
-                t = mfma(a, __builtin_bit_cast(bf16x8, hi[j][i]), t);
-                t = mfma(a, __builtin_bit_cast(bf16x8, lo[j][i]), t);
-            }
-        if constexpr (kW == kWFp8) acc += t * f;
-        else acc = t;
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < St::kParts; ++i) {
+                    const bf16x8 a = widen_w<kW>(w[f][j], i, byte[f][j]);
+                    t = mfma(a, __builtin_bit_cast(bf16x8, hi[j][i]), t);
+                    t = mfma(a, __builtin_bit_cast(bf16x8, lo[j][i]), t);
+                }
+            if constexpr (kW == kWFp8) acc[f] += t * (RF == 1 || n0 % 128 + 16 * f + 4 * part < 128 ? s0 : s1);
+            else acc[f] = t;
+        }
         if (++uk == units) {
             leave();
             uk = 0;
@@ -600,11 +611,12 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
     }
     wait_dma();
     __syncthreads();
-    for (int i = tid; i < p.T * 16; i += kWaves * 64) {
+    for (int i = tid; i < p.T * kCols; i += kWaves * 64) {
+        if (i % kCols >= n) continue;
         float y = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) y += sums[v * p.T * 16 + i];
-        uint16_t* o = static_cast<uint16_t*>(p.out) + (int64_t)(i / 16) * p.ld_out + n0 + i % 16;
+        for (int v = 0; v < kWaves; ++v) y += sums[v * p.T * kCols + i];
+        uint16_t* o = static_cast<uint16_t*>(p.out) + (int64_t)(i / kCols) * p.ld_out + n0 + i % kCols;
         if constexpr (kF16) *o = __builtin_bit_cast(uint16_t, (_Float16)y);
         else *o = __builtin_bit_cast(uint16_t, (__bf16)y);
     }
@@ -612,14 +624,15 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p) 
 
 constexpr int kDepth = 2;   // stages in flight: more takes LDS that further workgroups use better (T = 16: 317 -> 407 us with 3)
 
-template <int kW, bool kF16, int kR, int kWaves>
+template <int kW, int kR, int RF, int kWaves>
 static size_t down_smem(const ExpertsArgs& p) {
-    typedef StageOf<kW, 1, kR, (kW == kWFp8 ? 512 : 1024)> St;
-    return kWaves * (kDepth * St::kBytes + p.T * 64) + p.T * p.topk * (sizeof(Pass) + sizeof(Row));
+    typedef StageOf<kW, RF, kR, (kW == kWFp8 ? 512 : 1024)> St;
+    return kWaves * (kDepth * St::kBytes + p.T * 64 * RF) + p.T * p.topk * (sizeof(Pass) + sizeof(Row));
 }
-template <int kW, bool kF16, int kR, int kWaves>
-static int launch_down(const ExpertsArgs& p, hipStream_t st) {
-    down_kernel<kW, kF16, kR, kWaves, kDepth><<<p.H / 16, kWaves * 64, down_smem<kW, kF16, kR, kWaves>(p), st>>>(p);
+template <int kW, bool kF16, int kR, int RF, int kWaves>
+static int launch_down(const ExpertsArgs& p, int cols, hipStream_t st) {
+    down_kernel<kW, kF16, kR, RF, kWaves, kDepth>
+        <<<(p.H + cols - 1) / cols, kWaves * 64, down_smem<kW, kR, RF, kWaves>(p), st>>>(p, cols);
     KBN_CHECK_LAUNCH("few_token_experts");
     return 0;
 }
@@ -650,18 +663,33 @@ static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hi
 // 1.1 72 / 76 / 78, 1.6 174 / 169 / 174 and 282 / 294, 2.3 (FP8) 1692 / 1613, 4
 // 449 / 339 / 293.  Down with 2, 4 and 8: 1.1 rows 72 / 74 / 81, 1.6 (FP8) 290 / 280 /
 // 312, 2.3 (FP8) 1660 / 1516 / 1548, 4 360 / 309 / 294, 16 (FP8) 118 / 97 / 89.
+//
+// Columns of a down workgroup: 16, but for an H between 16 and 32 columns a CU
+// as many as give every CU one workgroup, in two fragments: with 16 columns
+// H = 7168 has 448 workgroups, of which LDS lets a CU hold one, and reads h as
+// often (64 tokens over 256 experts 1590 -> 1532 us, in MXFP4 1083 -> 976, over 64
+// experts 402 -> 362; H = 5120 165 -> 148; H = 10240 the same 65 either way).
 template <int kW, bool kF16>
 static int launch_for(const ExpertsArgs& p, hipStream_t st) {
     const double active = p.E * (1.0 - pow(1.0 - std::min(1.0, (double)p.topk / p.E), p.T)), rows = p.T * p.topk / active;
-    int down = rows < 1.5 ? 2 : rows < 3.0 ? 4 : 8;
-    if (down == 4 && down_smem<kW, kF16, 4, 8>(p) > 160 * 1024) down = 8;
+    const int cus = cu_count();
+    const bool wide = p.H > 16 * cus && p.H <= 32 * cus;
+    const int cols = wide ? (p.H + 4 * cus - 1) / (4 * cus) * 4 : 16;
+    constexpr size_t kLds = 160 * 1024;
+    const int down = rows < 1.5 ? 2 : rows < 3.0 && (down_smem<kW, 4, 1, 8>(p) <= kLds || (wide && down_smem<kW, 4, 2, 6>(p) <= kLds)) ? 4 : 8;
     const int rc = rows < 2.0 ? launch_gate_up<kW, kF16, (kW == kWMxfp4 ? 2 : 4)>(p, active, down, st)
                               : launch_gate_up<kW, kF16, 8>(p, active, down, st);
     if (rc) return rc;
-    if (down == 8) return launch_down<kW, kF16, 8, 4>(p, st);
-    if (down == 4) return launch_down<kW, kF16, 4, 8>(p, st);
-    // eight wavefronts on a CU, in one workgroup or two
-    return p.H / 16 < 1.5 * cu_count() ? launch_down<kW, kF16, 2, 8>(p, st) : launch_down<kW, kF16, 2, 4>(p, st);
+    if (down == 2) {
+        if (wide && down_smem<kW, 2, 2, 8>(p) <= kLds) return launch_down<kW, kF16, 2, 2, 8>(p, cols, st);
+        return launch_down<kW, kF16, 2, 1, 8>(p, 16, st);
+    }
+    if (down == 4) {
+        if (wide && down_smem<kW, 4, 2, 6>(p) <= kLds) return launch_down<kW, kF16, 4, 2, 6>(p, cols, st);
+        return launch_down<kW, kF16, 4, 1, 8>(p, 16, st);
+    }
+    if (wide && down_smem<kW, 8, 2, 4>(p) <= kLds) return launch_down<kW, kF16, 8, 2, 4>(p, cols, st);
+    return launch_down<kW, kF16, 8, 1, 4>(p, 16, st);
 }
 
 static int64_t list_bytes(int64_t T, int64_t topk) { return 256 + T * topk * (int64_t)(sizeof(Pass) + sizeof(Row)); }

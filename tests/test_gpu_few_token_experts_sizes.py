@@ -89,3 +89,34 @@ def test_fp16_subnormal_and_large_activations(gpu_device, w):
         over = ref.abs() >= 65520
         assert int(over.sum()) == 231 and bool((out[7][over].double() == torch.inf * ref[over].sign()).all())
         assert bool(out[7][~over].isfinite().all())
+
+
+def _among(d, E, dev):
+    """The same layer with its experts as some of E, the others' weights zeros."""
+    n = d["E"]
+    some = torch.arange(n) * (E - 1) // max(1, n - 1)
+    full = {**d, "E": E, "ids": some.to(torch.int32).to(dev)[d["ids"].long()]}
+    for name in ("w13", "s13", "w2", "s2"):
+        big = torch.zeros(E, *d[name].shape[1:], dtype=torch.uint8 if d[name].dtype is FP8 else d[name].dtype, device=dev)
+        big[some] = d[name].view(big.dtype)
+        full[name] = big.view(d[name].dtype)
+    return full
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("T,n,E,H,I,topk", [(1, 8, 64, 4224, 128, 4), (3, 9, 256, 5120, 384, 3), (16, 20, 64, 5248, 256, 6),
+                                            (16, 20, 64, 7168, 128, 6), (40, 6, 9, 8192, 256, 4), (64, 16, 1024, 4224, 128, 8),
+                                            (64, 32, 32, 4480, 128, 32), (64, 24, 300, 7040, 256, 8), (64, 32, 900, 4224, 128, 32)])
+def test_wide_hidden_sizes(gpu_device, T, n, E, H, I, topk, w):
+    """More than 16 columns a CU: workgroups of 20 to 32, across the scales' blocks and past the last column."""
+    print(f"few-token experts T={T} {n} of {E} H={H} I={I} topk={topk} {w}", flush=True)
+    dt = torch.float16 if T == 16 else torch.bfloat16
+    d = make(T, n, H, I, topk, w, dt, T + H, gpu_device)
+    wide = torch.full((T, H + 24), 3.0, dtype=dt, device=gpu_device)
+    full = _among(d, E, gpu_device)
+    out = call(full)
+    check(d, out, f"T={T} H={H} {w}")
+    from kb_nano_amd import _ops
+    _ops.few_token_experts(full["x"], full["w13"], full["s13"], full["w2"], full["s2"], full["tw"], full["ids"], wide[:, 8:8 + H])
+    assert torch.equal(wide[:, 8:8 + H], out)
+    assert bool((wide[:, :8] == 3).all() and (wide[:, 8 + H:] == 3).all())
