@@ -15,6 +15,10 @@
 // scales pass fp16's range, and h, which has fp32's) goes as a pair of bf16
 // values, x = hi + lo, hi the nearest and lo the nearest to the rest: 16 bits
 // and more, for one more matrix instruction on weights that are there already.
+// Bound by the weight stream, which a large read reaches 6.6 TB/s with: 64 tokens
+// over 256 experts (7168, 2048) 1439 us, 6.8 TB/s; 16 of fp16 over 128 (4096, 1536)
+// 243 us, 6.3; 5 over those in MXFP4 69 us, 5.1; one token on an eighth of the
+// 256, 44 MB, 14.6 us, of which two launches and their joins are about six.
 //
 // Both kernels stream like the few-rows MXFP4 product: each wavefront has a
 // private LDS ring filled by direct loads of whole 128-byte weight lines (a
@@ -622,7 +626,7 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, 
     }
 }
 
-constexpr int kDepth = 2;   // stages in flight: more takes LDS that further workgroups use better (T = 16: 317 -> 407 us with 3)
+constexpr int kDepth = 2;   // stages in flight: more takes LDS that further workgroups use better (T = 5, MXFP4, 72 -> 79 us with 3)
 
 template <int kW, int kR, int RF, int kWaves>
 static size_t down_smem(const ExpertsArgs& p) {
@@ -640,9 +644,10 @@ static int launch_down(const ExpertsArgs& p, int cols, hipStream_t st) {
 // active: experts named, on average over uniform routing.  Sixteen gate and
 // sixteen up rows a workgroup, in runs of up to four such tiles where that
 // leaves five workgroups a CU (a run's stages stream without a break: T = 5,
-// MXFP4, 82 us against 96 with single tiles); eight and eight where there would
-// be fewer workgroups than 1.5 a CU, then with eight wavefronts if there is at
-// most one a CU (T = 1 on an eighth 16.2 -> 15.3 us).
+// MXFP4, runs of 1 / 2 / 4 80 / 75 / 74 us; T = 1 on an eighth 17 / 23 / 34); eight and
+// eight where there would be fewer workgroups than 1.5 a CU (T = 1 on an eighth
+// 16.5 us, T = 5 82.6), then with eight wavefronts if there is at most one a CU
+// (15.6; T = 2 on a quarter 24.6 against 20.7 with four).
 template <int kW, bool kF16, int kR>
 static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hipStream_t st) {
     const int pairs = p.T * p.topk, by_pair = pairs <= p.E, owners = by_pair ? pairs : p.E, cus = cu_count();
@@ -659,10 +664,11 @@ static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hi
 }
 
 // Rows of a pass: more hold more tokens of an expert, fewer leave LDS for more
-// workgroups.  us, gate/up with 2 / 4 / 8 (MXFP4) and 4 / 8 (FP8): rows an expert
-// 1.1 72 / 76 / 78, 1.6 174 / 169 / 174 and 282 / 294, 2.3 (FP8) 1692 / 1613, 4
-// 449 / 339 / 293.  Down with 2, 4 and 8: 1.1 rows 72 / 74 / 81, 1.6 (FP8) 290 / 280 /
-// 312, 2.3 (FP8) 1660 / 1516 / 1548, 4 360 / 309 / 294, 16 (FP8) 118 / 97 / 89.
+// workgroups.  us of the layer, gate/up with 2 / 4 / 8: rows an expert 1.1 (MXFP4)
+// 75 / 77 / 80, 1.6 (MXFP4) 179 / 172 / 177, 2.3 (FP8) - / 1610 / 1532, 4 (MXFP4) 458 /
+// 341 / 294.  Down with 2 / 4 / 8: 1.1 rows 70 / 71 / 78, 1.6 (FP8) 266 / 259 / 295, 2.3
+// (FP8) 1702 / 1475 / 1461 and, with an eighth of the rows of h, 239 / 221 / 238, 4
+// 362 / 313 / 294, 16 (FP8) 118 / 97 / 88.
 //
 // Columns of a down workgroup: 16, but for an H between 16 and 32 columns a CU
 // as many as give every CU one workgroup, in two fragments: with 16 columns

@@ -32,7 +32,6 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K);
 // Bytes of the partial sums.
 int64_t mxfp4_plan_bytes(const MxPlan& plan, int64_t M, int64_t N);
 
-constexpr int kMxFusedRows = 2;   // activation rows that the few-rows kernel quantizes itself, at most
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st);
 int mxfp4_gemm_launch(MxGemmArgs& p, float* slabs, hipStream_t st);
 

@@ -13,6 +13,10 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4, weight rows first: a lane's four sums are
 // neighbours in one output row.
 //
+// Bound by what a CU has in flight: its 32 KB of L1 over the latency of a miss, 28
+// to 32 B/ns.  1 x 10240 x 8192 10.2 us, 4.4 TB/s; 1 x 36864 x 7168 23.7, 5.9; 64 x
+// 2048 x 2048 4.4 us, most of it a launch's 2.3 and the start of the stream.
+//
 // kX rows of bf16 or fp16 activations (kX > 0, M <= kX) are quantized by the
 // kernel itself: a lane of the second operand is one scale group of one row,
 // so its 32 values, their maximum, scale and codes stay in the lane.
@@ -25,8 +29,8 @@ namespace kbn {
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // Four wavefronts and two stages: more of either takes more LDS, so fewer
-// workgroups a CU.  us at 1 x 10240 x 8192: 11.1; four stages 11.5, eight
-// wavefronts 12.0.
+// workgroups a CU (1 x 10240 x 8192, 64 weight rows a workgroup: 11.1 us, four
+// stages 11.5, eight wavefronts 12.0).
 constexpr int kRowsWaves = 4, kRowsDepth = 2;
 
 template <int RF, int CG, int kX, int kIn, int kWaves, int kDepth>
@@ -204,13 +208,20 @@ template <int CG, int kX, int kIn>
 static int launch_for(const MxGemmArgs& p, int rf, hipStream_t st) {
     if (rf == 1) return launch<1, CG, kX, kIn>(p, st);
     if (rf == 2) return launch<2, CG, kX, kIn>(p, st);
-    if constexpr (CG < 4)   // with 64 rows there is always a cheaper tile
+    if constexpr (CG < 4 && kX < 8)   // 64 rows have a cheaper tile, 8 rows of values come with N <= 48 CUs
         if (rf == 4) return launch<4, CG, kX, kIn>(p, st);
     return launch<3, CG, kX, kIn>(p, st);
 }
 
+template <int kIn>
+static int launch_values(const MxGemmArgs& p, int rf, hipStream_t st) {
+    if (p.M <= 2) return launch_for<1, 2, kIn>(p, rf, st);
+    if (p.M <= 4) return launch_for<1, 4, kIn>(p, rf, st);
+    return launch_for<1, 8, kIn>(p, rf, st);
+}
+
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st) {
-    if (p.X) return x_dtype == kMxBf16 ? launch_for<1, kMxFusedRows, kMxBf16>(p, rf, st) : launch_for<1, kMxFusedRows, kMxF16>(p, rf, st);
+    if (p.X) return x_dtype == kMxBf16 ? launch_values<kMxBf16>(p, rf, st) : launch_values<kMxF16>(p, rf, st);
     switch ((p.M + 15) / 16) {
         case 1: return launch_for<1, 0, kMxBf16>(p, rf, st);
         case 2: return launch_for<2, 0, kMxBf16>(p, rf, st);

@@ -89,3 +89,29 @@ def test_past_32_bit_offsets(gpu_device):
         _ops.mxfp4_gemm_nt(a, sa, w2, s2, out)
         assert_product(out[:, -64:], values(a, sa), values(w2[-64:], s2[-64:]), f"{m} rows, a weight of 2.3 GB")
         assert_product(out[:, :64], values(a, sa), values(w2[:64], s2[:64]), f"{m} rows, a weight of 2.3 GB")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", range(1, 10))
+@pytest.mark.parametrize("N,K", [(67, 128), (515, 1152), (4357, 640), (9001, 1408), (12999, 384)])
+def test_linear_of_few_rows(gpu_device, M, N, K, dtype):
+    """One launch or two: the bits of the quantization and the product apart, in strided rows, with values
+    over the type's range and a NaN that makes its own row NaN."""
+    from kb_nano_amd import Mxfp4Linear, Mxfp4Quant, _ops
+    print(f"mxfp4 linear {M}x{N}x{K} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(M)
+    lim = 8 if dtype is torch.float16 else 30
+    x = torch.randn(M, K, generator=g) * torch.exp2(torch.randint(-lim, lim, (M, K // 32), generator=g).float()).repeat_interleave(32, 1)
+    wide = torch.full((M, K + 24), float("nan"), dtype=dtype, device=gpu_device)
+    wide[:, 16:16 + K] = x.to(dtype).to(gpu_device)
+    x = wide[:, 16:16 + K]
+    w, sw = random_mx((N, K), 4, gpu_device)
+    for nan in (False, True):
+        if nan:
+            x[M - 1, K - 1] = float("nan")
+        y = Mxfp4Linear()(x, w, sw)
+        codes, scales = Mxfp4Quant()(x)
+        ref = torch.empty_like(y)
+        _ops.mxfp4_gemm_nt(codes, scales, w, sw, ref)
+        assert_product(y, values(codes, scales), values(w, sw), f"{M}x{N}x{K}")
+        assert torch.equal(y.view(torch.int16), ref.view(torch.int16)) or (nan and torch.equal(y[:-1], ref[:-1]))
