@@ -25,7 +25,7 @@
 // stage: 128 K of FP8, 256 K of MXFP4, and the activations of that K), no
 // barrier in the loop.  An expert's tokens are taken kR at a time, a pass; one
 // pass is the rule (2 tokens an expert at 64 tokens and 256 experts with 8 a
-// token), and further ones find the weights in L2.
+// token); further ones read the weights again, as far as L2 has lost them.
 #include "mxfp4.h"
 
 #include "gemm_kernel.h"
@@ -37,6 +37,10 @@ namespace kbn {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// A lambda that holds direct loads is inlined: a call would pass its scalar
+// operands in vector registers.
+#define KBN_INLINE __attribute__((always_inline))
 
 constexpr int kMaxTokens = 64, kMaxTopk = 32, kMaxExperts = 1024;
 enum WFormat : int { kWFp8 = 0, kWMxfp4 = 1 };
@@ -285,7 +289,7 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
     // this lane's chunks lie in the upper half of the stage: behind H at the end
     // of an H that is an odd multiple of 128 (MXFP4)
     const bool behind0 = ((lane & 7) ^ swz(lane >> 3)) >= 4, behind1 = ((lane & 7) ^ swz(8 + (lane >> 3))) >= 4;
-    auto load_w = [&](uint32_t base, int tile, int s, bool none) {
+    auto load_w = [&](uint32_t base, int tile, int s, bool none) KBN_INLINE {
         v4i w = dW, sc = dS;
         if (none) w[2] = sc[2] = 0;   // an empty load keeps the count of loads in flight
         const bool half = kW == kWMxfp4 && (from + s + 1) * St::kK > p.H;
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
             xbehind[j] = c >= kChunks / 2;
         }
     };
-    auto load_x = [&](uint32_t base, int s, bool none) {
+    auto load_x = [&](uint32_t base, int s, bool none) KBN_INLINE {
         v4i x = dX;
         if (none) x[2] = 0;
         const int k = (from + s) * St::kK;
@@ -356,7 +360,7 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
         }
         if (rows > kR) set_rows();
     };
-    auto issue = [&](int buf) {
+    auto issue = [&](int buf) KBN_INLINE {
         const uint32_t base = lds0 + (uint32_t)buf * St::kBytes;
         load_w(base, lt, ls, lt >= ntiles);
         load_x(base, ls, lt >= ntiles);
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, 
     int hoff[St::kXLoads];
     bool hbehind[St::kXLoads];
     constexpr int kChunks = St::kXLoads * 64 / kR;   // 16-byte chunks of an h row's stage
-    auto enter = [&]() {
+    auto enter = [&]() KBN_INLINE {
         const Pass v = passes[lp < count ? lp : count - 1];
         const int e = __builtin_amdgcn_readfirstlane(v.expert);
         const int64_t row0 = (int64_t)e * p.H + n0;
@@ -518,7 +522,7 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, 
             hbehind[j] = c >= kChunks / 2;
         }
     };
-    auto issue = [&](auto buf_, int s) {
+    auto issue = [&](auto buf_, int s) KBN_INLINE {
         constexpr int b = decltype(buf_)::value * St::kBytes;
         v4i w = dW, x = dH, sc = dS;
         if (s >= S) w[2] = x[2] = sc[2] = 0;
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, 
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f] = v4f{};
     };
-    auto use = [&](auto buf_, int s) {
+    auto use = [&](auto buf_, int s) KBN_INLINE {
         constexpr int b = decltype(buf_)::value * St::kBytes;
         if (s >= S) return;
         const uint8_t* const at = ring + b;
@@ -651,24 +655,32 @@ static int launch_down(const ExpertsArgs& p, int cols, hipStream_t st) {
 template <int kW, bool kF16, int kR>
 static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hipStream_t st) {
     const int pairs = p.T * p.topk, by_pair = pairs <= p.E, owners = by_pair ? pairs : p.E, cus = cu_count();
-    if (active * (p.I / 16) >= 1.5 * cus) {
+    const bool many = active * (p.I / 16) >= 1.5 * cus;
+    if constexpr (kR == 16) {
+        if (!many) return launch_gate_up<kW, kF16, 8>(p, active, down_rows, st);
+    }
+    if (many) {
         const int run = (int)std::max(1.0, std::min(4.0, std::round(active * (p.I / 16) / (5.0 * cus))));
         gate_up_kernel<kW, kF16, kR, 2, 4, kDepth><<<1 + owners * ((p.I / 16 + run - 1) / run), 256, 0, st>>>(p, by_pair, run, down_rows);
-    } else if (owners * (p.I / 8) > cus) {
-        gate_up_kernel<kW, kF16, kR, 1, 4, kDepth><<<1 + owners * (p.I / 8), 256, 0, st>>>(p, by_pair, 1, down_rows);
-    } else {
-        gate_up_kernel<kW, kF16, kR, 1, 8, kDepth><<<1 + owners * (p.I / 8), 512, 0, st>>>(p, by_pair, 1, down_rows);
+    } else if constexpr (kR < 16) {
+        if (owners * (p.I / 8) > cus)
+            gate_up_kernel<kW, kF16, kR, 1, 4, kDepth><<<1 + owners * (p.I / 8), 256, 0, st>>>(p, by_pair, 1, down_rows);
+        else
+            gate_up_kernel<kW, kF16, kR, 1, 8, kDepth><<<1 + owners * (p.I / 8), 512, 0, st>>>(p, by_pair, 1, down_rows);
     }
     KBN_CHECK_LAUNCH("few_token_experts");
     return 0;
 }
 
 // Rows of a pass: more hold more tokens of an expert, fewer leave LDS for more
-// workgroups.  us of the layer, gate/up with 2 / 4 / 8: rows an expert 1.1 (MXFP4)
-// 75 / 77 / 80, 1.6 (MXFP4) 179 / 172 / 177, 2.3 (FP8) - / 1610 / 1532, 4 (MXFP4) 458 /
-// 341 / 294.  Down with 2 / 4 / 8: 1.1 rows 70 / 71 / 78, 1.6 (FP8) 266 / 259 / 295, 2.3
-// (FP8) 1702 / 1475 / 1461 and, with an eighth of the rows of h, 239 / 221 / 238, 4
-// 362 / 313 / 294, 16 (FP8) 118 / 97 / 88.
+// workgroups.  us of the layer, gate/up with 2 / 4 / 8 / 16: rows an expert 1.1
+// (MXFP4) 75 / 77 / 80, 1.6 (MXFP4) 179 / 172 / 177, 2.3 (FP8) - / 1610 / 1532, 4 (MXFP4)
+// 458 / 341 / 294 / 348, 4 (FP8) 439 with 8, 434 with 16, 8 (FP8) 357 and 290, (MXFP4)
+// 270 and 236, 16 (FP8) 642 and 522, (MXFP4) 452 and 384.  Down with 2 / 4 / 8 / 16:
+// 1.1 rows 70 / 71 / 78, 1.6 (FP8) 266 / 259 / 295, 2.3 (FP8) 1702 / 1475 / 1461 and,
+// with an eighth of h's columns, 239 / 221 / 238, 4 (MXFP4) 362 / 313 / 294, (FP8) 439
+// with 8, 439 with 16, 8 (FP8) 347 and 326, (MXFP4) 285 and 262, 16 (FP8) 642 and
+// 560, (MXFP4) 452 and 411.
 //
 // Columns of a down workgroup: 16, but for an H between 16 and 32 columns a CU
 // as many as give every CU one workgroup, in two fragments: with 16 columns
@@ -682,9 +694,11 @@ static int launch_for(const ExpertsArgs& p, hipStream_t st) {
     const bool wide = p.H > 16 * cus && p.H <= 32 * cus;
     const int cols = wide ? (p.H + 4 * cus - 1) / (4 * cus) * 4 : 16;
     constexpr size_t kLds = 160 * 1024;
-    const int down = rows < 1.5 ? 2 : rows < 3.0 && (down_smem<kW, 4, 1, 8>(p) <= kLds || (wide && down_smem<kW, 4, 2, 6>(p) <= kLds)) ? 4 : 8;
+    const bool fits4 = down_smem<kW, 4, 1, 8>(p) <= kLds || (wide && down_smem<kW, 4, 2, 6>(p) <= kLds);
+    const int down = rows < 1.5 ? 2 : fits4 && rows < 3.0 ? 4 : rows < 6.0 ? 8 : 16;
     const int rc = rows < 2.0 ? launch_gate_up<kW, kF16, (kW == kWMxfp4 ? 2 : 4)>(p, active, down, st)
-                              : launch_gate_up<kW, kF16, 8>(p, active, down, st);
+                   : rows < (kW == kWMxfp4 ? 6.0 : 3.0) ? launch_gate_up<kW, kF16, 8>(p, active, down, st)
+                                                        : launch_gate_up<kW, kF16, 16>(p, active, down, st);
     if (rc) return rc;
     if (down == 2) {
         if (wide && down_smem<kW, 2, 2, 8>(p) <= kLds) return launch_down<kW, kF16, 2, 2, 8>(p, cols, st);
@@ -694,8 +708,17 @@ static int launch_for(const ExpertsArgs& p, hipStream_t st) {
         if (wide && down_smem<kW, 4, 2, 6>(p) <= kLds) return launch_down<kW, kF16, 4, 2, 6>(p, cols, st);
         return launch_down<kW, kF16, 4, 1, 8>(p, 16, st);
     }
-    if (wide && down_smem<kW, 8, 2, 4>(p) <= kLds) return launch_down<kW, kF16, 8, 2, 4>(p, cols, st);
-    return launch_down<kW, kF16, 8, 1, 4>(p, 16, st);
+    if (down == 8) {
+        if (wide && down_smem<kW, 8, 2, 4>(p) <= kLds) return launch_down<kW, kF16, 8, 2, 4>(p, cols, st);
+        return launch_down<kW, kF16, 8, 1, 4>(p, 16, st);
+    }
+    if constexpr (kW == kWFp8) {
+        return wide ? launch_down<kW, kF16, 16, 2, 4>(p, cols, st) : launch_down<kW, kF16, 16, 1, 4>(p, 16, st);
+    } else {
+        if (wide && down_smem<kW, 16, 2, 3>(p) <= kLds) return launch_down<kW, kF16, 16, 2, 3>(p, cols, st);
+        if (down_smem<kW, 16, 1, 4>(p) <= kLds) return launch_down<kW, kF16, 16, 1, 4>(p, 16, st);
+        return launch_down<kW, kF16, 16, 1, 3>(p, 16, st);
+    }
 }
 
 static int64_t list_bytes(int64_t T, int64_t topk) { return 256 + T * topk * (int64_t)(sizeof(Pass) + sizeof(Row)); }

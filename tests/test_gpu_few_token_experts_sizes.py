@@ -120,3 +120,17 @@ def test_wide_hidden_sizes(gpu_device, T, n, E, H, I, topk, w):
     _ops.few_token_experts(full["x"], full["w13"], full["s13"], full["w2"], full["s2"], full["tw"], full["ids"], wide[:, 8:8 + H])
     assert torch.equal(wide[:, 8:8 + H], out)
     assert bool((wide[:, :8] == 3).all() and (wide[:, 8 + H:] == 3).all())
+
+
+@pytest.mark.parametrize("w", ["fp8", "mxfp4"])
+@pytest.mark.parametrize("T,E,H,I,topk,spread", [(64, 12, 256, 640, 4, True), (24, 16, 384, 512, 4, True), (37, 9, 4224, 768, 2, True),
+                                                 (64, 16, 128, 512, 8, False), (33, 8, 5120, 128, 1, True), (64, 14, 4224, 512, 14, True),
+                                                 (20, 4, 1152, 1664, 2, True), (64, 40, 128, 256, 32, True)])
+def test_many_rows_an_expert(gpu_device, T, E, H, I, topk, spread, w):
+    """Passes of sixteen rows, whole ones and the rest, in both launches."""
+    print(f"few-token experts T={T} E={E} H={H} I={I} topk={topk} spread={spread} {w}", flush=True)
+    for dt in (torch.bfloat16, torch.float16):
+        d = make(T, E, H, I, topk, w, dt, T + H, gpu_device, spread)
+        out = call(d)
+        check(d, out, f"T={T} {w} {dt}")
+        assert torch.equal(out, call(d))
