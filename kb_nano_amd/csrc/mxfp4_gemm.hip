@@ -19,10 +19,12 @@
 // What bounds it.  Large products: power.  4096 x 36864 x 7168 runs at 3.8
 // PFLOP/s with the matrix pipes busy half of the cycles at the 1.6 to 1.8 GHz
 // that the card then holds, and waits for data in 12%; the same instructions
-// alone on random operands reach 5.6 to 6.  Few tiles: the loads, 44 to 55 B/ns
-// a CU where weights come from memory once and from the L2 for the other rows
-// of tiles (200 x 8192 x 8192 19.4 us; more stages in flight change nothing, nor
-// does another row stride).
+// alone on random operands reach 5.6 to 6.  Smaller tiles: the CU's path
+// for loads.  With 64x128 tiles at 4096 x 8192 x 8192 its return side is busy 89%
+// of the cycles and its address side 79% (128x128 84 and 67%, 256x256 51 and 37%),
+// the matrix pipes 34%, LDS 35%; 44 to 55 B/ns a CU arrive, also where each CU has
+// one tile (200 x 8192 x 8192 19.4 us), whatever the depth of the ring or the row
+// stride.  Two wavefronts a tile instead of four take up to twice as long.
 #include "mxfp4_gemm.h"
 
 #include "gemm_kernel.h"

@@ -13,9 +13,9 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4, weight rows first: a lane's four sums are
 // neighbours in one output row.
 //
-// Bound by what a CU has in flight: its 32 KB of L1 over the latency of a miss, 28
-// to 32 B/ns.  1 x 10240 x 8192 10.2 us, 4.4 TB/s; 1 x 36864 x 7168 23.7, 5.9; 64 x
-// 2048 x 2048 4.4 us, most of it a launch's 2.3 and the start of the stream.
+// Bound by what a CU takes from memory, 28 to 32 B/ns, and the start of the
+// stream.  1 x 10240 x 8192 10.2 us, 4.4 TB/s; 1 x 36864 x 7168 23.7, 5.9; 64 x 2048 x
+// 2048 4.4 us, of which a launch is 2.3.
 //
 // kX rows of bf16 or fp16 activations (kX > 0, M <= kX) are quantized by the
 // kernel itself: a lane of the second operand is one scale group of one row,
