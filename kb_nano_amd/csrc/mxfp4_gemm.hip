@@ -4,7 +4,10 @@
 // codes, 16 bytes) of one row and the instruction takes the group's scale byte,
 // so scales cost no arithmetic.
 //
-// Tiled kernel: four wavefronts compute a BM x BN tile, (BM/2) x (BN/2) each.
+// Tiled kernel: WM x WN wavefronts compute a BM x BN tile, four of them for the
+// small tiles, of which a CU holds two, eight for the others: with four, 777 x
+// 4608 x 7168 takes 25.0 us in 128x128 tiles (20.5 with eight) and 47.1 in 256x256
+// (41.4), 4096 x 36864 x 7168 556 (534).
 // Codes go from memory to LDS by direct loads in a ring of kStages stages of
 // 256 K (128 bytes a row: whole lines, as the L2 serves a half line in the time
 // of a whole one, 67 against 133 B/ns for each CU when all read shared data).
@@ -23,8 +26,8 @@
 // for loads.  With 64x128 tiles at 4096 x 8192 x 8192 its return side is busy 89%
 // of the cycles and its address side 79% (128x128 84 and 67%, 256x256 51 and 37%),
 // the matrix pipes 34%, LDS 35%; 44 to 55 B/ns a CU arrive, also where each CU has
-// one tile (200 x 8192 x 8192 19.4 us), whatever the depth of the ring or the row
-// stride.  Two wavefronts a tile instead of four take up to twice as long.
+// one tile (200 x 8192 x 8192 18.5 us), whatever the depth of the ring or the row
+// stride.
 #include "mxfp4_gemm.h"
 
 #include "gemm_kernel.h"
@@ -33,15 +36,16 @@ namespace kbn {
 
 constexpr int kMxStageK = 256, kMxPairK = 512, kMxScaleK = 1024;
 
-template <int BM, int BN, int kStages, int kPerCu>
-__global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArgs p) {
+template <int BM, int BN, int kStages, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void mxfp4_gemm_kernel(const MxGemmArgs p) {
     constexpr int kRows = BM + BN, kStage = kRows * 128, kScaleAt = kStages * kStage;
-    constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 32, FN = TN / 32;
-    constexpr int kDma = kRows / 32;                            // loads of a wavefront per stage: 8 rows each
-    constexpr int kScaleDma = (kRows + 127) / 128;              // and per 1024 K of scales: 32 rows each
-    static_assert(BM % 64 == 0 && BN % 64 == 0 && BM * BN * 2 <= kScaleAt, "epilogue");
+    constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr int kDma = kRows / (8 * kWaves);                  // loads of a wavefront per stage: 8 rows each
+    constexpr int kScaleDma = (kRows + 32 * kWaves - 1) / (32 * kWaves);   // and per 1024 K of scales: 32 rows each
+    static_assert(BM * BN * 2 <= kScaleAt, "epilogue");
+    static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "a load lies in one operand");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kScaleAt + kRows * 32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
 
     int tm, tn, trel, split;
     tile_coords<8>(p.tiles_m, p.tiles_n, 0, p.splits, tm, tn, trel, split);
@@ -60,38 +64,38 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
     const v4i dsA = make_desc(p.sA + (int64_t)m0 * p.ld_sa + k_from / 32, (rows_a - 1) * p.ld_sa + k_len / 32);
     const v4i dsW = make_desc(p.sW + (int64_t)n0 * p.ld_sw + k_from / 32, (rows_w - 1) * p.ld_sw + k_len / 32);
 
-    // Load j of this wavefront: rows 8 q .. 8 q + 7 of the stage, q = 4 j + wave.
+    // Load j of this wavefront: rows 8 q .. 8 q + 7 of the stage, q = kWaves j + wave.
     // 16-byte chunk c of row r lies in slot c ^ swz(r) (the swizzle is applied
     // to the address read, a load's LDS side is contiguous).
     int voff[kDma];
 #pragma unroll
     for (int j = 0; j < kDma; ++j) {
-        const int r = (4 * j + wave) * 8 + (lane >> 3), chunk = (lane & 7) ^ swz(r);
-        voff[j] = (j < BM / 32 ? r * (int)p.lda : (r - BM) * (int)p.ldw) + chunk * 16;
+        const int r = (kWaves * j + wave) * 8 + (lane >> 3), chunk = (lane & 7) ^ swz(r);
+        voff[j] = (j < BM / (8 * kWaves) ? r * (int)p.lda : (r - BM) * (int)p.ldw) + chunk * 16;
     }
     int svoff[kScaleDma];
 #pragma unroll
     for (int j = 0; j < kScaleDma; ++j) {
-        const int r = ((4 * j + wave) * 32 + (lane >> 1)) % kRows;   // 192 rows: some load the same as another wavefront
+        const int r = ((kWaves * j + wave) * 32 + (lane >> 1)) % kRows;   // some may load the same as another wavefront
         svoff[j] = (r < BM ? r * (int)p.ld_sa : (r - BM) * (int)p.ld_sw) + (lane & 1) * 16;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, lds = lds0 + (uint32_t)wave * 1024u;
 
     // Loads of stages past the last fall outside an empty range; in a half stage
     // the lanes of the chunks behind k_len (the same for every j, whose rows
-    // differ by multiples of 32) fall outside as well.
+    // differ by multiples of 16) fall outside as well.
     const int behind = ((lane & 7) ^ swz(wave * 8 + (lane >> 3))) >= 4 ? kOob : 0;
     auto issue = [&](uint32_t base, auto j_, int s) {
         constexpr int j = decltype(j_)::value;
-        v4i d = j < BM / 32 ? dA : dW;
+        v4i d = j < BM / (8 * kWaves) ? dA : dW;
         if (s * kMxStageK >= k_len) d[2] = 0;
-        dma_b128<j * 4096, false>(d, base, voff[j] | (s == whole ? behind : 0), s * 128);
+        dma_b128<j * 1024 * kWaves, false>(d, base, voff[j] | (s == whole ? behind : 0), s * 128);
     };
     auto issue_scales = [&](int c) {   // 1024 K
         static_for<kScaleDma>([&](auto j_) {
             constexpr int j = decltype(j_)::value;
             // the 32 rows of one load lie in one operand
-            const int q = (4 * j + wave) % (kRows / 32);
+            const int q = (kWaves * j + wave) % (kRows / 32);
             v4i d = q < BM / 32 ? dsA : dsW;
             if (c * kMxScaleK >= k_len) d[2] = 0;
             dma_b128<kScaleAt, false>(d, lds0 + (uint32_t)q * 1024u, svoff[j], c * 32);
@@ -108,10 +112,10 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         return *reinterpret_cast<const u32x4*>(smem + kScaleAt + (f < FM ? ra : rw) * 32 + (o & 1) * 16 + (f < FM ? f : f - FM) * 1024);
     };
 
-    // The large tile reads the fragments of one step ahead, under the 16 MFMAs
-    // (512 cycles) of a step.  A smaller one's step is over before the reads of
+    // The large tile reads the fragments of one step ahead, under the 8 MFMAs
+    // (256 cycles) of a step.  A smaller one's step is over before the reads of
     // the next are back, so it reads a whole stage ahead.
-    constexpr bool kWhole = BM + BN <= 256;
+    constexpr bool kWhole = FM + FN <= 4;
     v16f acc[FM][FN] = {};
     constexpr int kR = FM + FN, kT = FM * FN;
     u32x4 f[kWhole ? 8 : 2][kR], raw[kR];
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(256, kPerCu) void mxfp4_gemm_kernel(const MxGemmArg
         // W as the first operand: a lane then holds runs of four columns of one row
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, acc[i][j], 4, 4, op, (int)sc[FM + j][step >> 1], op,
                                                                       (int)sc[i][step >> 1]);
-        keep_here<BM + BN == 512>(acc[i][j][0]);
+        keep_here<false>(acc[i][j][0]);
     };
 
     issue_scales(0);
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(256) void mxfp4_sum_kernel(const MxGemmArgs p) {
     }
 }
 
-template <int BM, int BN, int kStages, int kPerCu>
+template <int BM, int BN, int kStages, int WM, int WN>
 static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStream_t st) {
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
@@ -306,7 +310,7 @@ static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStre
     p.groups_per_split = (groups + plan.splits - 1) / plan.splits;
     p.splits = (groups + p.groups_per_split - 1) / p.groups_per_split;
     p.P = slabs;
-    mxfp4_gemm_kernel<BM, BN, kStages, kPerCu><<<p.tiles_m * p.tiles_n * p.splits, 256, 0, st>>>(p);
+    mxfp4_gemm_kernel<BM, BN, kStages, WM, WN><<<p.tiles_m * p.tiles_n * p.splits, WM * WN * 64, 0, st>>>(p);
     KBN_CHECK_LAUNCH("mxfp4_gemm_nt");
     if (p.splits > 1) {
         const int64_t lanes = (int64_t)p.tiles_m * p.tiles_n * BM * (BN / 4);
@@ -318,22 +322,22 @@ static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStre
 
 // Prices, in us, of the tiles: fixed cost, a further round of workgroups, a
 // stage of 256 K where each CU has one workgroup, one where it has several (a
-// workgroup's share), fitted to 72 shapes (M 40 .. 2048, eight weights) and
-// three split counts timed in graphs; 12% off each, but the tile picked is
-// 0.9% slower than the best one on average, 12% at most.  Each tile carries
-// shapes: 777 x 4608 x 7168 takes 24.3 us with 64x128 against 25.7, 29.4 and 47.8,
-// 4096 x 36864 x 7168 571 with 256x256 against 733, 924 and 1167, 320 x 1000 x
-// 4096 7.2 with 64x64 against 8.7 and 12.3, 777 x 7168 x 18432 84 with 128x128
-// against 97 with 64x128.
+// workgroup's share), fitted to 96 shapes (M 20 .. 4096, eight weights) and four
+// split counts timed in graphs; 14% off each, but the tile picked is 0.3%
+// slower than the best one on average, 6% at most.  Each tile carries shapes (us
+// with 64x64, 64x128, 128x128, 128x256, 256x256): 320 x 1000 x 4096 7.19 / 8.94 / 11.2 / 16.9 / 24.9, 65 x 24576 x
+// 1536 9.58 / 8.61 / 8.24 / 10 / 13.5, 777 x 4608 x 7168 28.7 / 23.3 / 20.1 / 26.1 / 41.8, 777 x 8192 x 8192 60.4 / 50 / 43.1 / 35.5 / 49.8, 4096 x 36864 x
+// 7168 1.17e+03 / 919 / 824 / 667 / 547.
 struct TilePrice {
     int bm, bn, per_cu;
     double fixed, round, stage_one, stage_many;
 };
 static const TilePrice kTiles[] = {
-    {64, 64, 2, 2.8, 1.2, 0.323, 0.272},
-    {64, 128, 2, 3.1, 1.65, 0.466, 0.40},
-    {128, 128, 2, 2.9, 3.0, 0.826, 0.567},
-    {256, 256, 1, 7.5, 8.8, 1.5, 1.7},
+    {64, 64, 2, 3.07, 0.975, 0.275, 0.275},
+    {64, 128, 2, 3.03, 1.45, 0.458, 0.407},
+    {128, 128, 1, 3.37, 1.81, 0.555, 0.655},
+    {128, 256, 1, 4.6, 4.3, 0.758, 0.835},
+    {256, 256, 1, 6.74, 4.43, 1.25, 1.42},
 };
 constexpr double kSplitFixed = 3.0, kSplitMb = 0.35;   // the sum's launch, and each MB of partial sums
 
@@ -366,7 +370,7 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K) {
     }
     for (const TilePrice& t : kTiles) {
         const int64_t tiles_m = ceil_div(M, t.bm), tiles = tiles_m * ceil_div(N, t.bn);
-        const double cold = tiles_m == 1 ? 1.15 : 1.0;   // one row of tiles: every weight line comes from memory
+        const double cold = tiles_m == 1 ? 1.1 : 1.0;   // one row of tiles: every weight line comes from memory
         for (int splits = 1; splits <= 4 && splits <= groups; ++splits) {
             const int64_t per = ceil_div(groups, splits), used = ceil_div(groups, per);
             if (used != splits) continue;
@@ -390,10 +394,11 @@ int64_t mxfp4_plan_bytes(const MxPlan& p, int64_t M, int64_t N) {
 int mxfp4_gemm_launch(MxGemmArgs& p, float* slabs, hipStream_t st) {
     const MxPlan plan = mxfp4_plan(p.M, p.N, p.K);
     if (plan.rf) return mxfp4_rows_launch(p, plan.rf, kMxBf16, st);
-    if (plan.bm == 256) return launch_tiled<256, 256, 2, 1>(p, plan, slabs, st);
-    if (plan.bm == 128) return launch_tiled<128, 128, 2, 2>(p, plan, slabs, st);
-    if (plan.bn == 128) return launch_tiled<64, 128, 3, 2>(p, plan, slabs, st);
-    return launch_tiled<64, 64, 4, 2>(p, plan, slabs, st);
+    if (plan.bm == 256) return launch_tiled<256, 256, 2, 2, 4>(p, plan, slabs, st);
+    if (plan.bn == 256) return launch_tiled<128, 256, 3, 2, 4>(p, plan, slabs, st);
+    if (plan.bm == 128) return launch_tiled<128, 128, 4, 4, 2>(p, plan, slabs, st);
+    if (plan.bn == 128) return launch_tiled<64, 128, 3, 2, 2>(p, plan, slabs, st);
+    return launch_tiled<64, 64, 4, 2, 2>(p, plan, slabs, st);
 }
 
 }  // namespace kbn

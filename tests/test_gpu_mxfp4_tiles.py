@@ -11,10 +11,13 @@ pytestmark = pytest.mark.gpu
 SHAPES = [(17, 67, 640), (33, 65, 640), (51, 67, 1152), (17, 4141, 640), (34, 4183, 1152), (49, 4331, 1152),   # few rows:
           (18, 8295, 1664), (35, 8213, 1664), (16, 8195, 1408), (1, 8209, 1152), (54, 8235, 1664),   # 16, 32, 48
           (2, 12305, 640), (17, 12841, 1664), (34, 12677, 1664), (64, 9001, 2176),        # and 64 wide
-          (74, 67, 3200), (75, 67, 4352), (2930, 65, 6784), (65, 130, 2176),              # 64 x 64: in 4, 3, 2 splits, 1
-          (2765, 73, 7296), (17, 8227, 18432), (3637, 131, 17280), (65, 16571, 1152),      # 64 x 128
-          (3714, 261, 16256), (65, 16401, 8832), (139, 11375, 12032), (1025, 2051, 640),  # 128 x 128
-          (2704, 907, 19072), (3300, 1185, 10368), (816, 5399, 16000), (913, 12331, 640)]  # 256 x 256
+          # 64 x 64, 64 x 128, 128 x 128, 128 x 256 and 256 x 256 in 1 to 4 splits
+          (65, 130, 2176), (2858, 67, 7808), (75, 67, 4352), (75, 67, 3712), (74, 67, 3200), (2930, 65, 6784), (2765, 73, 7296),
+          (17, 16627, 128), (129, 24579, 1152), (17, 8227, 18432), (2793, 65, 11904),
+          (1025, 2051, 640), (65, 16571, 1152), (1100, 2050, 2432), (65, 16401, 8832), (139, 11375, 12032), (3714, 261, 16256),
+          (2143, 449, 7296), (3637, 131, 17280),
+          (258, 13153, 128), (816, 5399, 16000), (3300, 1185, 10368), (2704, 907, 19072), (66, 17429, 12160), (69, 11363, 13440),
+          (913, 12331, 640), (3410, 2319, 1408), (129, 17445, 22912)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
