@@ -19,15 +19,14 @@
 // read and frees it for the loads of the stage kStages ahead, which are spread
 // over the MFMA slots behind it.
 //
-// What bounds it.  Large products: power.  4096 x 36864 x 7168 runs at 3.8
-// PFLOP/s with the matrix pipes busy half of the cycles at the 1.6 to 1.8 GHz
-// that the card then holds, and waits for data in 12%; the same instructions
-// alone on random operands reach 5.6 to 6.  Smaller tiles: the CU's path
-// for loads.  With 64x128 tiles at 4096 x 8192 x 8192 its return side is busy 89%
-// of the cycles and its address side 79% (128x128 84 and 67%, 256x256 51 and 37%),
-// the matrix pipes 34%, LDS 35%; 44 to 55 B/ns a CU arrive, also where each CU has
-// one tile (200 x 8192 x 8192 18.5 us), whatever the depth of the ring or the row
-// stride.
+// What bounds it.  Large products: power, and the CU's path for loads.  4096 x
+// 36864 x 7168 takes 534 us, 4.05 PFLOP/s, at the 1.76 GHz that the card then
+// holds; the matrix pipes are busy 55% of the cycles, the load path's return side
+// 79%.  The same instructions alone on random operands reach 5.6 to 6 PFLOP/s.
+// Smaller tiles: the load path.  With 64x128 tiles at 4096 x 8192 x 8192 its
+// return side is busy 89%, its address side 79%, the matrix pipes 34%, LDS 35%;
+// 44 to 55 B/ns a CU arrive, also where each CU has one tile (200 x 8192 x 8192
+// 18.5 us), whatever the depth of the ring or the row stride.
 #include "mxfp4_gemm.h"
 
 #include "gemm_kernel.h"
