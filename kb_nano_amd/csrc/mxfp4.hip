@@ -177,14 +177,16 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int
 // quantizes them for itself.  us, one launch / two: 1 x 10240 x 8192 10.2 / 11.9, 4 x
 // 10240 x 8192 10.7 / 12.0, 4 x 2048 x 2048 3.9 / 5.1, 4 x 36864 x 7168 26.5 / 26.3; 8
 // rows 2048 x 2048 4.1 / 4.9, 10240 x 8192 11.5 / 12.2, 4608 x 7168 8.7 / 8.5, but
-// 36864 x 7168 32.0 / 26.9: up to 8 where every CU has one workgroup.
-static bool linear_fused(int64_t M, int64_t N, int x_dtype) {
-    return x_dtype != kMxF32 && (M <= 4 || (M <= 8 && N <= 48 * cu_count()));
+// 36864 x 7168 32.0 / 26.9: up to 8 where every CU has one workgroup.  16 rows 2048 x
+// 2048 4.8 / 5.0, 7168 x 2048 5.7 / 6.0, 4096 x 4096 6.5 / 6.2, 8192 x 8192 11.7 / 10.9:
+// there up to K = 2048.
+static bool linear_fused(int64_t M, int64_t N, int64_t K, int x_dtype) {
+    return x_dtype != kMxF32 && (M <= 4 || (N <= 48 * cu_count() && (M <= 8 || (M <= 16 && K <= 2048))));
 }
 static int64_t linear_operand_bytes(int64_t M, int64_t K) { return (M * (K / 2 + K / kMxGroup) + 255) / 256 * 256; }
 
 extern "C" int64_t kbn_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || linear_fused(M, N, x_dtype)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || linear_fused(M, N, K, x_dtype)) return 0;
     return linear_operand_bytes(M, K) + kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
 }
 
@@ -200,7 +202,7 @@ extern "C" int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const 
     const int64_t need = kbn_mxfp4_linear_workspace_bytes(M, N, K, x_dtype);
     KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
                   what, (long long)need, (long long)workspace_bytes);
-    if (linear_fused(M, N, x_dtype)) {
+    if (linear_fused(M, N, K, x_dtype)) {
         MxGemmArgs p{nullptr, ld_x, nullptr, 0, (const uint8_t*)W, ldw, (const uint8_t*)sW, ld_sw, (uint16_t*)D, ldd,
                      (int)M, (int)N, (int)K};
         p.X = x;

@@ -208,7 +208,7 @@ template <int CG, int kX, int kIn>
 static int launch_for(const MxGemmArgs& p, int rf, hipStream_t st) {
     if (rf == 1) return launch<1, CG, kX, kIn>(p, st);
     if (rf == 2) return launch<2, CG, kX, kIn>(p, st);
-    if constexpr (CG < 4 && kX < 8)   // 64 rows have a cheaper tile, 8 rows of values come with N <= 48 CUs
+    if constexpr (CG < 4 && kX < 8)   // 64 rows have a cheaper tile, 5 to 16 rows of values come with N <= 48 CUs
         if (rf == 4) return launch<4, CG, kX, kIn>(p, st);
     return launch<3, CG, kX, kIn>(p, st);
 }
@@ -217,7 +217,8 @@ template <int kIn>
 static int launch_values(const MxGemmArgs& p, int rf, hipStream_t st) {
     if (p.M <= 2) return launch_for<1, 2, kIn>(p, rf, st);
     if (p.M <= 4) return launch_for<1, 4, kIn>(p, rf, st);
-    return launch_for<1, 8, kIn>(p, rf, st);
+    if (p.M <= 8) return launch_for<1, 8, kIn>(p, rf, st);
+    return launch_for<1, 16, kIn>(p, rf, st);
 }
 
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st) {

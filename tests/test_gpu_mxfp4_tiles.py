@@ -95,7 +95,7 @@ def test_past_32_bit_offsets(gpu_device):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M", range(1, 10))
+@pytest.mark.parametrize("M", [*range(1, 10), 13, 16, 17])
 @pytest.mark.parametrize("N,K", [(67, 128), (515, 1152), (4357, 640), (9001, 1408), (12999, 384)])
 def test_linear_of_few_rows(gpu_device, M, N, K, dtype):
     """One launch or two: the bits of the quantization and the product apart, in strided rows, with values
