@@ -13,12 +13,13 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr int kQuantThreads = 256;
 
 // A lane takes eight values of kRows rows, four lanes a group.  Memory bound.
-// Many 16-bit rows go four at a time, for more loads in flight, and are read as
-// values that are not needed again (us, one row at a time / four: 8192 x 18432
-// 66.1 / 59.7, which is 6.4 TB/s, 4096 x 7168 16.7 / 13.9, 512 x 18432 6.5 / 6.2,
-// but 1024 x 7168 4.8 / 5.6).  fp32 rows are wide enough one at a time: 8192 x
-// 8192 53.0 us, 5.7 TB/s, against 55.7.
-template <int kIn, int kRows>
+// Many values (9 Mi and more) are read as ones that are not needed again (kOnce),
+// which leaves the caches to the codes and to what was written last, and 16-bit
+// rows four at a time, for more loads in flight.  us, without / with: 8192 x 18432
+// bf16 66.1 / 59.7, which is 6.4 TB/s, 4096 x 7168 16.7 / 13.9, 512 x 18432 6.5 / 6.2,
+// but 1024 x 7168 4.8 / 5.6; 8192 x 8192 fp32 and back 134.7 / 104.9 (alone 53.0 /
+// 54.3; four rows 55.7).
+template <int kIn, int kRows, bool kOnce>
 __global__ __launch_bounds__(kQuantThreads) void mxfp4_quant_kernel(const void* x, int64_t ld_x, int64_t M, int64_t K,
                                                                    uint8_t* codes, int64_t ld_c, uint8_t* scales,
                                                                    int64_t ld_s) {
@@ -27,7 +28,7 @@ __global__ __launch_bounds__(kQuantThreads) void mxfp4_quant_kernel(const void* 
     for (int64_t m0 = (int64_t)blockIdx.y * kRows; m0 < M; m0 += (int64_t)gridDim.y * kRows) {
         uint32_t w[kRows][kIn == kMxF32 ? 8 : 4];
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) mx_load8<kIn, (kRows > 1)>(x, (m0 + r < M ? m0 + r : M - 1) * ld_x + k, w[r]);
+        for (int r = 0; r < kRows; ++r) mx_load8<kIn, kOnce>(x, (m0 + r < M ? m0 + r : M - 1) * ld_x + k, w[r]);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const int64_t m = m0 + r;
@@ -102,11 +103,11 @@ static int quant_args(const char* what, int dtype, int64_t M, int64_t K) {
 
 static int quant_launch(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, void* codes, int64_t ld_c,
                         void* scales, int64_t ld_s, hipStream_t st) {
-    const bool many = x_dtype != kMxF32 && M * K >= 9 << 20;
-    auto* const kernel = x_dtype == kMxF32    ? mxfp4_quant_kernel<kMxF32, 1>
-                         : x_dtype == kMxBf16 ? many ? mxfp4_quant_kernel<kMxBf16, 4> : mxfp4_quant_kernel<kMxBf16, 1>
-                         : many               ? mxfp4_quant_kernel<kMxF16, 4> : mxfp4_quant_kernel<kMxF16, 1>;
-    kernel<<<quant_grid(M, K, many ? 4 : 1), kQuantThreads, 0, st>>>(x, ld_x, M, K, (uint8_t*)codes, ld_c, (uint8_t*)scales, ld_s);
+    const bool many = M * K >= 9 << 20;
+    auto* const kernel = x_dtype == kMxF32    ? many ? mxfp4_quant_kernel<kMxF32, 1, true> : mxfp4_quant_kernel<kMxF32, 1, false>
+                         : x_dtype == kMxBf16 ? many ? mxfp4_quant_kernel<kMxBf16, 4, true> : mxfp4_quant_kernel<kMxBf16, 1, false>
+                         : many               ? mxfp4_quant_kernel<kMxF16, 4, true> : mxfp4_quant_kernel<kMxF16, 1, false>;
+    kernel<<<quant_grid(M, K, many && x_dtype != kMxF32 ? 4 : 1), kQuantThreads, 0, st>>>(x, ld_x, M, K, (uint8_t*)codes, ld_c, (uint8_t*)scales, ld_s);
     KBN_CHECK_LAUNCH("mxfp4_quant");
     return 0;
 }
