@@ -140,3 +140,46 @@ def test_refusals_reach_the_caller(gpu_device):
         call(d, block=[128, 64])
     with pytest.raises(RuntimeError, match="top_k=33"):
         call(d, ids=d["ids"][:, :1].repeat(1, 33), tw=d["tw"][:, :1].repeat(1, 33))
+
+
+def test_threads_at_once_and_packed_dtype(gpu_device):
+    """Calls of several threads on one stream and on their own, and codes as float4_e2m1fn_x2: the bits of
+    one call alone."""
+    import threading
+    from kb_nano_amd import FewTokenExperts, Mxfp4Linear, Mxfp4Quant, dequantize_mxfp4
+    print("mxfp4 threads", flush=True)
+    quant, lin, few = Mxfp4Quant(), Mxfp4Linear(), FewTokenExperts()
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(40, 512, generator=g).bfloat16().to(gpu_device)
+    w, sw = quant((torch.randn(4, 512, 512, generator=g) * 0.05).to(gpu_device))
+    w13, s13, w2, s2 = w, sw, w[:, :, :128].contiguous(), sw[:, :, :8].contiguous()
+    ids = torch.randint(0, 4, (40, 2), generator=g).to(torch.int32).to(gpu_device)
+    tw = torch.rand(40, 2, generator=g).to(gpu_device)
+
+    def calls(n):
+        return lin(x[:n], w[0], sw[0]), few(x[:n], w13, w2, tw[:n], ids[:n], 4, s13, s2, [1, 32]), *quant(x[:n])
+
+    rows = (1, 7, 30, 40)
+    refs = [calls(n) for n in rows]
+    f4 = torch.float4_e2m1fn_x2
+    assert torch.equal(lin(x, w[0].view(f4), sw[0]), refs[3][0])
+    assert torch.equal(dequantize_mxfp4(refs[3][2].view(f4), refs[3][3]), dequantize_mxfp4(refs[3][2], refs[3][3]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k, own):
+        stream = torch.cuda.Stream() if own else torch.cuda.current_stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                for a, b in zip(calls(rows[k]), refs[k]):
+                    if not torch.equal(a.view(torch.uint8), b.view(torch.uint8)):
+                        wrong.append((k, own))
+
+    for own in (False, True):
+        threads = [threading.Thread(target=work, args=(k, own)) for k in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong
