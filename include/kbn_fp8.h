@@ -468,6 +468,7 @@ int kbn_fp8_block_requant(const void* w_in, int in_f32, const float* s_in, int64
  *   codes   uint8 [M, K/2], two codes a byte, even k in the low nibble; row
  *           stride in bytes, a multiple of 4
  *   scales  uint8 [M, K/32], E8M0: the group's scale is 2^(byte - 127)
+ *   Rows may lie any distance apart.
  *   Per group: a = max|x| rounded to one mantissa bit (ties up); byte =
  *   exponent(a) - 2, biased, at least 1; codes = x / scale to the nearest, ties to
  *   even, at most 6 in magnitude.  A group that holds an infinity or a NaN gets
@@ -488,7 +489,8 @@ int kbn_mxfp4_dequant(const void* codes, int64_t ld_codes, const void* scales, i
  *   D[m, n] = bf16_rne( sum_g sA[m,g] sW[n,g] sum_{k in g} A[m,k] W[n,k] ), fp32 sums
  *   A codes [M, K/2] and scales [M, K/32], W codes [N, K/2] and scales
  *   [N, K/32], K % 128 == 0; code rows 16-byte, scale rows 4-byte aligned
- *   (strides in bytes, multiples of 16 and 4); D bf16 [M, N], row stride ldd.
+ *   (strides in bytes, multiples of 16 and 4, below 2^23); D bf16 [M, N], row
+ *   stride ldd.  M and N up to 2^30.
  * The workspace (bytes as asked for the shape, may be 0) is 16-byte aligned.
  */
 int64_t kbn_mxfp4_gemm_nt_workspace_bytes(int64_t M, int64_t N, int64_t K);
@@ -497,7 +499,8 @@ int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int64_t ld_sa,
                       int64_t workspace_bytes, void* stream);
 
 /* kbn_mxfp4_quant of x [M, K], then kbn_mxfp4_gemm_nt with W: the same bits.
- * x as for the quant, with K % 128 == 0. */
+ * x as for the quant, with K % 128 == 0; where the workspace is 0 bytes (few
+ * rows, quantized by the product's launch) its row stride is below 2^23. */
 int64_t kbn_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_dtype);
 int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const void* W, int64_t ldw, const void* sW, int64_t ld_sw,
                      void* D, int64_t ldd, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
@@ -510,7 +513,8 @@ int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const void* W, in
  *   out[t] = sum_e c[t,e] W2_e (silu(G_e x_t) * (U_e x_t)),  w13[e] = [G_e | U_e]
  *   c[t,e] = sum of topk_weights[t, j] over the slots j with topk_ids[t, j] == e;
  *   ids outside [0, E) count for nothing (a token with none gets zeros).
- *   x            [T, H] of x_dtype (0 bf16, 1 fp16), rows 16-byte aligned; T <= 64
+ *   x            [T, H] of x_dtype (0 bf16, 1 fp16), rows 16-byte aligned, row
+ *                stride a multiple of 8 below 2^24; T <= 64
  *   w_format     0: w13 fp8 [E, 2I, H], w2 fp8 [E, H, I], fp32 scales
  *                   [E, 2I/128, H/128] and [E, H/128, I/128], used as given
  *                1: MXFP4 codes [E, 2I, H/2] and [E, H, I/2], scales

@@ -905,6 +905,15 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+FAR_ROWS = 1 << 23   # elements from row to row that the kernels' 32-bit offsets do not reach
+
+
+def _near(x: torch.Tensor) -> torch.Tensor:
+    """``x``, copied where its rows lie far apart (the last token of each of some
+    long sequences): for kernels that few rows go to."""
+    return x.contiguous() if _ld(x) >= FAR_ROWS else x
+
+
 def _mx_types(what: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
     if codes.dtype not in MX_CODES:
         raise TypeError(f"{what}: {name} codes must be uint8 or float4_e2m1fn_x2 (two a byte), got {codes.dtype}")
@@ -1001,7 +1010,10 @@ def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tens
     L = lib()
     code = _QUANT_IN[x.dtype]
     nbytes = L.kbn_mxfp4_linear_workspace_bytes(M, N, K, code)
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    if nbytes:
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    else:   # the product reads x itself
+        x, buf = _near(x), None
     check(L.kbn_mxfp4_linear(x.data_ptr(), code, _ld(x), weight.data_ptr(), _ld(weight),
                              weight_scale.data_ptr(), _ld(weight_scale), output.data_ptr(), _ld(output),
                              M, N, K, buf.data_ptr() if nbytes else None, nbytes, _stream(x)), what)
@@ -1057,6 +1069,7 @@ def few_token_experts(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tenso
     _mx_rows(what, "output", out, (T, H))
     if T == 0:
         return
+    x = _near(x)
     L = lib()
     nbytes = L.kbn_few_token_experts_workspace_bytes(T, topk, inter)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)

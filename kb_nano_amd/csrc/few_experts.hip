@@ -750,7 +750,8 @@ extern "C" int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, c
                       E * (I / 8) < (1LL << 31),
                   "%s: H=%lld and I=%lld are too large", what, (long long)H, (long long)I);
     if (T == 0) return 0;
-    KBN_CHECK_ARG(ld_x >= H && ld_x % 8 == 0 && ld_x < (1 << 24) && x && aligned16(x), "%s: input rows must be 16-byte aligned", what);
+    KBN_CHECK_ARG(ld_x >= H && ld_x % 8 == 0 && x && aligned16(x), "%s: input rows must be 16-byte aligned", what);
+    KBN_CHECK_ARG(ld_x < (1 << 24), "%s: input row stride %lld is too large", what, (long long)ld_x);
     KBN_CHECK_ARG(ld_out >= H && out && reinterpret_cast<uintptr_t>(out) % 2 == 0, "%s: output row stride %lld below H=%lld", what,
                   (long long)ld_out, (long long)H);
     KBN_CHECK_ARG(w13 && w2 && s13 && s2 && topk_weights && topk_ids, "%s: null pointer", what);

@@ -82,12 +82,13 @@ static dim3 quant_grid(int64_t M, int64_t K, int rows = 1) {
     return dim3((unsigned)((K / 8 + kQuantThreads - 1) / kQuantThreads), (unsigned)std::min<int64_t>((M + rows - 1) / rows, 32768));
 }
 
+// Rows that a product reads (`near`) are at 32-bit offsets from their tile's
+// first; other rows may lie any distance apart.
 static int check_rows(const char* what, const char* name, int64_t ld, int64_t least, int64_t multiple, const void* ptr,
-                      int64_t align) {
+                      int64_t align, bool near = false) {
     KBN_CHECK_ARG(ld >= least && ld % multiple == 0, "%s: %s row stride %lld must be a multiple of %lld and at least %lld", what,
                   name, (long long)ld, (long long)multiple, (long long)least);
-    // a tile's row offsets are 32-bit
-    KBN_CHECK_ARG(ld < (1LL << 31) / 256, "%s: %s row stride %lld is too large", what, name, (long long)ld);
+    KBN_CHECK_ARG(!near || ld < (1LL << 31) / 256, "%s: %s row stride %lld is too large", what, name, (long long)ld);
     KBN_CHECK_ARG(ptr && reinterpret_cast<uintptr_t>(ptr) % align == 0, "%s: %s must be %lld-byte aligned", what, name,
                   (long long)align);
     return 0;
@@ -113,7 +114,8 @@ static int quant_launch(const void* x, int x_dtype, int64_t M, int64_t K, int64_
 }
 
 static int gemm_args(const char* what, int64_t M, int64_t N, int64_t K) {
-    KBN_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && M < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31),
+    // rows and columns are counted in 32 bits, a tile past the last ones too
+    KBN_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && M <= (1LL << 30) && N <= (1LL << 30) && K < (1LL << 31),
                   "%s: bad size M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
     KBN_CHECK_ARG(K % 128 == 0, "%s: K=%lld must be a multiple of 128", what, (long long)K);
     return 0;
@@ -161,8 +163,8 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int
     const char* what = "mxfp4_gemm_nt";
     if (gemm_args(what, M, N, K)) return 1;
     if (M == 0 || N == 0) return 0;
-    if (check_rows(what, "A", lda, K / 2, 16, A, 16) || check_rows(what, "A scales", ld_sa, K / kMxGroup, 4, sA, 4) ||
-        check_rows(what, "W", ldw, K / 2, 16, W, 16) || check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4) ||
+    if (check_rows(what, "A", lda, K / 2, 16, A, 16, true) || check_rows(what, "A scales", ld_sa, K / kMxGroup, 4, sA, 4, true) ||
+        check_rows(what, "W", ldw, K / 2, 16, W, 16, true) || check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4, true) ||
         check_rows(what, "output", ldd, N, 1, D, 2))
         return 1;
     const int64_t need = kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K);
@@ -197,8 +199,9 @@ extern "C" int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const 
     const char* what = "mxfp4_linear";
     if (quant_args(what, x_dtype, M, K) || gemm_args(what, M, N, K)) return 1;
     if (M == 0 || N == 0) return 0;
-    if (check_rows(what, "input", ld_x, K, 8, x, 16) || check_rows(what, "W", ldw, K / 2, 16, W, 16) ||
-        check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4) || check_rows(what, "output", ldd, N, 1, D, 2))
+    if (check_rows(what, "input", ld_x, K, 8, x, 16, linear_fused(M, N, K, x_dtype)) ||
+        check_rows(what, "W", ldw, K / 2, 16, W, 16, true) || check_rows(what, "W scales", ld_sw, K / kMxGroup, 4, sW, 4, true) ||
+        check_rows(what, "output", ldd, N, 1, D, 2))
         return 1;
     const int64_t need = kbn_mxfp4_linear_workspace_bytes(M, N, K, x_dtype);
     KBN_CHECK_ARG(workspace_bytes >= need && (need == 0 || aligned16(workspace)), "%s: workspace of %lld bytes needed, got %lld",
