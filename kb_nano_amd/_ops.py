@@ -1046,7 +1046,9 @@ def few_token_experts(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tenso
     E, N2 = w13.shape[:2]
     inter = N2 // 2
     if T > FEW_TOKENS:
-        raise ValueError(f"{what}: {T} tokens, at most {FEW_TOKENS}; VllmFusedExperts and FusedExperts take more")
+        more = ("VllmFusedExperts and FusedExperts take more" if w13.dtype is FP8
+                else "larger batches of MXFP4 weights go in parts")
+        raise ValueError(f"{what}: {T} tokens, at most {FEW_TOKENS}; {more}")
     if H % GROUP or N2 % (2 * GROUP) or H == 0 or N2 == 0:
         raise ValueError(f"{what}: H={H} and I={N2 / 2:g} must be multiples of {GROUP}")
     fp8 = w13.dtype is FP8

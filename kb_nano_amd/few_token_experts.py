@@ -4,7 +4,8 @@ Stands beside ``VllmFusedExperts`` (same ``forward`` arguments) for at most 64
 tokens: one launch for the gate and up products with SiLU*Mul, one for the down
 product with the routed sum.  The activations are not quantized, so its
 results are nearer to the exact ones than those of the FP8 x FP8 chain, and
-the weights may also be MXFP4.
+the weights may also be MXFP4.  No other layer takes MXFP4 experts: more tokens
+go through them 64 at a time, and each call reads the named experts' weights.
 """
 from __future__ import annotations
 
