@@ -568,6 +568,16 @@ int kbn_debug_splitk_regions(int64_t n_keys, int32_t* out_region, int64_t* out_f
 int kbn_debug_gemm_plan(int64_t M, int64_t N, int64_t K, int scale_ue8m0, int bf16a, int64_t* out);
 
 /*
+ * Test hook (no counterpart in the reference): what kbn_mxfp4_linear would
+ * launch for x_dtype (0 .. 2), or kbn_mxfp4_gemm_nt (-1), without a GPU (256 CUs
+ * are assumed when none is present).  out[0..5] = tile rows, tile columns (0 for
+ * the kernel of few rows), K splits, weight rows of its workgroups in 16s (0 for
+ * the tiles), rows of values that it quantizes itself (0: another launch does),
+ * and workspace bytes.
+ */
+int kbn_debug_mxfp4_plan(int64_t M, int64_t N, int64_t K, int x_dtype, int64_t* out);
+
+/*
  * Test hook (no counterpart in the reference): the kernels' bf16 SiLU
  * applied elementwise to n bf16 bit patterns, for exhaustive checking.
  * path 0 reads the table as the SiLU*Mul + quant kernels do; path 1 reads it

@@ -218,3 +218,15 @@ extern "C" int kbn_mxfp4_linear(const void* x, int x_dtype, int64_t ld_x, const 
                  (int)M, (int)N, (int)K};
     return mxfp4_gemm_launch(p, (float*)rest, (hipStream_t)stream);
 }
+
+extern "C" int kbn_debug_mxfp4_plan(int64_t M, int64_t N, int64_t K, int x_dtype, int64_t* out) {
+    const char* what = "debug_mxfp4_plan";
+    KBN_CHECK_ARG(out && M > 0 && N > 0 && x_dtype >= -1 && x_dtype <= 2, "%s: bad arguments", what);
+    if (gemm_args(what, M, N, K)) return 1;
+    const MxPlan plan = mxfp4_plan(M, N, K);
+    const bool fused = x_dtype >= 0 && linear_fused(M, N, K, x_dtype);
+    const int64_t v[6] = {plan.bm, plan.bn, plan.splits, plan.rf, fused ? mxfp4_value_rows(M) : 0,
+                          x_dtype < 0 ? kbn_mxfp4_gemm_nt_workspace_bytes(M, N, K) : kbn_mxfp4_linear_workspace_bytes(M, N, K, x_dtype)};
+    std::copy(v, v + 6, out);
+    return 0;
+}

@@ -32,6 +32,9 @@ MxPlan mxfp4_plan(int64_t M, int64_t N, int64_t K);
 // Bytes of the partial sums.
 int64_t mxfp4_plan_bytes(const MxPlan& plan, int64_t M, int64_t N);
 
+// Rows of values that the few-rows kernel's variant for M of them holds.
+inline int mxfp4_value_rows(int64_t M) { return M <= 2 ? 2 : M <= 4 ? 4 : M <= 8 ? 8 : 16; }
+
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st);
 int mxfp4_gemm_launch(MxGemmArgs& p, float* slabs, hipStream_t st);
 

@@ -215,10 +215,12 @@ static int launch_for(const MxGemmArgs& p, int rf, hipStream_t st) {
 
 template <int kIn>
 static int launch_values(const MxGemmArgs& p, int rf, hipStream_t st) {
-    if (p.M <= 2) return launch_for<1, 2, kIn>(p, rf, st);
-    if (p.M <= 4) return launch_for<1, 4, kIn>(p, rf, st);
-    if (p.M <= 8) return launch_for<1, 8, kIn>(p, rf, st);
-    return launch_for<1, 16, kIn>(p, rf, st);
+    switch (mxfp4_value_rows(p.M)) {
+        case 2: return launch_for<1, 2, kIn>(p, rf, st);
+        case 4: return launch_for<1, 4, kIn>(p, rf, st);
+        case 8: return launch_for<1, 8, kIn>(p, rf, st);
+        default: return launch_for<1, 16, kIn>(p, rf, st);
+    }
 }
 
 int mxfp4_rows_launch(const MxGemmArgs& p, int rf, int x_dtype, hipStream_t st) {
