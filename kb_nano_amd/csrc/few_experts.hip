@@ -15,10 +15,17 @@
 // scales pass fp16's range, and h, which has fp32's) goes as a pair of bf16
 // values, x = hi + lo, hi the nearest and lo the nearest to the rest: 16 bits
 // and more, for one more matrix instruction on weights that are there already.
-// Bound by the weight stream, which a large read reaches 6.6 TB/s with: 64 tokens
-// over 256 experts (7168, 2048) 1439 us, 6.8 TB/s; 16 of fp16 over 128 (4096, 1536)
-// 243 us, 6.3; 5 over those in MXFP4 69 us, 5.1; one token on an eighth of the
-// 256, 44 MB, 14.6 us, of which two launches and their joins are about six.
+// Few rows an expert: bound by the weight stream, which a large read reaches 6.6
+// TB/s with: 64 tokens over 256 experts (7168, 2048) 1440 to 1475 us, 6.6 to 6.8
+// TB/s; 16 of fp16 over 128 (4096, 1536) 243 to 254 us, 6.0 to 6.3; 5 over those in
+// MXFP4 69 us, 5.1; one token on an eighth of the 256, 44 MB, 14.8 us, of which two
+// launches and their joins are about six.  fp16 activations of MXFP4 weights take
+// twice the matrix instructions: 5 tokens 112 us (bf16 in the same run 74), 64 over
+// 64 (7168, 1024) 329 (237).
+// Many rows an expert: 2 to 5 times the weights' time (64 tokens over 8 experts
+// (4096, 14336), 16 rows each, 443 us against 214), as a stage's activations serve
+// 16 or 32 weight rows only and more than 16 rows read the weights again; the
+// sorted-token layer is faster there.
 //
 // Both kernels stream like the few-rows MXFP4 product: each wavefront has a
 // private LDS ring filled by direct loads of whole 128-byte weight lines (a
@@ -467,7 +474,7 @@ __global__ __launch_bounds__(kWaves * 64) void gate_up_kernel(const ExpertsArgs 
 // Workgroup: `cols` output columns (at most 16 RF, a multiple of 4) of every
 // token.  The stages of all passes form
 // one sequence, cut into a run for each wavefront; a pass's sums are weighted
-// and added to the wavefront's [T][16] sums in LDS when the run leaves it, and
+// and added to the wavefront's [T][16 RF] sums in LDS when the run leaves it, and
 // the wavefronts' are added in their order at the end.
 template <int kW, bool kF16, int kR, int RF, int kWaves, int kDepth>
 __global__ __launch_bounds__(kWaves * 64) void down_kernel(const ExpertsArgs p, int cols) {
@@ -681,6 +688,12 @@ static int launch_gate_up(const ExpertsArgs& p, double active, int down_rows, hi
 // with an eighth of h's columns, 239 / 221 / 238, 4 (MXFP4) 362 / 313 / 294, (FP8) 439
 // with 8, 439 with 16, 8 (FP8) 347 and 326, (MXFP4) 285 and 262, 16 (FP8) 642 and
 // 560, (MXFP4) 452 and 411.
+//
+// Pass sizes go by uniform routing with every id inside [0, E).  Other routings give the
+// same results from kernels for more or fewer rows than they have, us of 64 tokens,
+// 8 a token, (7168, 2048), FP8 / MXFP4: 32 of 256 experts here and the other ids
+// outside, 77 to 80 rows, 225 / 206 (16 rows a pass where an expert has two or
+// three); all tokens on the same 8 of 256 experts 651 / 495, on 64 of them 810 / 577.
 //
 // Columns of a down workgroup: 16, but for an H between 16 and 32 columns a CU
 // as many as give every CU one workgroup, in two fragments: with 16 columns

@@ -152,9 +152,13 @@ __device__ __forceinline__ v4i make_desc(const void* base, int64_t bytes) {
 // other stages; completion is awaited explicitly (wait_dma_n) before the
 // barrier that publishes a stage.  Lane i writes LDS bytes [lds + 16 i, +16)
 // (b128) or [lds + 4 i, +4) (b32), lds = base + kOff; it reads the buffer at
-// voff + soff, and the range check covers it whether or not the hardware
-// counts soff (every offset that must read zeros is out of range by voff
-// alone, and soff never exceeds the range).
+// voff + soff.  The range check counts both, for each dword by itself, and no
+// sum wraps: an empty range reads zeros at any soff, and the last dwords of a
+// b128 that crosses the end are zeros (tried on the device with all addresses
+// inside one buffer).  The FP8 kernels do not need that (what must read zeros is
+// out of range by voff alone, and soff never exceeds the range); the MXFP4 and
+// few-token kernels do: their empty loads keep soff, and the scale bytes asked
+// for behind the end of the last row are cut off by it.
 // The pair fills lds and lds + 1024 from v0 and v1: one M0 write for two
 // loads, the second through the instruction offset, which moves both
 // addresses, so v1 is the row's offset less 1024 (never negative: its row is

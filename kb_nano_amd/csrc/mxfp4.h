@@ -9,7 +9,11 @@
 // 6 scales are below 7, where 6 is the nearest code, and no value is off by
 // more than half the spacing of the codes at the top of the range.  In bits:
 // adding a quarter of the mantissa range carries into the exponent exactly for
-// mantissas >= 1.75.  At least 1 (2^-126, groups of zeros and of subnormal
+// mantissas >= 1.75.  This is a choice: the OCP microscaling document's own
+// conversion takes exponent(max) - 2 without the rounding, which clips magnitudes
+// of 7 to 8 scales to 6; groups whose maximum has a mantissa of 1.75 and more get
+// the next scale here, and so other codes than from a producer that goes by that
+// rule.  Codes and scales of either are read alike.  At least 1 (2^-126, groups of zeros and of subnormal
 // numbers), at most 253.  A group that holds an infinity or a NaN has no such
 // scale: byte 255 and codes of 0, so it reads back as NaN.
 #pragma once

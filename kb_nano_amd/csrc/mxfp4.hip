@@ -177,12 +177,13 @@ extern "C" int kbn_mxfp4_gemm_nt(const void* A, int64_t lda, const void* sA, int
 
 // x -> codes and scales in the workspace -> product.  Few rows of 16-bit values
 // go in one launch, without those: each workgroup of the few-rows kernel
-// quantizes them for itself.  us, one launch / two: 1 x 10240 x 8192 10.2 / 11.9, 4 x
-// 10240 x 8192 10.7 / 12.0, 4 x 2048 x 2048 3.9 / 5.1, 4 x 36864 x 7168 26.5 / 26.3; 8
-// rows 2048 x 2048 4.1 / 4.9, 10240 x 8192 11.5 / 12.2, 4608 x 7168 8.7 / 8.5, but
-// 36864 x 7168 32.0 / 26.9: up to 8 where every CU has one workgroup.  16 rows 2048 x
-// 2048 4.8 / 5.0, 7168 x 2048 5.7 / 6.0, 4096 x 4096 6.5 / 6.2, 8192 x 8192 11.7 / 10.9:
-// there up to K = 2048.
+// quantizes them for itself.  us in a graph with the weights in memory, one
+// launch / two: 1 x 10240 x 8192 10.3 / 12.0, 1 x 2048 x 2048 3.8 / 4.8, 1 x 36864 x 7168
+// 26.4 / 25.9, 4 x 10240 x 8192 11.7 / 13.0, 4 x 2048 x 2048 4.1 / 5.3, 4 x 36864 x 7168
+// 28.0 / 26.5 (an eager call saves a launch's host time as well); 8 rows 2048 x 2048
+// 4.3 / 5.1, 10240 x 8192 13.2 / 13.1, 4608 x 7168 8.9 / 9.2, but 36864 x 7168 32.0 /
+// 26.9: up to 8 where every CU has one workgroup.  16 rows 2048 x 2048 4.9 / 5.2, 7168 x
+// 2048 5.9 / 6.1, 4096 x 4096 6.5 / 6.2, 8192 x 8192 11.7 / 10.9: there up to K = 2048.
 static bool linear_fused(int64_t M, int64_t N, int64_t K, int x_dtype) {
     return x_dtype != kMxF32 && (M <= 4 || (N <= 48 * cu_count() && (M <= 8 || (M <= 16 && K <= 2048))));
 }

@@ -19,14 +19,17 @@
 // read and frees it for the loads of the stage kStages ahead, which are spread
 // over the MFMA slots behind it.
 //
-// What bounds it.  Large products: power, and the CU's path for loads.  4096 x
-// 36864 x 7168 takes 534 us, 4.05 PFLOP/s, at the 1.76 GHz that the card then
-// holds; the matrix pipes are busy 55% of the cycles, the load path's return side
-// 79%.  The same instructions alone on random operands reach 5.6 to 6 PFLOP/s.
-// Smaller tiles: the load path.  With 64x128 tiles at 4096 x 8192 x 8192 its
-// return side is busy 89%, its address side 79%, the matrix pipes 34%, LDS 35%;
-// 44 to 55 B/ns a CU arrive, also where each CU has one tile (200 x 8192 x 8192
-// 18.5 us), whatever the depth of the ring or the row stride.
+// What bounds it.  Large products: power.  4096 x 36864 x 7168 takes 533 us, 4.06
+// PFLOP/s, at the 1.6 to 1.8 GHz that the card then holds; the matrix pipes are
+// busy 56% of the cycles, the LDS 30%.  The same instructions alone on random
+// operands reach 5.6 to 6 PFLOP/s.
+// Smaller ones, 2 to 4 times their floor: not known.  A CU receives 45 B/ns at 200
+// x 8192 x 8192 (18.5 us, one 64x128 tile a CU) and 41 at 777 x 4608 x 7168 (24.0, one
+// 128x128 tile), a third of the 133 above, and no counted unit is at its limit:
+// the matrix pipes are busy 24 and 37% of the cycles, the LDS 25 and 38%, the
+// load path's address side 53 and 58%, and its return side, which has a load
+// pending in 83 and 82%, moves 30 and 31 bytes in such a cycle.  A deeper ring,
+// another row stride and the loads' cache scope change nothing.
 #include "mxfp4_gemm.h"
 
 #include "gemm_kernel.h"
@@ -323,7 +326,11 @@ static int launch_tiled(MxGemmArgs& p, const MxPlan& plan, float* slabs, hipStre
 // stage of 256 K where each CU has one workgroup, one where it has several (a
 // workgroup's share), fitted to 96 shapes (M 20 .. 4096, eight weights) and four
 // split counts timed in graphs; 14% off each, but the tile picked is 0.3%
-// slower than the best one on average, 6% at most.  Each tile carries shapes (us
+// slower than the best one on average, 6% at most.  Those are the shapes it was
+// fitted to; on 47 random ones of other weights (M 17 .. 4096, N 300 .. 40000, K 256
+// .. 19200) 0.5% on average and 11% at most, where K is 256 or 512 (1832 x 2478 x 256
+// 16.5 / 14.8).  Known to be off by more: 64 x 10240 x 8192 takes 64x64 tiles, 18.1
+// against 15.4 with 48 weight rows a workgroup.  Each tile carries shapes (us
 // with 64x64, 64x128, 128x128, 128x256, 256x256): 320 x 1000 x 4096 7.19 / 8.94 / 11.2 / 16.9 / 24.9, 65 x 24576 x
 // 1536 9.58 / 8.61 / 8.24 / 10 / 13.5, 777 x 4608 x 7168 28.7 / 23.3 / 20.1 / 26.1 / 41.8, 777 x 8192 x 8192 60.4 / 50 / 43.1 / 35.5 / 49.8, 4096 x 36864 x
 // 7168 1.17e+03 / 919 / 824 / 667 / 547.
@@ -338,7 +345,8 @@ static const TilePrice kTiles[] = {
     {128, 256, 1, 4.6, 4.3, 0.758, 0.835},
     {256, 256, 1, 6.74, 4.43, 1.25, 1.42},
 };
-constexpr double kSplitFixed = 3.0, kSplitMb = 0.35;   // the sum's launch, and each MB of partial sums
+// the sum's launch, and each MB of partial sums, which go through memory
+constexpr double kSplitFixed = 3.0, kSplitMb = 0.35;
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -14,8 +14,10 @@
 // neighbours in one output row.
 //
 // Bound by what a CU takes from memory, 28 to 32 B/ns, and the start of the
-// stream.  1 x 10240 x 8192 10.2 us, 4.4 TB/s; 1 x 36864 x 7168 23.7, 5.9; 64 x 2048 x
-// 2048 4.4 us, of which a launch is 2.3.
+// stream.  1 x 10240 x 8192 8.8 us of kernel, 5.1 TB/s, 9.6 back to back with the
+// quantization in it; 1 x 36864 x 7168 23.8, 5.9; 64 x 2048 x 2048 4.3 us, of which a
+// launch is 2.3.  Each workgroup also loads all activation codes, at 64 rows as
+// many bytes as 64 weight rows: 64 x 8192 x 8192 13.1 us, 2.8 TB/s.
 //
 // kX rows of bf16 or fp16 activations (kX > 0, M <= kX) are quantized by the
 // kernel itself: a lane of the second operand is one scale group of one row,

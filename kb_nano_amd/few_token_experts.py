@@ -6,6 +6,12 @@ product with the routed sum.  The activations are not quantized, so its
 results are nearer to the exact ones than those of the FP8 x FP8 chain, and
 the weights may also be MXFP4.  No other layer takes MXFP4 experts: more tokens
 go through them 64 at a time, and each call reads the named experts' weights.
+
+With many rows an expert (tokens that name it) the sorted-token layer is the
+faster one for FP8 weights: up to ten on average this one takes at most 1.05 of
+its time, at sixteen up to 1.5.  The kernels' sizes go by T * top_k / E rows, as for
+uniform routing with every id inside [0, E); other routings give the same results
+in more time than they need.
 """
 from __future__ import annotations
 

@@ -7,7 +7,10 @@ one byte: ``torch.float8_e8m0fnu``) and each value is an e2m1 code (0, 0.5, 1,
 nibble.  Per group, with a the largest magnitude rounded to one mantissa bit
 (ties up), the scale is 2^(floor(log2 a) - 2), at least 2^-126, and codes are
 to nearest, ties to even, at most 6 in magnitude; a group that holds an
-infinity or a NaN becomes NaN as a whole (scale byte 255).
+infinity or a NaN becomes NaN as a whole (scale byte 255).  The rounding in the
+scale is a choice: the OCP microscaling document's own conversion leaves it out
+and clips what passes 6 scales, so groups whose maximum has a mantissa of 1.75
+and more get other codes there; codes and scales of either are read alike.
 
 No counterpart in kb_nano; the modules stand beside ``PerTokenGroupQuantFp8``
 and ``Fp8Linear`` and take what those take.
