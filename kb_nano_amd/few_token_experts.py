@@ -11,7 +11,8 @@ With many rows an expert (tokens that name it) the sorted-token layer is the
 faster one for FP8 weights: up to ten on average this one takes at most 1.05 of
 its time, at sixteen up to 1.5.  The kernels' sizes go by T * top_k / E rows, as for
 uniform routing with every id inside [0, E); other routings give the same results
-in more time than they need.
+in more time than they need.  For inference, as the rest of the package: the
+output carries no gradient.
 """
 from __future__ import annotations
 

@@ -13,7 +13,8 @@ and clips what passes 6 scales, so groups whose maximum has a mantissa of 1.75
 and more get other codes there; codes and scales of either are read alike.
 
 No counterpart in kb_nano; the modules stand beside ``PerTokenGroupQuantFp8``
-and ``Fp8Linear`` and take what those take.
+and ``Fp8Linear`` and take what those take.  For inference, as the rest of the
+package: outputs carry no gradient.
 """
 from __future__ import annotations
 
