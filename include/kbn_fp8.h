@@ -531,6 +531,74 @@ int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* 
                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * The router's product (no kb_nano counterpart): logits[t, e] = sum_h x[t, h] w[e, h].
+ *   x      [T, H], row stride ld_x, w [E, H], row stride ld_w; x_dtype and
+ *          w_dtype 0 bf16, 1 fp16, 2 fp32, w of x's type or fp32; rows 16-byte
+ *          aligned, strides below 2^23 elements; H % 8 == 0
+ *   out    fp32 [T, E], row stride ld_out
+ * fp32 sums of exact products (fp32 operands as three bf16 numbers, products
+ * below 2^-24 of the largest left out), in one order for a shape and device.
+ */
+int kbn_moe_router_gemm(const void* x, int x_dtype, int64_t ld_x, const void* w, int w_dtype, int64_t ld_w,
+                        float* out, int64_t ld_out, int64_t T, int64_t E, int64_t H, void* stream);
+
+/*
+ * Experts of each token from its logits (no kb_nano counterpart).
+ *   logits   [T, E] (dtype 0 bf16, 1 fp16, 2 fp32), row stride ld; E <= 1024
+ *   bias     fp32 [E], finite, or NULL
+ *   score = softmax(logits) or (sigmoid != 0) 1 / (1 + exp(-logits)); the
+ *   choice goes by score + bias, without a bias by the logits (the same order).
+ *   The experts form num_groups (<= 64) groups of consecutive ones; a group ranks
+ *   by its largest choice value, with a bias by the sum of its two largest; the
+ *   experts outside the best topk_groups groups are masked.  The top_k (<= 64)
+ *   experts of the largest choice values are taken in descending order; equal
+ *   values (groups and experts) go to the lower index.
+ *   weights  fp32 [T, top_k]: the experts' scores, over their sum if
+ *            renormalize (0 where that is 0), times scale
+ *   ids      int32 or int64 (id_bytes 4, 8) [T, top_k]
+ * Experts of logit -inf or NaN are masked: taken only where no other is left,
+ * with weight 0.  +inf counts as the largest float.  Choice values and weights
+ * are computed in 64 bits.
+ */
+int kbn_moe_router_topk(const void* logits, int dtype, int64_t ld, const float* bias, int64_t T, int64_t E,
+                        int64_t top_k, int sigmoid, int64_t num_groups, int64_t topk_groups, int renormalize,
+                        float scale, float* weights, void* ids, int id_bytes, void* stream);
+
+/*
+ * The step between two blocks that are normed on both sides (no kb_nano counterpart):
+ *   p  = x / sqrt(mean(x^2) + eps) * post   (x without post)
+ *   r' = residual_scale * r + gate * p      (rounded to the rows' type)
+ *   n  = r' / sqrt(mean(r'^2) + eps) * w
+ * x, r, r_out and n_out [T, H] of one type (dtype 0 bf16, 1 fp16, 2 fp32), H % 8
+ * == 0, rows 16-byte aligned; w and post (or NULL) [H] of that type.  gate (or
+ * NULL) has element (t, h) at gate[t * gate_row + h * gate_col], gate_col 0 or 1.
+ * r_out may be r.  n leaves as rows (n_out) or as FP8 codes and scales (q_fp8
+ * [T, H] and scale, as kbn_rmsnorm_fp8_quant quantizes), or both; the other NULL.
+ */
+int kbn_gated_add_rmsnorm(const void* x, int dtype, int64_t ld_x, const void* r, int64_t ld_r, const void* w,
+                          const void* post, const void* gate, int64_t gate_row, int64_t gate_col,
+                          float residual_scale, float eps, int64_t T, int64_t H, void* r_out, int64_t ld_ro,
+                          void* n_out, int64_t ld_n, void* q_fp8, int64_t ld_q, float* scale, int64_t s_stride_m,
+                          int64_t s_stride_g, void* stream);
+
+/*
+ * Low-rank adapters of many requests (no kb_nano counterpart):
+ *   out[t] = base[t] + scaling[a] * B_a (A_a x[t]), a = ids[t]; base[t] for ids
+ *   outside [0, L)
+ *   x [T, K], base and out [T, N] (dtype 0 bf16, 1 fp16), lora_a [L, R, K] and
+ *   lora_b [L, N, R] contiguous, of that type; ids int32 or int64 (id_bytes 4, 8)
+ *   [T]; scaling fp32 [L] or NULL (1).  K % 8 == 0, R % 8 == 0 and at most 256,
+ *   adapters of smaller rank padded with zeros.  out may be base.
+ *   workspace: kbn_lora_add_workspace_bytes(T, K, L, R) bytes (-1 for sizes that
+ *   are refused), for this call alone while it runs.
+ */
+int64_t kbn_lora_add_workspace_bytes(int64_t T, int64_t K, int64_t L, int64_t R);
+int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* base, int64_t ld_base, const void* lora_a,
+                 const void* lora_b, const void* ids, int id_bytes, const float* scaling, int64_t T, int64_t N,
+                 int64_t K, int64_t L, int64_t R, void* out, int64_t ld_out, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/*
  * Split-K arrival counters (no counterpart in the reference; DeepGEMM has no
  * split-K).  The small-M split launches of the 64-row tiles sum their fp32
  * slabs themselves, counting arrivals in a region of a library-held device

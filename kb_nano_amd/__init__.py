@@ -17,7 +17,11 @@ quantized activations of a decoder layer's first linear.
 Beside them, without a kb_nano counterpart: MXFP4 (``Mxfp4Quant``,
 ``dequantize_mxfp4`` and ``Mxfp4Linear``, 4-bit codes with a scale per 32
 values) and ``FewTokenExperts``, the experts layer of a decode batch in two
-launches, over FP8 or MXFP4 weights.
+launches, over FP8 or MXFP4 weights; and what a layer does between its
+products: ``MoeRouterGemm`` and ``MoeRouterTopk`` (the experts of each token),
+``GatedAddRMSNorm`` / ``GatedAddRMSNormFP8Quant`` (norms after and before a
+block, gate and scaled residual) and ``LoraAdd`` / ``LoraFp8Linear`` (adapters
+of many requests).
 
 The compute runs in hand-written gfx950 HIP kernels (``csrc/``) behind the
 C-ABI of ``libkbn_fp8.so`` (declared in ``include/kbn_fp8.h``); this package
@@ -26,6 +30,7 @@ is the PyTorch-side host layer.
 from .few_token_experts import FewTokenExperts
 from .fp8_grouped_gemm_contiguous import Fp8GroupedGemmContiguous
 from .fused_experts import FusedExperts
+from .gated_rmsnorm import GatedAddRMSNorm, GatedAddRMSNormFP8Quant
 from .fp8_linear import (
     Fp8Linear,
     PerTokenGroupQuantFp8,
@@ -34,8 +39,10 @@ from .fp8_linear import (
     postprocess_fp8_weights,
     postprocess_fp8_weights_batched,
 )
+from .lora import LoraAdd, LoraFp8Linear
 from .moe_align import MoeAlign
 from .moe_grouped_gemm import MoeGroupedGemm, m_grouped_fp8_gemm_nt_contiguous
+from .moe_router import MoeRouterGemm, MoeRouterTopk
 from .moe_sum import MoeSum
 from .mxfp4 import Mxfp4Linear, Mxfp4Quant, dequantize_mxfp4
 from .rmsnorm_quant import FusedAddRMSNormFP8Quant, RMSNormFP8Quant
@@ -59,6 +66,12 @@ __all__ = [
     "dequantize_mxfp4",
     "Mxfp4Linear",
     "FewTokenExperts",
+    "MoeRouterGemm",
+    "MoeRouterTopk",
+    "GatedAddRMSNorm",
+    "GatedAddRMSNormFP8Quant",
+    "LoraAdd",
+    "LoraFp8Linear",
     "postprocess_model_fp8_weights",
     "warmup_fp8_linear",
     "m_grouped_fp8_gemm_nt_contiguous",

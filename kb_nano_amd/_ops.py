@@ -1090,6 +1090,180 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
 
 
+def moe_router_gemm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) -> None:
+    """``out[T, E]`` (fp32) = ``x [T, H]`` x ``weight [E, H]``^T; x bf16, fp16 or
+    fp32, the weight of x's type or fp32."""
+    what = "moe_router_gemm"
+    _dev_check(what, x, weight, out)
+    if x.dtype not in _QUANT_IN:
+        raise TypeError(f"{what}: hidden states must be bfloat16, float16 or float32, got {x.dtype}")
+    if weight.dtype is not x.dtype and weight.dtype is not _F32:
+        raise TypeError(f"{what}: the weight must be {x.dtype} as the hidden states or float32, got {weight.dtype}")
+    _dtype_check(what, out, _F32, "output")
+    if x.dim() != 2 or weight.dim() != 2:
+        raise ValueError(f"{what}: 2-D hidden states and weight expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    T, H = x.shape
+    E = weight.shape[0]
+    if H % 8 or H == 0 or E == 0:
+        raise ValueError(f"{what}: H={H} must be a positive multiple of 8, E={E} positive")
+    _mx_rows(what, "hidden states", x, (T, H))
+    _mx_rows(what, "weight", weight, (E, H))
+    _mx_rows(what, "output", out, (T, E))
+    if T == 0:
+        return
+    x, weight = _near(x), _near(weight)
+    check(lib().kbn_moe_router_gemm(x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), weight.data_ptr(), _QUANT_IN[weight.dtype],
+                                    _ld(weight), out.data_ptr(), _ld(out), T, E, H, _stream(x)), what)
+
+
+MAX_ROUTED = 1024   # experts moe_router_topk covers
+SCORINGS = ("softmax", "sigmoid")
+
+
+def moe_router_topk(logits: torch.Tensor, top_k: int, scoring: str, bias: torch.Tensor | None, num_groups: int,
+                    topk_groups: int, renormalize: bool, scale: float, weights: torch.Tensor, ids: torch.Tensor) -> None:
+    """The experts of ``logits [T, E]`` (bf16, fp16 or fp32) into ``weights`` fp32
+    and ``ids`` (int32 or int64) ``[T, top_k]``."""
+    what = "moe_router_topk"
+    _dev_check(what, *[t for t in (logits, bias, weights, ids) if t is not None])
+    if logits.dtype not in _QUANT_IN:
+        raise TypeError(f"{what}: logits must be bfloat16, float16 or float32, got {logits.dtype}")
+    if scoring not in SCORINGS:
+        raise ValueError(f"{what}: scoring must be one of {SCORINGS}, got {scoring!r}")
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: 2-D logits expected, got {tuple(logits.shape)}")
+    T, E = logits.shape
+    if not 1 <= E <= MAX_ROUTED:
+        raise ValueError(f"{what}: E={E} outside [1, {MAX_ROUTED}]")
+    if not 1 <= num_groups <= 64 or E % num_groups:
+        raise ValueError(f"{what}: num_groups={num_groups} must divide E={E} and be at most 64")
+    if not 1 <= topk_groups <= num_groups:
+        raise ValueError(f"{what}: topk_groups={topk_groups} outside [1, {num_groups}]")
+    if not 1 <= top_k <= min(64, topk_groups * (E // num_groups)):
+        raise ValueError(f"{what}: top_k={top_k} outside [1, 64] or more than the "
+                         f"{topk_groups * (E // num_groups)} experts of the kept groups")
+    _mx_rows(what, "logits", logits, (T, E))
+    if bias is not None:
+        _dtype_check(what, bias, _F32, "bias")
+        if bias.shape != (E,) or not bias.is_contiguous():
+            raise ValueError(f"{what}: bias must be contiguous {(E,)}, got {tuple(bias.shape)}")
+    _dtype_check(what, weights, _F32, "weights")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: ids must be int32 or int64, got {ids.dtype}")
+    for t, name in ((weights, "weights"), (ids, "ids")):
+        if tuple(t.shape) != (T, top_k) or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous {(T, top_k)}, got {tuple(t.shape)}")
+    check(lib().kbn_moe_router_topk(
+        logits.data_ptr(), _QUANT_IN[logits.dtype], _ld(logits), bias.data_ptr() if bias is not None else None, T, E, top_k,
+        1 if scoring == "sigmoid" else 0, num_groups, topk_groups, 1 if renormalize else 0, float(scale), weights.data_ptr(),
+        ids.data_ptr(), ids.element_size(), _stream(logits)), what)
+
+
+def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, post_weight: torch.Tensor | None,
+                      gate: torch.Tensor | None, residual_scale: float, eps: float, residual_out: torch.Tensor,
+                      out: torch.Tensor | None, out_fp8: torch.Tensor | None, out_scale: torch.Tensor | None) -> None:
+    """The norms after and before a block with its gate and scaled residual, over
+    ``x [T, H]``: the new residual into ``residual_out`` (which may be ``residual``),
+    its normed rows into ``out``, their 1x128 codes and scales into ``out_fp8`` and
+    ``out_scale [T, ceil(H/128)]`` (any strides); either may be None.  ``gate``
+    [T, H] with a row stride of any size and a column stride of 0 or 1."""
+    what = "gated_add_rmsnorm"
+    given = [t for t in (x, residual, weight, post_weight, gate, residual_out, out, out_fp8, out_scale) if t is not None]
+    _dev_check(what, *given)
+    if x.dtype not in _QUANT_IN:
+        raise TypeError(f"{what}: input must be bfloat16, float16 or float32, got {x.dtype}")
+    for t, name in ((residual, "residual"), (weight, "weight"), (post_weight, "post_weight"), (gate, "gate"),
+                    (residual_out, "residual output"), (out, "output")):
+        if t is not None:
+            _dtype_check(what, t, x.dtype, name)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: 2-D input expected, got {tuple(x.shape)}")
+    T, H = x.shape
+    if H % 8 or H == 0:
+        raise ValueError(f"{what}: hidden size {H} must be a positive multiple of 8")
+    for t, name in ((x, "input"), (residual, "residual"), (residual_out, "residual output"), (out, "output")):
+        if t is not None:
+            _mx_rows(what, name, t, (T, H))
+    for t, name in ((weight, "weight"), (post_weight, "post_weight")):
+        if t is not None and (t.shape != (H,) or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {(H,)}, got {tuple(t.shape)}")
+    gs = (0, 0)
+    if gate is not None:
+        if tuple(gate.shape) != (T, H) or gate.stride(1) not in (0, 1):
+            raise ValueError(f"{what}: gate must be {(T, H)} with a column stride of 0 or 1, got {tuple(gate.shape)}, "
+                             f"strides {gate.stride()}")
+        gs = (gate.stride(0) if T > 1 else 0, gate.stride(1))
+    if (out_fp8 is None) != (out_scale is None) or (out is None and out_fp8 is None):
+        raise ValueError(f"{what}: rows, codes with their scales, or both have to be asked for")
+    if out_fp8 is not None:
+        _dtype_check(what, out_fp8, FP8, "output_fp8")
+        _dtype_check(what, out_scale, _F32, "output_scales")
+        _mx_rows(what, "output_fp8", out_fp8, (T, H))
+        if tuple(out_scale.shape) != (T, -(-H // GROUP)):
+            raise ValueError(f"{what}: output_scales must be {(T, -(-H // GROUP))}, got {tuple(out_scale.shape)}")
+    if T == 0:
+        return
+    check(lib().kbn_gated_add_rmsnorm(
+        x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), residual.data_ptr(), _ld(residual), weight.data_ptr(),
+        post_weight.data_ptr() if post_weight is not None else None, gate.data_ptr() if gate is not None else None, *gs,
+        float(residual_scale), float(eps), T, H, residual_out.data_ptr(), _ld(residual_out),
+        out.data_ptr() if out is not None else None, _ld(out) if out is not None else 0,
+        out_fp8.data_ptr() if out_fp8 is not None else None, _ld(out_fp8) if out_fp8 is not None else 0,
+        out_scale.data_ptr() if out_scale is not None else None, out_scale.stride(0) if out_scale is not None else 0,
+        out_scale.stride(1) if out_scale is not None else 0, _stream(x)), what)
+
+
+LORA_MAX_RANK = 256
+
+
+def lora_add(x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
+             scaling: torch.Tensor | None, out: torch.Tensor) -> None:
+    """``out[t] = base[t] + scaling[a] * lora_b[a] (lora_a[a] x[t])`` with ``a =
+    adapter_ids[t]``; rows of ids outside [0, L) are base's.  ``x [T, K]``, ``base``
+    and ``out [T, N]`` (``out`` may be ``base``), ``lora_a [L, R, K]``, ``lora_b [L,
+    N, R]``, all bf16 or all fp16.  The sums between the two launches live in a
+    buffer of the call's own."""
+    what = "lora_add"
+    _dev_check(what, *[t for t in (x, base, lora_a, lora_b, adapter_ids, scaling, out) if t is not None])
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: input must be bfloat16 or float16, got {x.dtype}")
+    for t, name in ((base, "base"), (lora_a, "lora_a"), (lora_b, "lora_b"), (out, "output")):
+        _dtype_check(what, t, x.dtype, name)
+    if adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
+    if x.dim() != 2 or base.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
+        raise ValueError(f"{what}: x [T, K], base [T, N], lora_a [L, R, K] and lora_b [L, N, R] expected")
+    T, K = x.shape
+    N = base.shape[1]
+    L, R = lora_a.shape[:2]
+    if R % 8 or not 8 <= R <= LORA_MAX_RANK:
+        raise ValueError(f"{what}: rank {R} must be a multiple of 8 in [8, {LORA_MAX_RANK}]; pad adapters with zeros")
+    if K % 8 or K == 0 or N == 0 or L == 0:
+        raise ValueError(f"{what}: K={K} must be a positive multiple of 8, N={N} and L={L} positive")
+    for t, name, shape in ((lora_a, "lora_a", (L, R, K)), (lora_b, "lora_b", (L, N, R)), (adapter_ids, "adapter_ids", (T,))):
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous {shape}, got {tuple(t.shape)}")
+    if scaling is not None:
+        _dtype_check(what, scaling, _F32, "scaling")
+        if scaling.shape != (L,) or not scaling.is_contiguous():
+            raise ValueError(f"{what}: scaling must be contiguous {(L,)}, got {tuple(scaling.shape)}")
+    _mx_rows(what, "input", x, (T, K))
+    _mx_rows(what, "base", base, (T, N))
+    _mx_rows(what, "output", out, (T, N))
+    if _overlaps(base, out) and (base.data_ptr() != out.data_ptr() or _ld(base) != _ld(out)):
+        raise ValueError(f"{what}: output overlaps base (only exactly in place is allowed)")
+    if T == 0:
+        return
+    x = _near(x)
+    L_ = lib()
+    nbytes = L_.kbn_lora_add_workspace_bytes(T, K, L, R)
+    buf = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+    check(L_.kbn_lora_add(
+        x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), base.data_ptr(), _ld(base), lora_a.data_ptr(), lora_b.data_ptr(),
+        adapter_ids.data_ptr(), adapter_ids.element_size(), scaling.data_ptr() if scaling is not None else None, T, N, K, L, R,
+        out.data_ptr(), _ld(out), buf.data_ptr(), nbytes, _stream(x)), what)
+
+
 def fp8_block_requant(w_in: torch.Tensor, s_in: torch.Tensor | None, w_out: torch.Tensor, s_out: torch.Tensor,
                       use_ue8m0: bool, eps: float) -> None:
     """128x128 block quantization of ``w_in`` ([N, K] or [E, N, K]; fp8 codes
@@ -1156,6 +1330,7 @@ _fp8_lib = torch.library.Library("kb_nano_fp8", "FRAGMENT")
 _moe_lib = torch.library.Library("kb_nano_fp8_moe", "FRAGMENT")
 _norm_lib = torch.library.Library("kb_nano_norm", "FRAGMENT")
 _mx_lib = torch.library.Library("kb_nano_mxfp4", "FRAGMENT")
+_lora_lib = torch.library.Library("kb_nano_lora", "FRAGMENT")
 
 
 def _has_op(ns: str, name: str) -> bool:
@@ -1227,7 +1402,15 @@ def _register():
             ("kb_nano_mxfp4", _mx_lib, "linear(Tensor x, Tensor weight, Tensor weight_scale, Tensor! output) -> ()",
              mxfp4_linear),
             ("kb_nano_fp8_moe", _moe_lib, "few_token_experts(Tensor x, Tensor w13, Tensor w13_scale, Tensor w2, "
-             "Tensor w2_scale, Tensor topk_weights, Tensor topk_ids, Tensor! out) -> ()", few_token_experts)):
+             "Tensor w2_scale, Tensor topk_weights, Tensor topk_ids, Tensor! out) -> ()", few_token_experts),
+            ("kb_nano_fp8_moe", _moe_lib, "router_gemm(Tensor x, Tensor weight, Tensor! out) -> ()", moe_router_gemm),
+            ("kb_nano_fp8_moe", _moe_lib, "router_topk(Tensor logits, int top_k, str scoring, Tensor? bias, int num_groups, "
+             "int topk_groups, bool renormalize, float scale, Tensor! weights, Tensor! ids) -> ()", moe_router_topk),
+            ("kb_nano_norm", _norm_lib, "gated_add_rmsnorm(Tensor x, Tensor residual, Tensor weight, Tensor? post_weight, "
+             "Tensor? gate, float residual_scale, float eps, Tensor! residual_out, Tensor(a!)? out, Tensor(b!)? out_fp8, "
+             "Tensor(c!)? out_scale) -> ()", gated_add_rmsnorm),
+            ("kb_nano_lora", _lora_lib, "add(Tensor x, Tensor base, Tensor lora_a, Tensor lora_b, Tensor adapter_ids, "
+             "Tensor? scaling, Tensor! out) -> ()", lora_add)):
         name = schema[:schema.index("(")]
         if not _has_op(ns, name):
             ops.define(schema)
