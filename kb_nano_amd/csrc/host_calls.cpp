@@ -16,6 +16,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <utility>
@@ -459,11 +460,215 @@ PyObject* few_experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- router, gated norms and adapters
+
+constexpr int64_t kFarRows = 1 << 23;   // row strides from here on are copied by the Python path
+
+// A Python int or float (no subclass) as a number; false for anything else.
+bool int_of(PyObject* o, int64_t& v) {
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    return over == 0;
+}
+bool number_of(PyObject* o, double& v) {
+    int64_t i;
+    if (PyFloat_CheckExact(o)) v = PyFloat_AS_DOUBLE(o);
+    else if (int_of(o, i)) v = (double)i;
+    else return false;
+    return true;
+}
+// A tensor or None; false for anything else.
+bool plain_or_none(PyObject* o, const at::Tensor*& t) {
+    t = o == Py_None ? nullptr : plain_tensor(o);
+    return t || o == Py_None;
+}
+bool is_vector(const at::Tensor& t, at::ScalarType type, int64_t dev, int64_t n) {
+    return is(t, type, dev, 1) && t.size(0) == n && t.is_contiguous();
+}
+
+// router_gemm(x, weight) -> logits | None
+PyObject* router_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 2) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x = plain_tensor(args[0]), *w = plain_tensor(args[1]);
+        if (!x || !w || !plain_thread()) Py_RETURN_NONE;
+        const int xc = value_code(x->scalar_type()), wc = value_code(w->scalar_type());
+        const int64_t dev = x->get_device();
+        const Rows r = rows_of(*x), v = rows_of(*w);
+        hipStream_t st;
+        if (xc < 0 || (wc != xc && wc != 2) || !r.ok || !v.ok || w->dim() != 2 || w->get_device() != dev || v.k != r.k || r.k % 8 ||
+            r.ld >= kFarRows || v.ld >= kFarRows || !launch_stream(dev, st))
+            Py_RETURN_NONE;
+        const at::Tensor out = empty_like_rows(*x, v.n, at::kFloat);
+        Ref o{THPVariable_Wrap(out)};
+        if (!o.p) return nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_moe_router_gemm(x->data_ptr(), xc, r.ld, w->data_ptr(), wc, v.ld, (float*)out.data_ptr(), v.n, r.n, v.n, r.k,
+                                     (void*)st);
+        }
+        if (rc) return failed(rc, "moe_router_gemm");
+        return o.take();
+    });
+}
+
+// router_topk(logits, top_k, scoring, bias | None, num_groups, topk_groups, renormalize, scale, index dtype)
+//   -> (weights, ids) | None
+PyObject* router_topk(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 9) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *l = plain_tensor(args[0]), *bias = nullptr;
+        int64_t k, G, kept;
+        double scale;
+        if (!l || !int_of(args[1], k) || !PyUnicode_CheckExact(args[2]) || !plain_or_none(args[3], bias) || !int_of(args[4], G) ||
+            !int_of(args[5], kept) || !PyBool_Check(args[6]) || !number_of(args[7], scale) || !THPDtype_Check(args[8]) ||
+            !plain_thread())
+            Py_RETURN_NONE;
+        const bool sigmoid = PyUnicode_CompareWithASCIIString(args[2], "sigmoid") == 0;
+        if (!sigmoid && PyUnicode_CompareWithASCIIString(args[2], "softmax") != 0) Py_RETURN_NONE;
+        const at::ScalarType it = ((THPDtype*)args[8])->scalar_type;
+        const int code = value_code(l->scalar_type());
+        const int64_t dev = l->get_device();
+        const Rows r = rows_of(*l);
+        hipStream_t st;
+        if (code < 0 || !r.ok || k < 1 || k > 64 || (it != at::kInt && it != at::kLong) ||
+            (bias && !is_vector(*bias, at::kFloat, dev, r.k)) || !launch_stream(dev, st))
+            Py_RETURN_NONE;
+        const at::Tensor w = empty_like_rows(*l, k, at::kFloat), ids = empty_like_rows(*l, k, it);
+        Ref out{pair(w, ids)};
+        if (!out.p) return nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_moe_router_topk(l->data_ptr(), code, r.ld, bias ? (const float*)bias->data_ptr() : nullptr, r.n, r.k, k, sigmoid, G,
+                                     kept, args[6] == Py_True, (float)scale, (float*)w.data_ptr(), ids.data_ptr(),
+                                     (int)ids.element_size(), (void*)st);
+        }
+        if (rc) return failed(rc, "moe_router_topk");
+        return out.take();
+    });
+}
+
+// gated_norm(x, residual, weight, post_weight | None, gate | None, residual_scale, eps, rows, codes)
+//   -> (normed | None, codes | None, scales | None, residual') | None
+PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 9) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x = plain_tensor(args[0]), *r = plain_tensor(args[1]), *w = plain_tensor(args[2]), *post, *gate;
+        double rs, eps;
+        if (!x || !r || !w || !plain_or_none(args[3], post) || !plain_or_none(args[4], gate) || !number_of(args[5], rs) ||
+            !number_of(args[6], eps) || !plain_thread())
+            Py_RETURN_NONE;
+        const bool rows = args[7] == Py_True, codes = args[8] == Py_True;
+        const at::ScalarType type = x->scalar_type();
+        const int code = value_code(type);
+        const int64_t dev = x->get_device();
+        const Rows xr = rows_of(*x), rr = rows_of(*r);
+        hipStream_t st;
+        if (code < 0 || !xr.ok || !rr.ok || !is(*r, type, dev, x->dim()) || r->sizes() != x->sizes() || xr.k % 8 ||
+            !is_vector(*w, type, dev, xr.k) || (post && !is_vector(*post, type, dev, xr.k)) || (!rows && !codes))
+            Py_RETURN_NONE;
+        const int64_t T = xr.n, H = xr.k;
+        int64_t g_row = 0, g_col = 0;   // [H]; as x; or a column of one value a token
+        if (gate) {
+            if (gate->scalar_type() != type || gate->get_device() != dev) Py_RETURN_NONE;
+            const Rows g = rows_of(*gate);
+            if (!g.ok) Py_RETURN_NONE;
+            if (gate->dim() == 1 && g.k == H) {
+                g_col = 1;
+            } else if (gate->dim() == x->dim() && gate->sizes() == x->sizes()) {
+                g_col = 1;
+                g_row = T > 1 ? g.ld : 0;
+            } else if (gate->dim() == x->dim() && g.k == 1 && g.n == T &&
+                       gate->sizes().slice(0, gate->dim() - 1) == x->sizes().slice(0, x->dim() - 1)) {
+                g_row = T > 1 ? g.ld : 0;
+            } else {
+                Py_RETURN_NONE;
+            }
+        }
+        if (!launch_stream(dev, st)) Py_RETURN_NONE;
+        const int64_t groups = (H + kGroup - 1) / kGroup;
+        const at::Tensor res = empty_like_rows(*x, H, type);
+        at::Tensor out, q, s;
+        Ref res_o{THPVariable_Wrap(res)}, out_o{nullptr}, q_o{nullptr}, s_o{nullptr};
+        if (rows) {
+            out = empty_like_rows(*x, H, type);
+            out_o.p = THPVariable_Wrap(out);
+        }
+        if (codes) {
+            q = empty_codes(*x, T, H);
+            s = empty_scales(*x, T, groups);
+            q_o.p = THPVariable_Wrap(q);
+            s_o.p = THPVariable_Wrap(s);
+        }
+        if (!res_o.p || (rows && !out_o.p) || (codes && (!q_o.p || !s_o.p))) return nullptr;
+        Ref all{PyTuple_Pack(4, rows ? out_o.p : Py_None, codes ? q_o.p : Py_None, codes ? s_o.p : Py_None, res_o.p)};
+        if (!all.p) return nullptr;
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_gated_add_rmsnorm(x->data_ptr(), code, xr.ld, r->data_ptr(), rr.ld, w->data_ptr(), post ? post->data_ptr() : nullptr,
+                                       gate ? gate->data_ptr() : nullptr, g_row, g_col, (float)rs, (float)eps, T, H, res.data_ptr(), H,
+                                       rows ? out.data_ptr() : nullptr, H, codes ? q.data_ptr() : nullptr, H,
+                                       codes ? (float*)s.data_ptr() : nullptr, codes ? s.stride(0) : 0, codes ? s.stride(1) : 0,
+                                       (void*)st);
+        }
+        if (rc) return failed(rc, "gated_add_rmsnorm");
+        return all.take();
+    });
+}
+
+// lora_add(x, base, lora_a, lora_b, adapter_ids, scaling | None) -> a new output | None
+PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 6) Py_RETURN_NONE;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *x = plain_tensor(args[0]), *base = plain_tensor(args[1]), *a = plain_tensor(args[2]), *b = plain_tensor(args[3]),
+                         *ids = plain_tensor(args[4]), *sc;
+        if (!x || !base || !a || !b || !ids || !plain_or_none(args[5], sc) || !plain_thread()) Py_RETURN_NONE;
+        const at::ScalarType type = x->scalar_type();
+        const int code = value_code(type);
+        const int64_t dev = x->get_device();
+        const Rows xr = rows_of(*x), br = rows_of(*base);
+        hipStream_t st;
+        if ((code != 0 && code != 1) || !xr.ok || !br.ok || !is(*base, type, dev, x->dim()) || xr.n != br.n ||
+            x->sizes().slice(0, x->dim() - 1) != base->sizes().slice(0, base->dim() - 1) || !is(*a, type, dev, 3) ||
+            !is(*b, type, dev, 3) || !a->is_contiguous() || !b->is_contiguous() || xr.ld >= kFarRows)
+            Py_RETURN_NONE;
+        const int64_t T = xr.n, K = xr.k, N = br.k, L = a->size(0), R = a->size(1);
+        if (a->size(2) != K || b->size(0) != L || b->size(1) != N || b->size(2) != R || K % 8 || L < 1 ||
+            (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->get_device() != dev || ids->numel() != T ||
+            !ids->is_contiguous() || (sc && !is_vector(*sc, at::kFloat, dev, L)) || !launch_stream(dev, st))
+            Py_RETURN_NONE;
+        const int64_t bytes = kbn_lora_add_workspace_bytes(T, K, L, R);
+        if (bytes <= 0) Py_RETURN_NONE;
+        const at::Tensor out = empty_like_rows(*base, N, type);
+        Ref o{THPVariable_Wrap(out)};
+        if (!o.p) return nullptr;
+        const at::Tensor ws = at::empty({bytes}, x->options().dtype(at::kByte).requires_grad(false));   // of the call's own
+        void* const wsp = ws.data_ptr();
+        int rc;
+        {
+            NoGil no_gil;
+            rc = kbn_lora_add(x->data_ptr(), code, xr.ld, base->data_ptr(), br.ld, a->data_ptr(), b->data_ptr(), ids->data_ptr(),
+                              (int)ids->element_size(), sc ? (const float*)sc->data_ptr() : nullptr, T, N, K, L, R, out.data_ptr(), N,
+                              wsp, bytes, (void*)st);
+        }
+        if (rc) return failed(rc, "lora_add");
+        return o.take();
+    });
+}
+
 PyMethodDef kMethods[] = {
     {"mx_quant", (PyCFunction)(void (*)())mx_quant, METH_FASTCALL, "MXFP4 quantization"},
     {"mx_dequant", (PyCFunction)(void (*)())mx_dequant, METH_FASTCALL, "the values of MXFP4 codes"},
     {"mx_linear", (PyCFunction)(void (*)())mx_linear, METH_FASTCALL, "rows through an MXFP4 weight"},
     {"few_experts", (PyCFunction)(void (*)())few_experts, METH_FASTCALL, "experts layer for few tokens"},
+    {"router_gemm", (PyCFunction)(void (*)())router_gemm, METH_FASTCALL, "router logits"},
+    {"router_topk", (PyCFunction)(void (*)())router_topk, METH_FASTCALL, "experts of each token"},
+    {"gated_norm", (PyCFunction)(void (*)())gated_norm, METH_FASTCALL, "norms after and before a block, gate, residual"},
+    {"lora_add", (PyCFunction)(void (*)())lora_add, METH_FASTCALL, "adapters added to a projection's output"},
     {"norm", (PyCFunction)(void (*)())norm, METH_FASTCALL, "RMSNorm (+ residual add) + 1x128 quant"},
     {"silu", (PyCFunction)(void (*)())silu, METH_FASTCALL, "SiLU*Mul + 1x128 quant"},
     {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "bf16 activations through an FP8 weight"},

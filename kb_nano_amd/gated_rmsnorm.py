@@ -35,6 +35,10 @@ def _gate_rows(gate: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor | 
 
 
 def _run(input, residual, weight, post_weight, gate, residual_scale, eps, rows, codes):
+    if _ops._host is not None and not torch.compiler.is_compiling():
+        got = _ops._host.gated_norm(input, residual, weight, post_weight, gate, residual_scale, eps, rows, codes)
+        if got is not None:   # the plain case in one native step
+            return got
     if residual.shape != input.shape:
         raise ValueError(f"gated_add_rmsnorm: residual {tuple(residual.shape)} and input {tuple(input.shape)} differ")
     H = input.shape[-1]

@@ -26,6 +26,10 @@ class LoraAdd(nn.Module):
 
     def forward(self, x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter_ids: torch.Tensor, scaling: torch.Tensor | None = None, inplace: bool = False) -> torch.Tensor:
+        if _ops._host is not None and not inplace and not torch.compiler.is_compiling():
+            out = _ops._host.lora_add(x, base, lora_a, lora_b, adapter_ids, scaling)   # the plain case in one native step
+            if out is not None:
+                return out
         if x.shape[:-1] != base.shape[:-1]:
             raise ValueError(f"lora_add: x {tuple(x.shape)} and base {tuple(base.shape)} have other rows")
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])

@@ -20,6 +20,10 @@ class MoeRouterGemm(nn.Module):
     rounding between the product and the choice of experts."""
 
     def forward(self, hidden_states: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        if _ops._host is not None and not torch.compiler.is_compiling():
+            out = _ops._host.router_gemm(hidden_states, weight)   # the plain case in one native step
+            if out is not None:
+                return out
         x2 = hidden_states if hidden_states.dim() == 2 else hidden_states.reshape(-1, hidden_states.shape[-1])
         out = torch.empty(x2.shape[0], weight.shape[0], dtype=torch.float32, device=x2.device)
         if torch.compiler.is_compiling():
@@ -50,6 +54,10 @@ class MoeRouterTopk(nn.Module):
     def forward(self, logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None,
                 num_groups: int = 1, topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0,
                 index_dtype: torch.dtype = torch.int32) -> tuple[torch.Tensor, torch.Tensor]:
+        if _ops._host is not None and not torch.compiler.is_compiling():
+            out = _ops._host.router_topk(logits, top_k, scoring, bias, num_groups, topk_groups, renormalize, scale, index_dtype)
+            if out is not None:
+                return out
         l2 = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
         weights = torch.empty(l2.shape[0], top_k, dtype=torch.float32, device=l2.device)
         ids = torch.empty(l2.shape[0], top_k, dtype=index_dtype, device=l2.device)
