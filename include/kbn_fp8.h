@@ -538,9 +538,13 @@ int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* 
  *   out    fp32 [T, E], row stride ld_out
  * fp32 sums of exact products (fp32 operands as three bf16 numbers, products
  * below 2^-24 of the largest left out), in one order for a shape and device.
+ *   workspace: kbn_moe_router_gemm_workspace_bytes(...) bytes (0: none needed, -1
+ *   for sizes that are refused), for this call alone while it runs.
  */
+int64_t kbn_moe_router_gemm_workspace_bytes(int64_t T, int64_t E, int64_t H, int x_dtype, int w_dtype);
 int kbn_moe_router_gemm(const void* x, int x_dtype, int64_t ld_x, const void* w, int w_dtype, int64_t ld_w,
-                        float* out, int64_t ld_out, int64_t T, int64_t E, int64_t H, void* stream);
+                        float* out, int64_t ld_out, int64_t T, int64_t E, int64_t H, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /*
  * Experts of each token from its logits (no kb_nano counterpart).

@@ -67,7 +67,8 @@ SIGNATURES = {
     "kbn_few_token_experts_workspace_bytes": ([_I64, _I64, _I64], _I64),
     "kbn_few_token_experts": ([_P, _I, _I64, _P, _P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P,
                                _I64, _P], _I),
-    "kbn_moe_router_gemm": ([_P, _I, _I64, _P, _I, _I64, _P, _I64, _I64, _I64, _I64, _P], _I),
+    "kbn_moe_router_gemm_workspace_bytes": ([_I64, _I64, _I64, _I, _I], _I64),
+    "kbn_moe_router_gemm": ([_P, _I, _I64, _P, _I, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "kbn_moe_router_topk": ([_P, _I, _I64, _P, _I64, _I64, _I64, _I, _I64, _I64, _I, _F, _P, _P, _I, _P], _I),
     "kbn_gated_add_rmsnorm": ([_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _F, _F, _I64, _I64, _P, _I64, _P, _I64, _P,
                                _I64, _P, _I64, _I64, _P], _I),

@@ -1112,8 +1112,12 @@ def moe_router_gemm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) ->
     if T == 0:
         return
     x, weight = _near(x), _near(weight)
-    check(lib().kbn_moe_router_gemm(x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), weight.data_ptr(), _QUANT_IN[weight.dtype],
-                                    _ld(weight), out.data_ptr(), _ld(out), T, E, H, _stream(x)), what)
+    L = lib()
+    xc, wc = _QUANT_IN[x.dtype], _QUANT_IN[weight.dtype]
+    nbytes = max(0, L.kbn_moe_router_gemm_workspace_bytes(T, E, H, xc, wc))
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    check(L.kbn_moe_router_gemm(x.data_ptr(), xc, _ld(x), weight.data_ptr(), wc, _ld(weight), out.data_ptr(), _ld(out), T, E, H,
+                                buf.data_ptr() if nbytes else None, nbytes, _stream(x)), what)
 
 
 MAX_ROUTED = 1024   # experts moe_router_topk covers

@@ -503,11 +503,15 @@ PyObject* router_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor out = empty_like_rows(*x, v.n, at::kFloat);
         Ref o{THPVariable_Wrap(out)};
         if (!o.p) return nullptr;
+        const int64_t bytes = kbn_moe_router_gemm_workspace_bytes(r.n, v.n, r.k, xc, wc);
+        if (bytes < 0) Py_RETURN_NONE;
+        const at::Tensor ws = bytes ? at::empty({bytes}, w->options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+        void* const wsp = bytes ? ws.data_ptr() : nullptr;
         int rc;
         {
             NoGil no_gil;
-            rc = kbn_moe_router_gemm(x->data_ptr(), xc, r.ld, w->data_ptr(), wc, v.ld, (float*)out.data_ptr(), v.n, r.n, v.n, r.k,
-                                     (void*)st);
+            rc = kbn_moe_router_gemm(x->data_ptr(), xc, r.ld, w->data_ptr(), wc, v.ld, (float*)out.data_ptr(), v.n, r.n, v.n, r.k, wsp,
+                                     bytes, (void*)st);
         }
         if (rc) return failed(rc, "moe_router_gemm");
         return o.take();

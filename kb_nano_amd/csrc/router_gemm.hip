@@ -1,17 +1,22 @@
 // The router's product: logits[t, e] = sum_h x[t, h] w[e, h] in fp32.
 //
 // Few experts (8 to some hundred) and a long sum: what bounds it is reading w
-// (few tokens) or x (many).  No operand is worth the LDS: both are read
-// straight into the registers that the matrix instruction takes, 16 bytes a
-// lane, and the wavefronts of a workgroup share one tile of logits and split
-// its K instead, unit by unit, their sums meeting in LDS in wavefront order
-// (the same bits on every run; no second launch, no workspace).
+// (few tokens) or x (many).  The wavefronts of a workgroup share one tile of
+// logits and split its K, unit by unit; each streams whole 128-byte lines of its
+// units through a private LDS ring by direct loads, so there is no barrier until
+// their sums meet in LDS, in wavefront order.  (Fragments loaded straight into
+// the matrix instruction's layout have neighbouring lanes in different rows: 4096
+// x 256 x 7168 took 58 us so.)  Where tiles are too few for the CUs, workgroups
+// split K as well and a second launch adds their sums in order: the same bits on
+// every run.
 //
 // fp32 operands go through the 16-bit matrix instruction as well: a float is
 // the exact sum of three bf16 numbers (8 + 8 + 8 bits of its significand, cut
 // off by clearing low bits), and the products of pieces down to 2^-16 of the
 // largest are added, as good as fp32 products.
-#include "kbn_common.h"
+#include "gemm_kernel.h"
+
+#include <algorithm>
 
 namespace kbn {
 namespace {
@@ -26,6 +31,8 @@ struct GateArgs {
     float* out;
     int64_t ld_o;
     int T, E, H;
+    int splits;      // of K over workgroups
+    float* sums;     // [splits, T, E] where splits > 1
 };
 
 template <int kD> constexpr int bytes_of() { return kD == kG32 ? 4 : 2; }
@@ -76,7 +83,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <int kP> struct Pieces { u32x4 p[kP]; };
 
 template <int kD, int kP>
-__device__ __forceinline__ Pieces<kP> split(const Raw8<kD>& r) {
+__device__ __forceinline__ Pieces<kP> pieces_of(const Raw8<kD>& r) {
     Pieces<kP> o;
     if constexpr (kP == 1) {
         o.p[0] = r.v[0];
@@ -109,47 +116,98 @@ __device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, const f32x4
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// A tile of 16 kTM tokens x 16 kTE experts by a workgroup of kNW wavefronts;
-// kDepth units of 64 K in flight a wavefront.
-template <int kTM, int kTE, int kNW, int kDepth, int kX, int kW>
-__global__ __launch_bounds__(64 * kNW) void router_gemm_tile_kernel(const GateArgs a) {
-    __shared__ f32x4 part[kNW * kTM * kTE * 64];
+// What one operand of a stage (64 K) takes in LDS: rows of 128-byte lines, one
+// line a row of 16-bit values, two of fp32 (set 0: K 0 .. 31, set 1: 32 .. 63).
+// Sixteen-byte chunk c of row r lies in slot c ^ swz(r).
+template <int kD, int kTiles>
+struct Operand {
+    static constexpr int kSets = kD == kG32 ? 2 : 1, kLoads = 2 * kTiles * kSets, kBytes = kLoads * 1024;
+    // values 32 s + 8 q .. + 7 of fragment i's row
+    static __device__ __forceinline__ Raw8<kD> at(const uint8_t* p, int i, int row, int s, int q) {
+        Raw8<kD> r;
+        if constexpr (kD == kG32) {
+            const uint8_t* const line = p + s * (kTiles * 2048) + (16 * i + row) * 128;
+            r.v[0] = *reinterpret_cast<const u32x4*>(line + (((2 * q) ^ swz(row)) << 4));
+            r.v[1] = *reinterpret_cast<const u32x4*>(line + (((2 * q + 1) ^ swz(row)) << 4));
+        } else {
+            r.v[0] = *reinterpret_cast<const u32x4*>(p + (16 * i + row) * 128 + (((4 * s + q) ^ swz(row)) << 4));
+        }
+        return r;
+    }
+};
+
+constexpr int kGateK = 64;       // K of a stage
+constexpr int kGateWaves = 4;
+
+// A tile of 16 kTM tokens x 16 kTE experts; kDepth stages a wavefront.
+template <int kTM, int kTE, int kDepth, int kX, int kW>
+__global__ __launch_bounds__(64 * kGateWaves) void router_gemm_tile_kernel(const GateArgs a) {
+    typedef Operand<kX, kTM> OX;
+    typedef Operand<kW, kTE> OW;
+    constexpr int kLoads = OX::kLoads + OW::kLoads, kStage = OX::kBytes + OW::kBytes, kRing = kDepth * kStage;
+    constexpr int kSums = kTM * kTE * 1024;                 // bytes of a wavefront's sums
+    constexpr int kSmem = kGateWaves * (kRing > kSums ? kRing : kSums);
+    static_assert(kSmem <= 163840 && (kDepth - 1) * kLoads <= 63);
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kSmem];
     constexpr int bx = bytes_of<kX>(), bw = bytes_of<kW>();
     // two pieces hold fp16's 11 bits where the other side is bf16 pieces
     constexpr int PX = kX == kG32 ? 3 : (kX == kG16f && kW == kG32) ? 2 : 1;
     constexpr int PW = kW == kG32 ? 3 : 1;
     constexpr bool kHalf = kX == kG16f && kW == kG16f;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t0 = blockIdx.y * 16 * kTM, e0 = blockIdx.x * 16 * kTE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // workgroups go to the XCDs in turn: the tiles of one block of tokens run on
+    // one XCD, whose L2 then reads x once
+    const int te = (a.E + 16 * kTE - 1) / (16 * kTE), tt = (a.T + 16 * kTM - 1) / (16 * kTM), across = te * a.splits;
+    const int per = blockIdx.x / (8 * across) * 8, width = min(8, tt - per), in = blockIdx.x - per * across;
+    const int tile_t = per + in % width, tile_e = in / width / a.splits, split = in / width % a.splits;
+    const int t0 = tile_t * 16 * kTM, e0 = tile_e * 16 * kTE;
     const int nt = min(16 * kTM, a.T - t0), ne = min(16 * kTE, a.E - e0);
-    // rows past the tile's last lie outside the descriptors and read zeros
-    const __amdgpu_buffer_rsrc_t xr =
-        rsrc(static_cast<const uint8_t*>(a.x) + (int64_t)t0 * a.ld_x * bx, (int)(((int64_t)(nt - 1) * a.ld_x + a.H) * bx));
-    const __amdgpu_buffer_rsrc_t wr =
-        rsrc(static_cast<const uint8_t*>(a.w) + (int64_t)e0 * a.ld_w * bw, (int)(((int64_t)(ne - 1) * a.ld_w + a.H) * bw));
-    const int row = lane & 15, q = lane >> 4;
-    int xo[kTM], wo[kTE];
+    const v4i dX = make_desc(static_cast<const uint8_t*>(a.x) + (int64_t)t0 * a.ld_x * bx, ((int64_t)(nt - 1) * a.ld_x + a.H) * bx);
+    const v4i dW = make_desc(static_cast<const uint8_t*>(a.w) + (int64_t)e0 * a.ld_w * bw, ((int64_t)(ne - 1) * a.ld_w + a.H) * bw);
+    const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)wave * kRing;
+    const uint8_t* const ring = smem + wave * kRing;
+    // load j of an operand brings rows 8 j .. 8 j + 7 (of its second set from
+    // the middle on); rows past the tile's last read zeros
+    const int r8 = lane >> 3;
+    auto offset = [&](int j, int tiles, int rows, int64_t ld, int bytes) {
+        const int q = 8 * (j % (2 * tiles)) + r8;
+        return q < rows ? q * (int)ld * bytes + j / (2 * tiles) * 128 + (((lane & 7) ^ swz(q)) << 4) : kOob;
+    };
+    int xo[OX::kLoads], wo[OW::kLoads];
 #pragma unroll
-    for (int i = 0; i < kTM; ++i) xo[i] = 16 * i + row < nt ? ((16 * i + row) * (int)a.ld_x + 16 * q) * bx : kOob;
+    for (int j = 0; j < OX::kLoads; ++j) xo[j] = offset(j, kTM, nt, a.ld_x, bx);
 #pragma unroll
-    for (int i = 0; i < kTE; ++i) wo[i] = 16 * i + row < ne ? ((16 * i + row) * (int)a.ld_w + 16 * q) * bw : kOob;
-    // lane q of a row owns K 16 q .. 16 q + 15 of the unit, eight in each of two
-    // products (any order of K will do, if both operands have the same): the
-    // loads of a unit cover whole 128-byte lines
-    Raw8<kX> xb[kDepth][kTM][2];
-    Raw8<kW> wb[kDepth][kTE][2];
-    auto load = [&](int d, int u) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int k = 64 * u + 16 * q + 8 * s;
-            const bool in = k < a.H;   // H is a multiple of 8
-#pragma unroll
-            for (int i = 0; i < kTM; ++i)
-                xb[d][i][s] = load_raw8<kX>(xr, in && xo[i] >= 0 ? xo[i] + (64 * u + 8 * s) * bx : kOob);
-#pragma unroll
-            for (int i = 0; i < kTE; ++i)
-                wb[d][i][s] = load_raw8<kW>(wr, in && wo[i] >= 0 ? wo[i] + (64 * u + 8 * s) * bw : kOob);
+    for (int j = 0; j < OW::kLoads; ++j) wo[j] = offset(j, kTE, ne, a.ld_w, bw);
+    const int units = (a.H + kGateK - 1) / kGateK;
+    const int from = (int)((int64_t)units * split / a.splits), end = (int)((int64_t)units * (split + 1) / a.splits);
+    // Unit u into buffer buf.  Units past the end load nothing (and keep the
+    // count of loads in flight); in the last unit of a ragged H the chunks
+    // behind H read zeros, not the next row.
+    auto issue = [&](int buf, int u) __attribute__((always_inline)) {
+        const uint32_t base = lds + (uint32_t)buf * kStage;
+        v4i x = dX, w = dW;
+        if (u >= end) x[2] = w[2] = 0;
+        const int left = a.H - u * kGateK;
+        if (left >= kGateK || u >= end) {
+            static_for<OX::kLoads>([&](auto j_) __attribute__((always_inline)) {
+                dma_b128<decltype(j_)::value * 1024, false>(x, base, xo[decltype(j_)::value], u * kGateK * bx);
+            });
+            static_for<OW::kLoads>([&](auto j_) __attribute__((always_inline)) {
+                dma_b128<OX::kBytes + decltype(j_)::value * 1024, false>(w, base, wo[decltype(j_)::value], u * kGateK * bw);
+            });
+        } else {
+            auto cut = [&](int j, int tiles, int off, int bytes) {
+                const int q = 8 * (j % (2 * tiles)) + r8;
+                return j / (2 * tiles) * 128 + (((lane & 7) ^ swz(q)) << 4) < left * bytes ? off : kOob;
+            };
+            static_for<OX::kLoads>([&](auto j_) __attribute__((always_inline)) {
+                constexpr int j = decltype(j_)::value;
+                dma_b128<j * 1024, false>(x, base, cut(j, kTM, xo[j], bx), u * kGateK * bx);
+            });
+            static_for<OW::kLoads>([&](auto j_) __attribute__((always_inline)) {
+                constexpr int j = decltype(j_)::value;
+                dma_b128<OX::kBytes + j * 1024, false>(w, base, cut(j, kTE, wo[j], bw), u * kGateK * bw);
+            });
         }
     };
     f32x4 acc[kTM][kTE];
@@ -157,15 +215,32 @@ __global__ __launch_bounds__(64 * kNW) void router_gemm_tile_kernel(const GateAr
     for (int i = 0; i < kTM; ++i)
 #pragma unroll
         for (int j = 0; j < kTE; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](int d) {
+    const int row = lane & 15, q = lane >> 4;
+    for (int d = 0; d < kDepth; ++d) issue(d, from + wave + d * kGateWaves);
+    int buf = 0;
+    for (int u = from + wave; u < end; u += kGateWaves) {
+        wait_dma_n<(kDepth - 1) * kLoads>();
+        const uint8_t* const at = ring + buf * kStage;
+        Raw8<kX> xv[2][kTM];
+        Raw8<kW> wv[2][kTE];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < kTM; ++i) xv[s][i] = OX::at(at, i, row, s, q);
+#pragma unroll
+            for (int j = 0; j < kTE; ++j) wv[s][j] = OW::at(at + OX::kBytes, j, row, s, q);
+        }
+        wait_lds();   // all of the stage is read: its buffer may be filled again
+        issue(buf, u + kDepth * kGateWaves);
+        buf = buf == kDepth - 1 ? 0 : buf + 1;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Pieces<PX> px[kTM];
             Pieces<PW> pw[kTE];
 #pragma unroll
-            for (int i = 0; i < kTM; ++i) px[i] = split<kX, PX>(xb[d][i][s]);
+            for (int i = 0; i < kTM; ++i) px[i] = pieces_of<kX, PX>(xv[s][i]);
 #pragma unroll
-            for (int j = 0; j < kTE; ++j) pw[j] = split<kW, PW>(wb[d][j][s]);
+            for (int j = 0; j < kTE; ++j) pw[j] = pieces_of<kW, PW>(wv[s][j]);
 #pragma unroll
             for (int sum = PX + PW - 2; sum >= 0; --sum) {   // the smallest products first
                 if (sum > 2) continue;
@@ -180,32 +255,46 @@ __global__ __launch_bounds__(64 * kNW) void router_gemm_tile_kernel(const GateAr
                 }
             }
         }
-    };
-    const int units = (a.H + 63) / 64;
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) load(d, wave + d * kNW);
-    for (int u = wave; u < units; u += kNW * kDepth) {
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            multiply(d);
-            load(d, u + (d + kDepth) * kNW);
-        }
     }
+    wait_dma();         // no load writes to LDS any more
+    __syncthreads();    // no wavefront reads its ring any more
+    f32x4* const part = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
     for (int i = 0; i < kTM; ++i)
 #pragma unroll
         for (int j = 0; j < kTE; ++j) part[((wave * kTM + i) * kTE + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    for (int s = threadIdx.x; s < kTM * kTE * 64; s += 64 * kNW) {
+    float* const out = a.splits > 1 ? a.sums + (int64_t)split * a.T * a.E : a.out;
+    const int64_t ld = a.splits > 1 ? a.E : a.ld_o;
+    for (int s = tid; s < kTM * kTE * 64; s += 64 * kGateWaves) {
         f32x4 v = part[s];
 #pragma unroll
-        for (int n = 1; n < kNW; ++n) v += part[n * kTM * kTE * 64 + s];
+        for (int n = 1; n < kGateWaves; ++n) v += part[n * kTM * kTE * 64 + s];
         const int l = s & 63, tile = s >> 6;
         const int e = 16 * (tile % kTE) + (l & 15), t = 16 * (tile / kTE) + 4 * (l >> 4);
         if (e < ne) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (t + i < nt) a.out[(int64_t)(t0 + t + i) * a.ld_o + e0 + e] = v[i];
+                if (t + i < nt) out[(t0 + t + i) * ld + e0 + e] = v[i];
+        }
+    }
+}
+
+// out = the sums of the splits, in order.
+__global__ __launch_bounds__(256) void router_gemm_sum_kernel(const GateArgs a) {
+    const int64_t n = (int64_t)a.T * a.E, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    if (a.E % 4 == 0) {
+        f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + i);
+        for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.sums + s * n + i);
+        const int t = (int)(i / a.E), e = (int)(i - (int64_t)t * a.E);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.out[t * a.ld_o + e + k] = v[k];
+    } else {
+        for (int64_t k = i; k < min(n, i + 4); ++k) {
+            float v = a.sums[k];
+            for (int s = 1; s < a.splits; ++s) v += a.sums[s * n + k];
+            a.out[k / a.E * a.ld_o + k % a.E] = v;
         }
     }
 }
@@ -265,9 +354,26 @@ __global__ __launch_bounds__(64 * kRowWaves) void router_gemm_rows_kernel(const 
 
 constexpr int kRowTokens = 8;   // most tokens of the rows kernel
 
+// Tiles of 16 tm x 16 te logits, K in `splits` parts; tm = 0: the rows kernel.
+struct GatePlan {
+    int tm, te, splits;
+};
+GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
+    if (T <= kRowTokens) return {0, 0, 1};
+    const int64_t units = (H + kGateK - 1) / kGateK;
+    GatePlan p;
+    p.tm = xd == kG32 ? 2 : 4;
+    p.te = wd == kG32 ? 2 : 4;
+    auto tiles = [&](int te) { return (T + 16 * p.tm - 1) / (16 * p.tm) * ((E + 16 * te - 1) / (16 * te)); };
+    const int64_t cus = cu_count();
+    if (tiles(p.te) * 4 < cus) p.te = 1;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cus / tiles(p.te), 32, units / kGateWaves}));
+    return p;
+}
+
 template <int kX, int kW>
-void launch(const GateArgs& a, hipStream_t st) {
-    if (a.T <= kRowTokens) {
+void launch(GateArgs a, const GatePlan& p, hipStream_t st) {
+    if (p.tm == 0) {
         const dim3 grid((unsigned)a.E), block(64 * kRowWaves);
         if (a.T <= 1) router_gemm_rows_kernel<1, kX, kW><<<grid, block, 0, st>>>(a);
         else if (a.T <= 2) router_gemm_rows_kernel<2, kX, kW><<<grid, block, 0, st>>>(a);
@@ -275,17 +381,19 @@ void launch(const GateArgs& a, hipStream_t st) {
         else router_gemm_rows_kernel<8, kX, kW><<<grid, block, 0, st>>>(a);
         return;
     }
-    // the largest tile that still gives every CU a workgroup
-    const int cus = cu_count();
-    auto groups = [&](int tm, int te) {
-        return (int64_t)((a.T + 16 * tm - 1) / (16 * tm)) * ((a.E + 16 * te - 1) / (16 * te));
-    };
-    auto grid = [&](int tm, int te) {
-        return dim3((unsigned)((a.E + 16 * te - 1) / (16 * te)), (unsigned)((a.T + 16 * tm - 1) / (16 * tm)));
-    };
-    if (groups(4, 4) >= cus) router_gemm_tile_kernel<4, 4, 4, 2, kX, kW><<<grid(4, 4), dim3(256), 0, st>>>(a);
-    else if (groups(2, 2) >= cus) router_gemm_tile_kernel<2, 2, 8, 2, kX, kW><<<grid(2, 2), dim3(512), 0, st>>>(a);
-    else router_gemm_tile_kernel<1, 1, 16, 2, kX, kW><<<grid(1, 1), dim3(1024), 0, st>>>(a);
+    constexpr int kTM = kX == kG32 ? 2 : 4, kTE = kW == kG32 ? 2 : 4;
+    const int64_t tiles = (int64_t)((a.T + 16 * p.tm - 1) / (16 * p.tm)) * ((a.E + 16 * p.te - 1) / (16 * p.te));
+    const dim3 grid((unsigned)(tiles * p.splits)), block(64 * kGateWaves);
+    if (p.te == 1) router_gemm_tile_kernel<kTM, 1, 2, kX, kW><<<grid, block, 0, st>>>(a);
+    else router_gemm_tile_kernel<kTM, kTE, 2, kX, kW><<<grid, block, 0, st>>>(a);
+    if (p.splits > 1) {
+        const int64_t n = (int64_t)a.T * a.E;
+        router_gemm_sum_kernel<<<dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st>>>(a);
+    }
+}
+
+bool gate_sizes(int64_t T, int64_t E, int64_t H) {
+    return T >= 0 && T < (1 << 24) && E >= 1 && E <= 65536 && H >= 8 && H % 8 == 0 && H <= (1 << 22);
 }
 
 }  // namespace
@@ -293,15 +401,21 @@ void launch(const GateArgs& a, hipStream_t st) {
 
 using namespace kbn;
 
+extern "C" int64_t kbn_moe_router_gemm_workspace_bytes(int64_t T, int64_t E, int64_t H, int x_dtype, int w_dtype) {
+    if (!gate_sizes(T, E, H) || x_dtype < 0 || x_dtype > 2 || (w_dtype != x_dtype && w_dtype != kG32)) return -1;
+    const GatePlan p = gate_plan(T, E, H, x_dtype, w_dtype);
+    return p.splits > 1 ? (int64_t)p.splits * T * E * 4 : 0;
+}
+
 extern "C" int kbn_moe_router_gemm(const void* x, int x_dtype, int64_t ld_x, const void* w, int w_dtype, int64_t ld_w,
-                                   float* out, int64_t ld_out, int64_t T, int64_t E, int64_t H, void* stream) {
+                                   float* out, int64_t ld_out, int64_t T, int64_t E, int64_t H, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
     const char* what = "moe_router_gemm";
     KBN_CHECK_ARG(x_dtype >= 0 && x_dtype <= 2 && w_dtype >= 0 && w_dtype <= 2,
                   "%s: dtype codes %d and %d (0 bf16, 1 fp16, 2 fp32)", what, x_dtype, w_dtype);
     KBN_CHECK_ARG(w_dtype == x_dtype || w_dtype == kG32, "%s: weights must have the rows' dtype or be fp32", what);
-    KBN_CHECK_ARG(T >= 0 && T <= 0x7FFFFFFFLL - 64 && E >= 1 && E <= 65535 * 16, "%s: bad sizes T=%lld, E=%lld", what,
-                  (long long)T, (long long)E);
     KBN_CHECK_ARG(H >= 8 && H % 8 == 0 && H <= (1 << 22), "%s: H=%lld must be a multiple of 8 in [8, 2^22]", what, (long long)H);
+    KBN_CHECK_ARG(gate_sizes(T, E, H), "%s: bad sizes T=%lld (below 2^24), E=%lld (1 to 65536)", what, (long long)T, (long long)E);
     if (T == 0) return 0;
     KBN_CHECK_ARG(x && w && out, "%s: null pointer", what);
     const int bx = x_dtype == kG32 ? 4 : 2, bw = w_dtype == kG32 ? 4 : 2;
@@ -309,12 +423,15 @@ extern "C" int kbn_moe_router_gemm(const void* x, int x_dtype, int64_t ld_x, con
                   "%s: rows must be 16-byte aligned with strides of at least H", what);
     KBN_CHECK_ARG(ld_x < (1 << 23) && ld_w < (1 << 23), "%s: row strides must be below 2^23 elements", what);
     KBN_CHECK_ARG(ld_out >= E && (reinterpret_cast<uintptr_t>(out) & 3u) == 0, "%s: bad output rows", what);
-    GateArgs a{x, ld_x, w, ld_w, out, ld_out, (int)T, (int)E, (int)H};
-    KBN_CHECK_ARG((T + 15) / 16 <= 65535, "%s: T=%lld is more than 2^20 - 16 rows", what, (long long)T);
+    const GatePlan p = gate_plan(T, E, H, x_dtype, w_dtype);
+    const int64_t need = p.splits > 1 ? (int64_t)p.splits * T * E * 4 : 0;
+    KBN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+                  "%s: workspace of %lld bytes, 16-byte aligned, needed", what, (long long)need);
+    GateArgs a{x, ld_x, w, ld_w, out, ld_out, (int)T, (int)E, (int)H, p.splits, static_cast<float*>(workspace)};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (x_dtype == kG16b) w_dtype == kG16b ? launch<kG16b, kG16b>(a, st) : launch<kG16b, kG32>(a, st);
-    else if (x_dtype == kG16f) w_dtype == kG16f ? launch<kG16f, kG16f>(a, st) : launch<kG16f, kG32>(a, st);
-    else launch<kG32, kG32>(a, st);
+    if (x_dtype == kG16b) w_dtype == kG16b ? launch<kG16b, kG16b>(a, p, st) : launch<kG16b, kG32>(a, p, st);
+    else if (x_dtype == kG16f) w_dtype == kG16f ? launch<kG16f, kG16f>(a, p, st) : launch<kG16f, kG32>(a, p, st);
+    else launch<kG32, kG32>(a, p, st);
     KBN_CHECK_LAUNCH(what);
     return 0;
 }

@@ -13,18 +13,19 @@ def refused(rc, words):
     assert rc == 1 and words in msg, (rc, msg)
 
 
-GEMM = dict(x=P, xd=0, ldx=256, w=P, wd=0, ldw=256, out=P, ldo=8, T=4, E=8, H=256)
+GEMM = dict(x=P, xd=0, ldx=256, w=P, wd=0, ldw=256, out=P, ldo=8, T=4, E=8, H=256, ws=None, wsb=0)
 
 
 @pytest.mark.parametrize("over,words", [
     (dict(xd=3), "dtype codes"), (dict(wd=1), "rows' dtype"), (dict(xd=2), "rows' dtype"), (dict(H=252), "multiple of 8"),
     (dict(H=0), "multiple of 8"), (dict(E=0), "bad sizes"), (dict(T=-1), "bad sizes"), (dict(x=None), "null"), (dict(out=None), "null"),
-    (dict(x=ODD), "16-byte"), (dict(ldx=248), "16-byte"), (dict(ldw=260), "16-byte"), (dict(ldx=1 << 23), "2^23"), (dict(ldo=7), "output rows")])
+    (dict(x=ODD), "16-byte"), (dict(ldx=248), "16-byte"), (dict(ldw=260), "16-byte"), (dict(ldx=1 << 23), "2^23"), (dict(ldo=7), "output rows"),
+    (dict(T=20, H=4096, ldx=4096, ldw=4096), "workspace"), (dict(T=20, H=4096, ldx=4096, ldw=4096, ws=P, wsb=16), "workspace")])
 def test_router_gemm(over, words):
     from kb_nano_amd._lib import lib
     a = {**GEMM, **over}
-    refused(lib().kbn_moe_router_gemm(a["x"], a["xd"], a["ldx"], a["w"], a["wd"], a["ldw"], a["out"], a["ldo"], a["T"], a["E"], a["H"], None),
-            words)
+    refused(lib().kbn_moe_router_gemm(a["x"], a["xd"], a["ldx"], a["w"], a["wd"], a["ldw"], a["out"], a["ldo"], a["T"], a["E"], a["H"],
+                                      a["ws"], a["wsb"], None), words)
 
 
 TOPK = dict(l=P, d=2, ld=64, bias=None, T=4, E=64, k=4, sig=0, G=1, kept=1, renorm=1, w=P, ids=P, b=4)
@@ -76,7 +77,9 @@ def test_lora_add(over, words):
 def test_empty_batches_are_noops_and_workspaces_are_told():
     from kb_nano_amd._lib import lib
     L = lib()
-    assert L.kbn_moe_router_gemm(None, 0, 0, None, 0, 0, None, 0, 0, 8, 256, None) == 0
+    assert L.kbn_moe_router_gemm(None, 0, 0, None, 0, 0, None, 0, 0, 8, 256, None, 0, None) == 0
+    assert L.kbn_moe_router_gemm_workspace_bytes(4, 8, 252, 0, 0) == -1 and L.kbn_moe_router_gemm_workspace_bytes(4, 8, 256, 0, 1) == -1
+    assert L.kbn_moe_router_gemm_workspace_bytes(1, 8, 256, 0, 0) == 0
     assert L.kbn_moe_router_topk(None, 2, 0, None, 0, 64, 4, 0, 1, 1, 1, 1.0, None, None, 4, None) == 0
     assert L.kbn_gated_add_rmsnorm(None, 0, 0, None, 0, None, None, None, 0, 0, 1.0, 1e-6, 0, 256, None, 0, None, 0, None, 0, None, 0, 0, None) == 0
     assert L.kbn_lora_add(None, 0, 0, None, 0, None, None, None, 4, None, 0, 64, 256, 3, 16, None, 0, None, 0, None) == 0
