@@ -96,12 +96,9 @@ __device__ __forceinline__ Pieces<kP> pieces_of(const Raw8<kD>& r) {
             for (int i = 0; i < 4; ++i) {
                 const uint32_t a = __float_as_uint(f[2 * i]), b = __float_as_uint(f[2 * i + 1]);
                 o.p[k][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);   // the upper halves
-                if (k + 1 < kP) {
-                    // infinities and NaN stay whole in the first piece
-                    const float ra = f[2 * i] - __uint_as_float(a & 0xFFFF0000u);
-                    const float rb = f[2 * i + 1] - __uint_as_float(b & 0xFFFF0000u);
-                    f[2 * i] = (a & 0x7F800000u) == 0x7F800000u ? 0.f : ra;
-                    f[2 * i + 1] = (b & 0x7F800000u) == 0x7F800000u ? 0.f : rb;
+                if (k + 1 < kP) {   // (an infinity leaves a NaN here: its row has no finite result either way)
+                    f[2 * i] -= __uint_as_float(a & 0xFFFF0000u);
+                    f[2 * i + 1] -= __uint_as_float(b & 0xFFFF0000u);
                 }
             }
     }
@@ -280,23 +277,33 @@ __global__ __launch_bounds__(64 * kGateWaves) void router_gemm_tile_kernel(const
     }
 }
 
-// out = the sums of the splits, in order.
-__global__ __launch_bounds__(256) void router_gemm_sum_kernel(const GateArgs a) {
-    const int64_t n = (int64_t)a.T * a.E, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    if (a.E % 4 == 0) {
-        f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + i);
-        for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.sums + s * n + i);
-        const int t = (int)(i / a.E), e = (int)(i - (int64_t)t * a.E);
+// out = the sums of the splits, in order; eight of them asked for at a time
+// (one by one, each waits for the memory: 5.8 us for 16 sums of 61 x 256).
+template <int kV>
+__device__ __forceinline__ void sum_splits(const float* p, int64_t n, int splits, float (&v)[kV]) {
+    typedef float vec __attribute__((ext_vector_type(kV)));
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+        vec u[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a.out[t * a.ld_o + e + k] = v[k];
-    } else {
-        for (int64_t k = i; k < min(n, i + 4); ++k) {
-            float v = a.sums[k];
-            for (int s = 1; s < a.splits; ++s) v += a.sums[s * n + k];
-            a.out[k / a.E * a.ld_o + k % a.E] = v;
-        }
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < splits) u[s] = *reinterpret_cast<const vec*>(p + (s0 + s) * n);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < splits) {
+#pragma unroll
+                for (int k = 0; k < kV; ++k) v[k] = s0 + s == 0 ? u[s][k] : v[k] + u[s][k];
+            }
     }
+}
+template <int kV>
+__global__ __launch_bounds__(64) void router_gemm_sum_kernel(const GateArgs a) {
+    const int64_t n = (int64_t)a.T * a.E, i = ((int64_t)blockIdx.x * 64 + threadIdx.x) * kV;
+    if (i >= n) return;
+    float v[kV];
+    sum_splits<kV>(a.sums + i, n, a.splits, v);
+    const int64_t t = i / a.E, e = i - t * a.E;   // kV divides E
+#pragma unroll
+    for (int k = 0; k < kV; ++k) a.out[t * a.ld_o + e + k] = v[k];
 }
 
 // Few tokens: a workgroup for one expert, whose row it reads once; fp32
@@ -352,23 +359,47 @@ __global__ __launch_bounds__(64 * kRowWaves) void router_gemm_rows_kernel(const 
     }
 }
 
-constexpr int kRowTokens = 8;   // most tokens of the rows kernel
+// Most tokens of the rows kernel: past 8 its time grows with the tokens (us for
+// 8, 12, 16 tokens and 61 through tiles: 256 x 7168 bf16 4.6, 6.9, 7.0, 7.1; 128 x
+// 4096 3.7, 5.3, 5.4, 6.5; fp32 rows 5.5, 9.7, 11.3, 11.7 and 4.0, 6.0, 6.8, 8.2).
+constexpr int kRowTokens = 16, kRowTokens32 = 12;
 
 // Tiles of 16 tm x 16 te logits, K in `splits` parts; tm = 0: the rows kernel.
 struct GatePlan {
     int tm, te, splits;
 };
+
+// The cheapest of the tile widths and splits by what one takes in ns: the bytes
+// of a CU's workgroups, of which a lone CU takes 100 a ns and each of 256 at
+// work 80 (half where fp32 values are taken apart), a price on wide tiles (one
+// workgroup a CU), and with splits the second launch.  Fitted to 13 token counts
+// from 4 to 4096 with (256, 7168), (128, 4096) and (16, 2048), each type: 1.3%
+// above the best of up to 30 choices on average, 14% at most (512 x 256 x 7168:
+// 12.0 us with 32 experts a tile and four splits, 14.7 with 64 and three; 2048
+// tokens 18.8 with 32 and none, 27.4 with 16).
 GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
-    if (T <= kRowTokens) return {0, 0, 1};
-    const int64_t units = (H + kGateK - 1) / kGateK;
-    GatePlan p;
-    p.tm = xd == kG32 ? 2 : 4;
-    p.te = wd == kG32 ? 2 : 4;
-    auto tiles = [&](int te) { return (T + 16 * p.tm - 1) / (16 * p.tm) * ((E + 16 * te - 1) / (16 * te)); };
-    const int64_t cus = cu_count();
-    if (tiles(p.te) * 4 < cus) p.te = 1;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cus / tiles(p.te), 32, units / kGateWaves}));
-    return p;
+    if (T <= (xd == kG32 ? kRowTokens32 : kRowTokens)) return {0, 0, 1};
+    const int64_t units = (H + kGateK - 1) / kGateK, cus = cu_count();
+    const int tm = xd == kG32 ? 2 : 4, most = wd == kG32 ? 2 : 4;
+    const double bx = xd == kG32 ? 4 : 2, bw = wd == kG32 ? 4 : 2, slow = wd == kG32 ? 2.0 : 1.0;
+    GatePlan best{tm, 1, 1};
+    double least = 1e30;
+    double wide = 0.0;
+    for (int te = 1; te <= most; te *= 2, wide += 900.0) {
+        if (te > 1 && 8 * te >= E) break;
+        const int64_t tiles = (T + 16 * tm - 1) / (16 * tm) * ((E + 16 * te - 1) / (16 * te));
+        for (const int s : {1, 2, 3, 4, 8, 16, 32}) {
+            if (s > 1 && (s > units / kGateWaves || tiles * s > 2 * cus)) break;
+            const double rate = 80.0 + 20.0 * std::max<double>(0.0, 1.0 - (double)(tiles * s) / cus);
+            double ns = (double)((tiles * s + cus - 1) / cus) * (16 * tm * bx + 16 * te * bw) * H / s / rate * slow + wide;
+            if (s > 1) ns += 2400.0 + 200.0 * ((s + 7) / 8) + 60.0 * s + 8.0 * s * T * E / 4000.0;
+            if (ns < least) {
+                least = ns;
+                best = {tm, te, s};
+            }
+        }
+    }
+    return best;
 }
 
 template <int kX, int kW>
@@ -378,17 +409,20 @@ void launch(GateArgs a, const GatePlan& p, hipStream_t st) {
         if (a.T <= 1) router_gemm_rows_kernel<1, kX, kW><<<grid, block, 0, st>>>(a);
         else if (a.T <= 2) router_gemm_rows_kernel<2, kX, kW><<<grid, block, 0, st>>>(a);
         else if (a.T <= 4) router_gemm_rows_kernel<4, kX, kW><<<grid, block, 0, st>>>(a);
-        else router_gemm_rows_kernel<8, kX, kW><<<grid, block, 0, st>>>(a);
+        else if (a.T <= 8) router_gemm_rows_kernel<8, kX, kW><<<grid, block, 0, st>>>(a);
+        else router_gemm_rows_kernel<16, kX, kW><<<grid, block, 0, st>>>(a);
         return;
     }
-    constexpr int kTM = kX == kG32 ? 2 : 4, kTE = kW == kG32 ? 2 : 4;
+    constexpr int kTM = kX == kG32 ? 2 : 4;
     const int64_t tiles = (int64_t)((a.T + 16 * p.tm - 1) / (16 * p.tm)) * ((a.E + 16 * p.te - 1) / (16 * p.te));
     const dim3 grid((unsigned)(tiles * p.splits)), block(64 * kGateWaves);
     if (p.te == 1) router_gemm_tile_kernel<kTM, 1, 2, kX, kW><<<grid, block, 0, st>>>(a);
-    else router_gemm_tile_kernel<kTM, kTE, 2, kX, kW><<<grid, block, 0, st>>>(a);
+    else if (p.te == 2) router_gemm_tile_kernel<kTM, 2, 2, kX, kW><<<grid, block, 0, st>>>(a);
+    else if constexpr (kW != kG32) router_gemm_tile_kernel<kTM, 4, 2, kX, kW><<<grid, block, 0, st>>>(a);
     if (p.splits > 1) {
         const int64_t n = (int64_t)a.T * a.E;
-        router_gemm_sum_kernel<<<dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st>>>(a);
+        if (a.E % 2 == 0) router_gemm_sum_kernel<2><<<dim3((unsigned)((n + 127) / 128)), dim3(64), 0, st>>>(a);
+        else router_gemm_sum_kernel<1><<<dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st>>>(a);
     }
 }
 
