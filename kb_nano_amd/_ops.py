@@ -908,10 +908,10 @@ def _ld(t: torch.Tensor) -> int:
 FAR_ROWS = 1 << 23   # elements from row to row that the kernels' 32-bit offsets do not reach
 
 
-def _near(x: torch.Tensor) -> torch.Tensor:
+def _near(x: torch.Tensor, far: int = FAR_ROWS) -> torch.Tensor:
     """``x``, copied where its rows lie far apart (the last token of each of some
     long sequences): for kernels that few rows go to."""
-    return x.contiguous() if _ld(x) >= FAR_ROWS else x
+    return x.contiguous() if _ld(x) >= far else x
 
 
 def _mx_types(what: str, codes: torch.Tensor, scales: torch.Tensor, name: str) -> None:
@@ -1218,6 +1218,7 @@ def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
 
 
 LORA_MAX_RANK = 256
+LORA_FAR_ROWS = 1 << 22   # FAR_ROWS for windows of 256 rows
 
 
 def lora_add(x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_ids: torch.Tensor,
@@ -1258,7 +1259,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         raise ValueError(f"{what}: output overlaps base (only exactly in place is allowed)")
     if T == 0:
         return
-    x = _near(x)
+    x = _near(x, LORA_FAR_ROWS)
     L_ = lib()
     nbytes = L_.kbn_lora_add_workspace_bytes(T, K, L, R)
     buf = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)

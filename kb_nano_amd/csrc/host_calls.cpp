@@ -638,7 +638,7 @@ PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
         hipStream_t st;
         if ((code != 0 && code != 1) || !xr.ok || !br.ok || !is(*base, type, dev, x->dim()) || xr.n != br.n ||
             x->sizes().slice(0, x->dim() - 1) != base->sizes().slice(0, base->dim() - 1) || !is(*a, type, dev, 3) ||
-            !is(*b, type, dev, 3) || !a->is_contiguous() || !b->is_contiguous() || xr.ld >= kFarRows)
+            !is(*b, type, dev, 3) || !a->is_contiguous() || !b->is_contiguous() || xr.ld >= kFarRows / 2)
             Py_RETURN_NONE;
         const int64_t T = xr.n, K = xr.k, N = br.k, L = a->size(0), R = a->size(1);
         if (a->size(2) != K || b->size(0) != L || b->size(1) != N || b->size(2) != R || K % 8 || L < 1 ||

@@ -7,28 +7,25 @@
 // workgroups, fp32 partial sums [S, T, R]) and out (the partial sums added in
 // order, so results do not depend on which workgroup ends first).
 //
-// Tokens go by windows of 64.  In a window, slot s is its s-th adapter in
-// order of appearance, and a workgroup works on the tokens of one slot: a
-// decode batch in which every request has its own adapter reads each adapter
-// once, a window inside one prompt has one slot of 64 tokens.  Nothing has to
-// be known of the ids on the host.
+// Tokens go by windows, of 256 (of 64 where there are more than 64 adapters, so
+// that few tokens share one).  A workgroup finds the window's adapters in order
+// of appearance and works on chunks of one adapter's tokens, which need not be
+// neighbours: a decode batch reads each adapter once a window, a window inside one
+// prompt has one adapter and full chunks.  Nothing has to be known of the ids on
+// the host.
 //
 // h enters the second product as the sum of two bf16 numbers (16 bits of its
 // significand, 2^-16 of the value lost, far below the output's own rounding).
-#include "kbn_common.h"
+#include "row_stream.h"
 
 #include <algorithm>
 
 namespace kbn {
 namespace {
 
-constexpr int kWindow = 64;       // tokens
-constexpr int kLoraWaves = 4;
-constexpr int kRankChunk = 64;    // ranks of one shrink workgroup
-constexpr int kUnit = 64;         // K of one step
-constexpr int kMaxSplits = 16;
-
-enum : int { kLBf16 = 0, kLF16 = 1 };
+constexpr int kChunk = 64;        // tokens of one workgroup of the first launch
+constexpr int kRankChunk = 64;    // ranks of one workgroup of the first launch
+constexpr int kMaxSplits = 4;     // more gain nothing: the second launch reads them all back
 
 struct LoraArgs {
     const void* x;
@@ -44,156 +41,121 @@ struct LoraArgs {
     void* out;
     int64_t ld_o;
     float* h;            // [splits, T, R]
-    int splits, slots;   // slots: workgroups a window
-    int vec;             // rows of base and out take 16-byte accesses
+    int splits;
+    int slots1, slots2;  // workgroups a window that share its chunks, in each launch
+    int blocks;          // 256-column blocks of a workgroup of the second launch
 };
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, (int)kRsrcWord3);
-}
-__device__ __forceinline__ f32x4 mma_bf16(const u32x4& a, const u32x4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma_f16(const u32x4& a, const u32x4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// A window's tokens: lane i's adapter (-1: none), and the adapters in order of appearance.
+// A window of kWords x 64 tokens: lane i's adapter of each 64, the window's
+// adapters in order of appearance, and chunks of their tokens.  kNone: the tokens
+// without an adapter come as those of adapter -1, else they do not come.
+template <int kWords, bool kNone>
 struct Window {
-    int t0, n;
-    int64_t id;
-    uint64_t left;   // tokens whose adapter was not yet taken
+    int t0;
+    int id[kWords];
+    uint64_t left[kWords];    // tokens whose adapter was not yet taken
+    uint64_t now[kWords];     // tokens of the adapter that is
+    int adapter, n;           // it, and how many
     __device__ __forceinline__ Window(const LoraArgs& a, int w, int lane) {
-        t0 = w * kWindow;
-        n = min(kWindow, a.T - t0);
-        id = -1;
-        if (lane < n)
-            id = a.id64 ? static_cast<const int64_t*>(a.ids)[t0 + lane] : (int64_t)static_cast<const int32_t*>(a.ids)[t0 + lane];
-        if (id >= a.L) id = -1;
-        left = __ballot(id >= 0);
+        t0 = w * 64 * kWords;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            const int64_t t = t0 + 64 * k + lane;
+            int64_t v = -1;
+            if (t < a.T) v = a.id64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t)static_cast<const int32_t*>(a.ids)[t];
+            id[k] = t >= a.T ? -2 : v >= 0 && v < a.L ? (int)v : -1;
+            left[k] = __ballot(id[k] >= (kNone ? -1 : 0));
+        }
     }
-    // The next adapter and its tokens; false if there is none.
-    __device__ __forceinline__ bool next(int& adapter, uint64_t& tokens) {
-        if (!left) return false;
-        adapter = __builtin_amdgcn_readlane((int)id, (int)__builtin_ctzll(left));
-        tokens = __ballot((int)id == adapter && id >= 0);
-        left &= ~tokens;
+    // The next adapter; false if there is none.
+    __device__ __forceinline__ bool next() {
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k)
+            if (!found && left[k]) {
+                adapter = __builtin_amdgcn_readlane(id[k], (int)__builtin_ctzll(left[k]));
+                found = true;
+            }
+        if (!found) return false;
+        n = 0;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            now[k] = __ballot(id[k] == adapter);
+            left[k] &= ~now[k];
+            n += __builtin_popcountll(now[k]);
+        }
         return true;
     }
-};
-// Writes the positions of the set bits in order.
-__device__ __forceinline__ void list_tokens(uint64_t tokens, int lane, uint8_t* list) {
-    if (tokens >> lane & 1) list[__builtin_popcountll(tokens & ((1ull << lane) - 1))] = (uint8_t)lane;
-}
-
-// h[split, t, r0 ..] of one slot's tokens: kTM tiles of 16 tokens, kTR of 16 ranks.
-template <int kD, int kTM, int kTR>
-__device__ __forceinline__ void shrink_tile(const LoraArgs& a, int t0, int n, const uint8_t* list, int adapter, int r0,
-                                            int split, f32x4* part) {
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = lane & 15, q = lane >> 4;
-    const int nr = min(16 * kTR, a.R - r0);
-    const __amdgpu_buffer_rsrc_t xr = rsrc(static_cast<const uint8_t*>(a.x) + (int64_t)t0 * a.ld_x * 2,
-                                           (int)(((int64_t)(min(kWindow, a.T - t0) - 1) * a.ld_x + a.K) * 2));
-    const __amdgpu_buffer_rsrc_t ar =
-        rsrc(static_cast<const uint8_t*>(a.a) + ((int64_t)adapter * a.R + r0) * a.K * 2, (int)((int64_t)nr * a.K * 2));
-    int xo[kTM], ao[kTR];
+    // Writes tokens from .. from + count - 1 of now, as places in the window (one wavefront).
+    __device__ __forceinline__ void list(int from, int count, int lane, uint8_t* to) const {
+        int before = -from;
 #pragma unroll
-    for (int i = 0; i < kTM; ++i) xo[i] = 16 * i + row < n ? (list[16 * i + row] * (int)a.ld_x + 16 * q) * 2 : kOob;
-#pragma unroll
-    for (int j = 0; j < kTR; ++j) ao[j] = 16 * j + row < nr ? ((16 * j + row) * a.K + 16 * q) * 2 : kOob;
-    constexpr int kDepth = 2;
-    u32x4 xb[kDepth][kTM][2], ab[kDepth][kTR][2];
-    auto load = [&](int d, int u) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool in = u * kUnit + 16 * q + 8 * s < a.K;
-#pragma unroll
-            for (int i = 0; i < kTM; ++i)
-                xb[d][i][s] = __builtin_amdgcn_raw_buffer_load_b128(xr, in && xo[i] >= 0 ? xo[i] + (u * kUnit + 8 * s) * 2 : kOob, 0, 0);
-#pragma unroll
-            for (int j = 0; j < kTR; ++j)
-                ab[d][j][s] = __builtin_amdgcn_raw_buffer_load_b128(ar, in && ao[j] >= 0 ? ao[j] + (u * kUnit + 8 * s) * 2 : kOob, 0, 0);
-        }
-    };
-    f32x4 acc[kTM][kTR];
-#pragma unroll
-    for (int i = 0; i < kTM; ++i)
-#pragma unroll
-        for (int j = 0; j < kTR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int units = (a.K + kUnit - 1) / kUnit, per = (units + a.splits - 1) / a.splits;
-    const int end = min(units, (split + 1) * per);
-    // units past this split's end read zeros
-    auto load_in = [&](int d, int u) { load(d, u < end ? u : units); };
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) load_in(d, split * per + wave + d * kLoraWaves);
-    for (int u = split * per + wave; u < end; u += kLoraWaves * kDepth) {
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < kTM; ++i)
-#pragma unroll
-                    for (int j = 0; j < kTR; ++j)
-                        acc[i][j] = kD == kLBf16 ? mma_bf16(xb[d][i][s], ab[d][j][s], acc[i][j])
-                                                 : mma_f16(xb[d][i][s], ab[d][j][s], acc[i][j]);
-            load_in(d, u + (d + kDepth) * kLoraWaves);
+        for (int k = 0; k < kWords; ++k) {
+            const int at = before + (int)__builtin_popcountll(now[k] & ((1ull << lane) - 1));
+            if ((now[k] >> lane & 1) && at >= 0 && at < count) to[at] = (uint8_t)(64 * k + lane);
+            before += (int)__builtin_popcountll(now[k]);
         }
     }
-#pragma unroll
-    for (int i = 0; i < kTM; ++i)
-#pragma unroll
-        for (int j = 0; j < kTR; ++j) part[((wave * kTM + i) * kTR + j) * 64 + lane] = acc[i][j];
-    __syncthreads();
+};
+
+// h[split, t, r0 ..] of n tokens of one adapter (lane i has the i-th's place in
+// the window): kTM tiles of 16 tokens, kTR of 16 ranks.
+template <int kD, int kTM, int kTR>
+__device__ __forceinline__ void shrink_tile(const LoraArgs& a, int t0, int places, int n, int list, int adapter,
+                                            int r0, int split, uint8_t* smem) {
+    typedef Stream<kTM, kTR, 2, kD, kD> St;
+    const int nr = min(16 * kTR, a.R - r0);
+    const v4i dX = make_desc(static_cast<const uint8_t*>(a.x) + (int64_t)t0 * a.ld_x * 2,
+                             ((int64_t)(min(places, a.T - t0) - 1) * a.ld_x + a.K) * 2);
+    const v4i dA = make_desc(static_cast<const uint8_t*>(a.a) + ((int64_t)adapter * a.R + r0) * a.K * 2, (int64_t)nr * a.K * 2);
+    const int units = (a.K + kStreamK - 1) / kStreamK;
+    St::run(dX, dA, [&](int q) { const int t = __shfl(list, q, 64);
+                        return q < n ? t * (int)a.ld_x * 2 : kOob; }, [&](int q) { return q < nr ? q * a.K * 2 : kOob; },
+            a.K, units * split / a.splits, units * (split + 1) / a.splits, smem);
     float* h = a.h + (int64_t)split * a.T * a.R;
-    for (int s = threadIdx.x; s < kTM * kTR * 64; s += 64 * kLoraWaves) {
-        f32x4 v = part[s];
-#pragma unroll
-        for (int w = 1; w < kLoraWaves; ++w) v += part[w * kTM * kTR * 64 + s];
+    for (int s = threadIdx.x; s < kTM * kTR * 64; s += 64 * kStreamWaves) {
+        const f32x4 v = St::sum(smem, s);
         const int l = s & 63, tile = s >> 6;
         const int r = 16 * (tile % kTR) + (l & 15), t = 16 * (tile / kTR) + 4 * (l >> 4);
-        if (r < nr) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t + i < n) h[(int64_t)(t0 + list[t + i]) * a.R + r0 + r] = v[i];
+        for (int i = 0; i < 4; ++i) {
+            const int token = __shfl(list, t + i, 64);
+            if (r < nr && t + i < n) h[(int64_t)(t0 + token) * a.R + r0 + r] = v[i];
         }
     }
-    __syncthreads();   // part and list are used again by the next slot
+    __syncthreads();   // smem is used again by the next chunk
 }
 
 // grid (splits, windows, slots x rank chunks)
-template <int kD, int kTR>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_kernel(const LoraArgs a) {
-    __shared__ f32x4 part[kLoraWaves * 4 * kTR * 64];
-    __shared__ uint8_t list[kWindow];
+template <int kD, int kTR, int kWords>
+__global__ __launch_bounds__(64 * kStreamWaves) void lora_shrink_kernel(const LoraArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[Stream<4, kTR, 2, kD, kD>::kSmem];
     const int lane = threadIdx.x & 63;
-    const int chunks = (a.R + kRankChunk - 1) / kRankChunk;
-    const int first = blockIdx.z / chunks, r0 = blockIdx.z % chunks * kRankChunk;
-    Window win(a, blockIdx.y, lane);
-    int adapter;
-    uint64_t tokens;
-    for (int slot = 0; win.next(adapter, tokens); ++slot) {
-        if (slot % a.slots != first) continue;
-        if (threadIdx.x < 64) list_tokens(tokens, lane, list);
-        __syncthreads();
-        const int n = __builtin_popcountll(tokens);
-        if (n <= 16) shrink_tile<kD, 1, kTR>(a, win.t0, n, list, adapter, r0, blockIdx.x, part);
-        else if (n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, n, list, adapter, r0, blockIdx.x, part);
-        else shrink_tile<kD, 4, kTR>(a, win.t0, n, list, adapter, r0, blockIdx.x, part);
+    const int parts = (a.R + kRankChunk - 1) / kRankChunk;
+    const int r0 = blockIdx.z % parts * kRankChunk;
+    int skip = blockIdx.z / parts;   // chunks until this workgroup's next one
+    Window<kWords, false> win(a, blockIdx.y, lane);
+    while (win.next()) {
+        for (int from = 0; from < win.n; from += kChunk) {
+            if (skip-- > 0) continue;
+            skip = a.slots1 - 1;
+            const int n = min(kChunk, win.n - from);
+            if (threadIdx.x < 64) win.list(from, n, lane, smem);
+            __syncthreads();
+            const int list = smem[min(lane, n - 1)];
+            __syncthreads();
+            if (n <= 16) shrink_tile<kD, 1, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
+            else if (n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
+            else shrink_tile<kD, 4, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
+        }
     }
 }
 
 __device__ __forceinline__ float value_of(int d, uint16_t v) {
-    return d == kLBf16 ? __uint_as_float((uint32_t)v << 16) : (float)__builtin_bit_cast(_Float16, v);
+    return d == kG16b ? __uint_as_float((uint32_t)v << 16) : (float)__builtin_bit_cast(_Float16, v);
 }
 __device__ __forceinline__ uint16_t value_to(int d, float f) {
-    if (d == kLBf16) return __builtin_bit_cast(uint16_t, (__bf16)f);
+    if (d == kG16b) return __builtin_bit_cast(uint16_t, (__bf16)f);
     return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
@@ -211,146 +173,274 @@ __device__ __forceinline__ void split8(const float (&f)[8], u32x4& hi, u32x4& lo
 }
 
 constexpr int kStrip = 64;                          // output columns of a wavefront
-constexpr int kColumns = kLoraWaves * kStrip;       // of a workgroup
+constexpr int kColumns = kStreamWaves * kStrip;     // of a workgroup's block
+constexpr int kRows = 32;                           // tokens of one workgroup of the second launch
 constexpr int kMaxRank = 256;
 
-// grid (column blocks, windows, slots + 1): the last slot copies the rows that
-// have no adapter (where out is not base itself).
+// A wavefront's LDS writes come before its reads that follow.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Four columns' values as they lie in memory with the adapter's added.
 template <int kD>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(const LoraArgs a) {
-    __shared__ uint8_t list[kWindow];
+__device__ __forceinline__ u32x2 added(const u32x2& was, float v0, float v1, float v2, float v3) {
+    if constexpr (kD == kG16b) {
+        const bf16x2 lo = __builtin_convertvector((f32x2{bf16lo(was.x) + v0, bf16hi(was.x) + v1}), bf16x2);
+        const bf16x2 hi = __builtin_convertvector((f32x2{bf16lo(was.y) + v2, bf16hi(was.y) + v3}), bf16x2);
+        return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const uint32_t a = was.x, b = was.y;
+        const h2 wa = __builtin_bit_cast(h2, a), wb = __builtin_bit_cast(h2, b);
+        const h2 lo{(_Float16)((float)wa.x + v0), (_Float16)((float)wa.y + v1)};
+        const h2 hi{(_Float16)((float)wb.x + v2), (_Float16)((float)wb.y + v3)};
+        return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    }
+}
+
+// grid (column blocks, windows, slots).  Rows without an adapter are chunks too,
+// and are copied (where out is not base itself).  A wavefront owns 64 columns
+// of a block and all tokens of the chunk.  Tile j of its second operand holds
+// columns 4 c + j, c = 0 .. 15, so a lane's results are four neighbouring columns
+// of four tokens, and 16 lanes read and write whole lines of base and out; B's
+// rows come straight into the matrix instruction's layout, once for all tokens;
+// h comes from LDS, summed over the splits and cut in two by the workgroup.
+// kKS: steps of 32 ranks whose rows of B are asked for ahead of h (0: any rank).
+// kVec: base and out go four columns at a time.
+template <int kD, int kKS, int kWords, bool kVec>
+__global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const LoraArgs a) {
+    constexpr int kRow = (kKS ? 32 * kKS : kMaxRank) + 8;   // values of a row of h: an odd number of 16-byte slots
+    constexpr int kTM = kRows / 16;
+    __shared__ __attribute__((aligned(16))) uint16_t part[2][kRows * kRow];
+    __shared__ uint8_t places[kStreamWaves][kRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * kColumns + wave * kStrip;
-    const uint16_t* const base = static_cast<const uint16_t*>(a.base);
-    uint16_t* const out = static_cast<uint16_t*>(a.out);
-    Window win(a, blockIdx.y, lane);
-    if ((int)blockIdx.z == a.slots) {
-        if (a.base == a.out) return;
-        uint64_t rows = ~win.left & (win.n == 64 ? ~0ull : (1ull << win.n) - 1);
-        const int n = n0 + lane;
-        for (; rows; rows &= rows - 1) {
-            const int64_t t = win.t0 + __builtin_ctzll(rows);
-            if (n < a.N) out[t * a.ld_o + n] = base[t * a.ld_b + n];
-        }
-        return;
-    }
     const int row = lane & 15, q = lane >> 4;
-    int adapter;
-    uint64_t tokens;
-    for (int slot = 0; win.next(adapter, tokens); ++slot) {
-        if (slot % a.slots != (int)blockIdx.z) continue;
-        __syncthreads();
-        if (threadIdx.x < 64) list_tokens(tokens, lane, list);
-        __syncthreads();
-        const int n = __builtin_popcountll(tokens);
-        const float sc = a.scaling ? a.scaling[adapter] : 1.f;
-        const uint8_t* bp = static_cast<const uint8_t*>(a.b) + (int64_t)adapter * a.N * a.R * 2;
-        const __amdgpu_buffer_rsrc_t br = rsrc(bp, (int)((int64_t)a.N * a.R * 2));
-        for (int i = 0; 16 * i < n; ++i) {
-            const int at = 16 * i + row;
-            const int64_t t = win.t0 + list[min(at, n - 1)];   // this lane's token
-            f32x4 acc[4];
+    Window<kWords, true> win(a, blockIdx.y, lane);
+    const uint16_t* const base = static_cast<const uint16_t*>(a.base) + (int64_t)win.t0 * a.ld_b;
+    uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)win.t0 * a.ld_o;
+    const int rows = (int)min((int64_t)64 * kWords, (int64_t)a.T - win.t0);
+    const __amdgpu_buffer_rsrc_t bi = rsrc(base, kVec ? (int)(((int64_t)(rows - 1) * a.ld_b + a.N) * 2) : 0);
+    const __amdgpu_buffer_rsrc_t bo = rsrc(out, kVec ? (int)(((int64_t)(rows - 1) * a.ld_o + a.N) * 2) : 0);
+    const int first = blockIdx.x * a.blocks * kColumns + wave * kStrip;
+    // B: rows past N lie behind the descriptor, ranks past R are not asked for
+    int wo[kKS ? kKS : 1];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < a.R; k += 32) {
-                const int r = k + 8 * q;
-                float hv[8];
+    for (int k = 0; k < (kKS ? kKS : 1); ++k) wo[k] = 32 * k + 8 * q < a.R ? (4 * row * a.R + 32 * k + 8 * q) * 2 : kOob;
+    uint8_t* const mine = places[wave];
+    int skip = blockIdx.z;
+    while (win.next()) {
+        for (int from = 0; from < win.n; from += kRows) {
+            if (skip-- > 0) continue;
+            skip = a.slots2 - 1;
+            const int n = min(kRows, win.n - from), tiles = (n + 15) / 16;
+            const bool copy = win.adapter < 0;
+            if (copy && a.base == a.out) continue;
+            win.list(from, n, lane, mine);   // each wavefront for itself
+            wave_lds_fence();
+            const __amdgpu_buffer_rsrc_t br = rsrc(static_cast<const uint8_t*>(a.b) + (int64_t)win.adapter * a.N * a.R * 2,
+                                                   copy ? 0 : (int)((int64_t)a.N * a.R * 2));
+            // h of the chunk's tokens, eight ranks of one a thread: asked for first,
+            // as everything waits for it
+            const int octets = (a.R + 31) / 32 * 4;
+            const float sc = a.scaling && !copy ? a.scaling[win.adapter] : 1.f;
+            f32x4 u[kMaxSplits][2];
+            auto load_h = [&](int s) {
+                const int i = s / octets, r = s % octets * 8;
+                const bool in = i < n && r < a.R && !copy;
+                const float* hp = a.h + (in ? (int64_t)(win.t0 + mine[i & (kRows - 1)]) * a.R + r : 0);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) hv[j] = 0.f;
-                if (r < a.R && at < n) {
-                    const float* hp = a.h + t * a.R + r;
-                    for (int s = 0; s < a.splits; ++s, hp += (int64_t)a.T * a.R) {
-                        const f32x4 u = *reinterpret_cast<const f32x4*>(hp), v = *reinterpret_cast<const f32x4*>(hp + 4);
+                for (int k = 0; k < kMaxSplits; ++k) {
+                    u[k][0] = u[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (k < a.splits && in) {
+                        u[k][0] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R);
+                        u[k][1] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R + 4);
+                    }
+                }
+            };
+            // summed over the splits, scaled, cut in two; zeros past the rank and past the tokens
+            auto put_h = [&](int s) {
+                const int i = s / octets, r = s % octets * 8;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = u[0][j / 4][j & 3];
+#pragma unroll
+                for (int k = 1; k < kMaxSplits; ++k)
+                    if (k < a.splits) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] += u[k][j / 4][j & 3];
+                    }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= sc;
+                u32x4 hi, lo;
+                split8(v, hi, lo);
+                if (i < 16 * tiles) {
+                    *reinterpret_cast<u32x4*>(&part[0][i * kRow + r]) = hi;
+                    *reinterpret_cast<u32x4*>(&part[1][i * kRow + r]) = lo;
+                }
+            };
+            if constexpr (kKS > 0) load_h(threadIdx.x);   // 32 tokens x 8 octets at most
+            // a lane's tokens in base and out: 4 q + i of each 16 of the chunk
+            int bo_at[kTM][4], oo_at[kTM][4];
+#pragma unroll
+            for (int m = 0; m < kTM; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = 16 * m + 4 * q + i, t = mine[min(at, n - 1)];
+                    bo_at[m][i] = at < n ? (t * (int)a.ld_b + 4 * row) * 2 : kOob;
+                    oo_at[m][i] = at < n ? (t * (int)a.ld_o + 4 * row) * 2 : kOob;
+                }
+            struct Strip {
+                u32x2 was[kTM][4];
+                u32x4 w[kKS ? kKS : 1][4];
+            };
+            auto load_b = [&](int n0, int k, u32x4 (&to)[4]) __attribute__((always_inline)) {
+                const int off = kKS ? wo[kKS ? k : 0] : 32 * k + 8 * q < a.R ? (4 * row * a.R + 32 * k + 8 * q) * 2 : kOob;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to[j] = __builtin_amdgcn_raw_buffer_load_b128(br, off, (n0 + j) * a.R * 2, 0);
+            };
+            auto ask = [&](int n0, Strip& t) __attribute__((always_inline)) {
+                if constexpr (kKS > 0) {
+#pragma unroll
+                    for (int k = 0; k < kKS; ++k) load_b(n0, k, t.w[k]);
+                }
+                if constexpr (kVec) {   // (past N a row's columns are the next row's: the last strip masks them)
+                    const bool in = n0 + 4 * row < a.N;
+#pragma unroll
+                    for (int m = 0; m < kTM; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            t.was[m][i] = __builtin_amdgcn_raw_buffer_load_b64(bi, in ? bo_at[m][i] : kOob, n0 * 2, 0);
+                }
+            };
+            auto finish = [&](int n0, Strip& t) __attribute__((always_inline)) {
+                f32x4 acc[kTM][4];
+#pragma unroll
+                for (int m = 0; m < kTM; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                auto step = [&](int kk, u32x4 (&b)[4]) __attribute__((always_inline)) {
+                    u32x4 bl[4];
+                    if constexpr (kD == kG16f) {   // as two bf16 numbers (exact): h may pass fp16's range
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            hv[j] += u[j];
-                            hv[4 + j] += v[j];
+                            float wf[8];
+                            to_floats<kG16f>(Raw8<kG16f>{{b[j]}}, wf);
+                            split8(wf, b[j], bl[j]);
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) hv[j] *= sc;
+                    for (int m = 0; m < kTM; ++m) {
+                        if (m >= tiles) continue;
+                        const u32x4 hh = *reinterpret_cast<const u32x4*>(&part[0][(16 * m + row) * kRow + 32 * kk + 8 * q]);
+                        const u32x4 hl = *reinterpret_cast<const u32x4*>(&part[1][(16 * m + row) * kRow + 32 * kk + 8 * q]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (kD == kG16f) acc[m][j] = mma<false>(hh, bl[j], acc[m][j]);
+                            acc[m][j] = mma<false>(hl, b[j], acc[m][j]);
+                            acc[m][j] = mma<false>(hh, b[j], acc[m][j]);
+                        }
+                    }
+                };
+                if constexpr (kKS > 0) {
+#pragma unroll
+                    for (int kk = 0; kk < kKS; ++kk) step(kk, t.w[kk]);
+                } else if (!copy) {
+                    for (int kk = 0; 32 * kk < a.R; ++kk) {
+                        load_b(n0, kk, t.w[0]);
+                        step(kk, t.w[0]);
+                    }
                 }
-                u32x4 hh, hl;
-                split8(hv, hh, hl);
+                const int c = n0 + 4 * row;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // row m of tile j is column 16 (m / 4) + 4 j + m % 4 of the strip,
-                    // so that a lane's results are 16 columns in a row
-                    const int col = n0 + 16 * (row >> 2) + 4 * j + (row & 3);
-                    const int off = r < a.R && col < a.N ? (col * a.R + r) * 2 : kOob;
-                    u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(br, off, 0, 0);
-                    if constexpr (kD == kLBf16) {
-                        acc[j] = mma_bf16(w, hl, acc[j]);
-                        acc[j] = mma_bf16(w, hh, acc[j]);
-                    } else {   // fp16 as two bf16 numbers (exact): h may pass fp16's range
-                        float wf[8];
+                for (int m = 0; m < kTM; ++m) {
+                    if (m >= tiles) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            wf[2 * e] = value_of(kLF16, (uint16_t)w[e]);
-                            wf[2 * e + 1] = value_of(kLF16, (uint16_t)(w[e] >> 16));
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (kVec) {
+                            const u32x2 y = copy ? t.was[m][i] : added<kD>(t.was[m][i], acc[m][0][i], acc[m][1][i], acc[m][2][i], acc[m][3][i]);
+                            __builtin_amdgcn_raw_buffer_store_b64(y, bo, c < a.N ? oo_at[m][i] : kOob, n0 * 2, 0);
+                        } else if (16 * m + 4 * q + i < n) {
+                            const int64_t at = mine[16 * m + 4 * q + i];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < a.N) {
+                                    const uint16_t v = base[at * a.ld_b + c + e];
+                                    out[at * a.ld_o + c + e] = copy ? v : value_to(kD, value_of(kD, v) + acc[m][e][i]);
+                                }
                         }
-                        u32x4 wl;
-                        split8(wf, w, wl);
-                        acc[j] = mma_bf16(wl, hh, acc[j]);
-                        acc[j] = mma_bf16(w, hl, acc[j]);
-                        acc[j] = mma_bf16(w, hh, acc[j]);
                     }
+                }
+            };
+            Strip one, two;
+            ask(first, one);
+            __syncthreads();   // part of the last chunk is done with
+            if constexpr (kKS > 0) {
+                put_h(threadIdx.x);
+            } else {
+                for (int s = threadIdx.x; s < 16 * tiles * octets; s += 64 * kStreamWaves) {
+                    load_h(s);
+                    put_h(s);
                 }
             }
-            if (at < n) {
-                const int c0 = n0 + 16 * q;
-                const uint16_t* bi = base + t * a.ld_b + c0;
-                uint16_t* o = out + t * a.ld_o + c0;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {   // eight columns each
-                    if (a.vec && c0 + 8 * g + 8 <= a.N) {
-                        const u32x4 v = *reinterpret_cast<const u32x4*>(bi + 8 * g);
-                        u32x4 y;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float lo = value_of(kD, (uint16_t)v[e]) + acc[2 * g + e / 2][2 * (e & 1)];
-                            const float hi = value_of(kD, (uint16_t)(v[e] >> 16)) + acc[2 * g + e / 2][2 * (e & 1) + 1];
-                            y[e] = (uint32_t)value_to(kD, lo) | (uint32_t)value_to(kD, hi) << 16;
-                        }
-                        *reinterpret_cast<u32x4*>(o + 8 * g) = y;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (c0 + 8 * g + e < a.N)
-                                o[8 * g + e] = value_to(kD, value_of(kD, bi[8 * g + e]) + acc[2 * g + e / 4][e & 3]);
-                    }
-                }
+            __syncthreads();
+            // the next strip is asked for before this one is done
+            const int end = min(a.N, (int)(blockIdx.x + 1) * a.blocks * kColumns);
+            for (int n0 = first; n0 < end; n0 += 2 * kColumns) {
+                const int n1 = n0 + kColumns;
+                if (n1 < end) ask(n1, two);
+                finish(n0, one);
+                if (n1 >= end) break;
+                if (n1 + kColumns < end) ask(n1 + kColumns, one);
+                finish(n1, two);
             }
         }
     }
 }
 
-// K splits and slots a window of a batch.
+// Windows of words x 64 tokens, workgroups a window that share its chunks in each
+// launch, K splits of the first and 256-column blocks of a workgroup of the second.
 struct LoraPlan {
-    int windows, splits, slots;
+    int words, windows, slots1, slots2, splits, blocks;
 };
-LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R) {
+LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     LoraPlan p;
-    p.windows = (int)((T + kWindow - 1) / kWindow);
-    p.slots = (int)std::min<int64_t>({L, T, kWindow});
-    if (p.windows > 4) p.slots = std::min(p.slots, 2);
-    const int64_t chunks = (R + kRankChunk - 1) / kRankChunk;
-    const int64_t units = (K + kUnit - 1) / kUnit;
-    const int64_t want = std::max<int64_t>(1, 512 / (p.windows * chunks));
-    p.splits = (int)std::min<int64_t>({want, kMaxSplits, std::max<int64_t>(1, units / kLoraWaves)});
+    p.words = L > 64 || T <= 64 ? 1 : 4;
+    const int64_t size = std::min<int64_t>(T, 64 * p.words), cus = cu_count();
+    p.windows = (int)((T + 64 * p.words - 1) / (64 * p.words));
+    // chunks a window can have: full ones, and a last one of each adapter; in many
+    // windows (prompts) mostly the full ones, and the rest waits its turn
+    const int64_t adapters = std::min(L, size), last = p.windows > 2 ? std::min<int64_t>(adapters, 2) : adapters;
+    const int64_t full1 = size / kChunk, full2 = size / kRows + 1;   // (and the tokens without an adapter)
+    p.slots1 = (int)std::max<int64_t>(1, full1 + last);
+    p.slots2 = (int)std::max<int64_t>(1, full2 + last);
+    const int64_t parts = (R + kRankChunk - 1) / kRankChunk, units = (K + kStreamK - 1) / kStreamK;
+    const int64_t busy = p.windows * std::max<int64_t>(std::max<int64_t>(1, full1), p.windows > 2 ? 1 : adapters * 2 / 3) * parts;
+    const int64_t few = std::max<int64_t>(1, 65536 / (std::min<int64_t>(T, kRows) * R * 4));   // that a chunk reads back
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cus + busy - 1) / busy, few, kMaxSplits, units / kStreamWaves}));
+    // of the second launch's workgroups a CU holds two, and one takes about 5 us
+    // whatever its columns: one round of them
+    const int64_t cols = (N + kColumns - 1) / kColumns, all = p.windows * std::min<int64_t>(p.slots2, (size + kRows - 1) / kRows + adapters);
+    p.blocks = (int)std::max<int64_t>(1, std::min(cols, (all * cols + 2 * cus - 1) / (2 * cus)));
     return p;
 }
 
-template <int kD>
-void launch_lora(const LoraArgs& a, int windows, hipStream_t st) {
-    const int chunks = (a.R + kRankChunk - 1) / kRankChunk;
-    const dim3 grid((unsigned)a.splits, (unsigned)windows, (unsigned)(a.slots * chunks)), block(64 * kLoraWaves);
-    if (a.R <= 16) lora_shrink_kernel<kD, 1><<<grid, block, 0, st>>>(a);
-    else if (a.R <= 32) lora_shrink_kernel<kD, 2><<<grid, block, 0, st>>>(a);
-    else lora_shrink_kernel<kD, 4><<<grid, block, 0, st>>>(a);
-    const dim3 egrid((unsigned)((a.N + kColumns - 1) / kColumns), (unsigned)windows, (unsigned)(a.slots + 1));
-    lora_expand_kernel<kD><<<egrid, block, 0, st>>>(a);
+template <int kD, int kWords>
+void launch_lora(const LoraArgs& a, const LoraPlan& p, bool vec, hipStream_t st) {
+    const int parts = (a.R + kRankChunk - 1) / kRankChunk;
+    const dim3 grid((unsigned)a.splits, (unsigned)p.windows, (unsigned)(a.slots1 * parts)), block(64 * kStreamWaves);
+    if (a.R <= 16) lora_shrink_kernel<kD, 1, kWords><<<grid, block, 0, st>>>(a);
+    else if (a.R <= 32) lora_shrink_kernel<kD, 2, kWords><<<grid, block, 0, st>>>(a);
+    else lora_shrink_kernel<kD, 4, kWords><<<grid, block, 0, st>>>(a);
+    const int cols = kColumns * a.blocks;
+    const dim3 egrid((unsigned)((a.N + cols - 1) / cols), (unsigned)p.windows, (unsigned)a.slots2);
+    if (!vec) lora_expand_kernel<kD, 0, kWords, false><<<egrid, block, 0, st>>>(a);
+    else if (a.R <= 32) lora_expand_kernel<kD, 1, kWords, true><<<egrid, block, 0, st>>>(a);
+    else if (a.R <= 64) lora_expand_kernel<kD, 2, kWords, true><<<egrid, block, 0, st>>>(a);
+    else lora_expand_kernel<kD, 0, kWords, true><<<egrid, block, 0, st>>>(a);
 }
 
 }  // namespace
@@ -359,9 +449,9 @@ void launch_lora(const LoraArgs& a, int windows, hipStream_t st) {
 using namespace kbn;
 
 extern "C" int64_t kbn_lora_add_workspace_bytes(int64_t T, int64_t K, int64_t L, int64_t R) {
-    if (T < 0 || T > 65535LL * kWindow || K < 8 || K % 8 || L < 1 || R < 8 || R % 8 || R > kMaxRank) return -1;
+    if (T < 0 || T > 65535LL * 64 || K < 8 || K % 8 || L < 1 || R < 8 || R % 8 || R > kMaxRank) return -1;
     if (T == 0) return 0;
-    return (int64_t)lora_plan(T, K, L, R).splits * T * R * 4;
+    return (int64_t)lora_plan(T, K, L, R, 1).splits * T * R * 4;
 }
 
 extern "C" int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* base, int64_t ld_base, const void* lora_a,
@@ -369,9 +459,9 @@ extern "C" int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* 
                             int64_t K, int64_t L, int64_t R, void* out, int64_t ld_out, void* workspace,
                             int64_t workspace_bytes, void* stream) {
     const char* what = "lora_add";
-    KBN_CHECK_ARG(dtype == kLBf16 || dtype == kLF16, "%s: dtype code %d (0 bf16, 1 fp16)", what, dtype);
+    KBN_CHECK_ARG(dtype == kG16b || dtype == kG16f, "%s: dtype code %d (0 bf16, 1 fp16)", what, dtype);
     KBN_CHECK_ARG(id_bytes == 4 || id_bytes == 8, "%s: ids of %d bytes (4 or 8)", what, id_bytes);
-    KBN_CHECK_ARG(T >= 0 && T <= 65535LL * kWindow && N >= 1 && L >= 1 && L <= 0x7FFFFFFF, "%s: bad sizes T=%lld, N=%lld, L=%lld",
+    KBN_CHECK_ARG(T >= 0 && T <= 65535LL * 64 && N >= 1 && L >= 1 && L <= 0x7FFFFFFF, "%s: bad sizes T=%lld, N=%lld, L=%lld",
                   what, (long long)T, (long long)N, (long long)L);
     KBN_CHECK_ARG(K >= 8 && K % 8 == 0 && K <= (1 << 22), "%s: K=%lld must be a multiple of 8 in [8, 2^22]", what, (long long)K);
     KBN_CHECK_ARG(R >= 8 && R % 8 == 0 && R <= kMaxRank, "%s: rank %lld must be a multiple of 8 in [8, %d]", what, (long long)R,
@@ -382,10 +472,10 @@ extern "C" int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* 
     KBN_CHECK_ARG(x && base && lora_a && lora_b && ids && out, "%s: null pointer", what);
     KBN_CHECK_ARG(aligned16(x) && aligned16(lora_a) && aligned16(lora_b) && ld_x >= K && ld_x % 8 == 0,
                   "%s: rows and adapters must be 16-byte aligned, the rows' stride at least K", what);
-    KBN_CHECK_ARG(ld_x < (1 << 23), "%s: row stride must be below 2^23 elements", what);
+    KBN_CHECK_ARG(ld_x < (1 << 22), "%s: row stride must be below 2^22 elements", what);
     KBN_CHECK_ARG(ld_base >= N && ld_out >= N, "%s: base and output rows' strides must be at least N", what);
     KBN_CHECK_ARG(base != out || ld_base == ld_out, "%s: in place, base and output must have one stride", what);
-    const LoraPlan p = lora_plan(T, K, L, R);
+    const LoraPlan p = lora_plan(T, K, L, R, N);
     KBN_CHECK_ARG(workspace && workspace_bytes >= (int64_t)p.splits * T * R * 4 && aligned16(workspace),
                   "%s: workspace of %lld bytes, 16-byte aligned, needed", what, (long long)((int64_t)p.splits * T * R * 4));
     LoraArgs a{};
@@ -407,11 +497,15 @@ extern "C" int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* 
     a.ld_o = ld_out;
     a.h = static_cast<float*>(workspace);
     a.splits = p.splits;
-    a.slots = p.slots;
-    a.vec = aligned16(base) && aligned16(out) && ld_base % 8 == 0 && ld_out % 8 == 0;
+    a.slots1 = p.slots1;
+    a.slots2 = p.slots2;
+    a.blocks = p.blocks;
+    const auto aligned8 = [](const void* v) { return (reinterpret_cast<uintptr_t>(v) & 7u) == 0; };
+    const bool vec = N % 4 == 0 && aligned8(base) && aligned8(out) && ld_base % 4 == 0 && ld_out % 4 == 0 && ld_base < (1 << 22) &&
+            ld_out < (1 << 22);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == kLBf16) launch_lora<kLBf16>(a, p.windows, st);
-    else launch_lora<kLF16>(a, p.windows, st);
+    if (dtype == kG16b) p.words == 1 ? launch_lora<kG16b, 1>(a, p, vec, st) : launch_lora<kG16b, 4>(a, p, vec, st);
+    else p.words == 1 ? launch_lora<kG16f, 1>(a, p, vec, st) : launch_lora<kG16f, 4>(a, p, vec, st);
     KBN_CHECK_LAUNCH(what);
     return 0;
 }

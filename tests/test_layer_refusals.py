@@ -65,7 +65,7 @@ LORA = dict(x=P, d=0, ldx=256, base=P, ldb=64, a=P, b=P, ids=P, ib=4, T=4, N=64,
 @pytest.mark.parametrize("over,words", [
     (dict(d=2), "dtype code"), (dict(ib=1), "ids of 1"), (dict(N=0), "bad sizes"), (dict(L=0), "bad sizes"), (dict(K=252), "multiple of 8"),
     (dict(R=12), "rank 12"), (dict(R=264), "rank 264"), (dict(x=None), "null"), (dict(ids=None), "null"), (dict(x=ODD), "16-byte"),
-    (dict(ldx=250), "16-byte"), (dict(ldx=1 << 23), "2^23"), (dict(ldb=63), "strides"), (dict(ldo=80), "in place"), (dict(wsb=16), "workspace"),
+    (dict(ldx=250), "16-byte"), (dict(ldx=1 << 22), "2^22"), (dict(ldb=63), "strides"), (dict(ldo=80), "in place"), (dict(wsb=16), "workspace"),
     (dict(ws=None), "workspace"), (dict(N=1 << 23, R=256, ldb=1 << 23, ldo=1 << 23), "too large")])
 def test_lora_add(over, words):
     from kb_nano_amd._lib import lib
