@@ -54,20 +54,88 @@ __device__ __forceinline__ float group_sum(float p, float* part, int wave, int l
     return p;
 }
 
-// One lane's eight elements of a token: residual, gate and post norm.
+// Eight elements of a row as they lie in memory (zeros past the range).
+template <int kT>
+struct Eight {
+    u32x4 w[kT == kNormF32 ? 2 : 1];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off, int nt) {
+        if (nt) {
+            w[0] = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, kNtLoad);
+            if constexpr (kT == kNormF32) w[1] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16, 0, kNtLoad);
+        } else {
+            w[0] = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
+            if constexpr (kT == kNormF32) w[1] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t word = w[0][j];
+            if constexpr (kT == kNormF32) {
+                v[j] = __uint_as_float(word);
+                v[4 + j] = __uint_as_float(w[1][j]);
+            } else if constexpr (kT == kNormBf16) {
+                v[2 * j] = bf16lo(word);
+                v[2 * j + 1] = bf16hi(word);
+            } else {
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                const h2 h = __builtin_bit_cast(h2, word);
+                v[2 * j] = (float)h.x;
+                v[2 * j + 1] = (float)h.y;
+            }
+        }
+    }
+    // v rounded to the type
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (kT == kNormF32) {
+                w[0][j] = __float_as_uint(v[j]);
+                w[1][j] = __float_as_uint(v[4 + j]);
+            } else {
+                w[0][j] = pack2<kT>(v[2 * j], v[2 * j + 1]);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t rs, int off) const {
+        __builtin_amdgcn_raw_buffer_store_b128(w[0], rs, off, 0, 0);
+        if constexpr (kT == kNormF32) __builtin_amdgcn_raw_buffer_store_b128(w[1], rs, off + 16, 0, 0);
+    }
+};
+
+// What a token's elements have in common.
 struct Step {
     float inv;          // of the post norm
     float scale;        // residual's
     float gate;         // the token's gate (1 without one)
 };
+// A lane's eight elements of the new residual, rounded.
 template <int kT>
-__device__ __forceinline__ void new_residual(const Step& st, bool post, const float (&x)[8], const float (&r)[8],
-                                             const float (&wp)[8], const float (&g)[8], float (&out)[8]) {
+__device__ __forceinline__ Eight<kT> new_residual(const Step& st, bool post, bool gated, const float (&x)[8], const Eight<kT>& r,
+                                                  const Eight<kT>& wp, const Eight<kT>& g) {
+    float p[8], f[8], o[8];
+    if (post) {
+        wp.floats(f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float p = post ? (x[j] * st.inv) * wp[j] : x[j];
-        out[j] = round_to<kT>(fmaf(st.scale, r[j], g[j] * p));
+        for (int j = 0; j < 8; ++j) p[j] = (x[j] * st.inv) * f[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = x[j];
     }
+    if (gated) {
+        g.floats(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = f[j] * p[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = st.gate * p[j];
+    }
+    r.floats(f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = fmaf(st.scale, f[j], p[j]);
+    Eight<kT> out;
+    out.set(o);
+    return out;
 }
 
 // Rows or codes of a lane's eight normalized values at element e0 of token m.
@@ -102,7 +170,7 @@ __device__ __forceinline__ void put(const GatedArgs& a, int m, int e0, int lane,
 // length, its values computed again in each of three passes (no pass reads
 // what another wrote, so r' may replace r).
 template <int kW, int kCW, int kT>
-__global__ __launch_bounds__(64 * kW) void gated_norm_kernel(const GatedArgs a) {
+__global__ __launch_bounds__(64 * kW, kCW == 2 && kT != kNormF32 ? 4 : 1) void gated_norm_kernel(const GatedArgs a) {
 #pragma clang fp contract(off)
     __shared__ float part[2][kW];
     constexpr int kB = elt_bytes<kT>();
@@ -123,20 +191,24 @@ __global__ __launch_bounds__(64 * kW) void gated_norm_kernel(const GatedArgs a) 
         else if constexpr (kT == kNormF16) st.gate = (float)static_cast<const _Float16*>(a.gate)[at];
         else st.gate = __uint_as_float((uint32_t)static_cast<const uint16_t*>(a.gate)[at] << 16);
     }
-    auto gate8 = [&](int off, float (&g)[8]) {
-        if (gated) {
-            load8<kT>(gr, off, g);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = st.gate;
-        }
-    };
     if constexpr (kCW > 0) {
+        // all that the token takes is asked for at once: one wait for the memory
+        // instead of three (the weights mostly come from L2)
+        Eight<kT> x[kCW], r[kCW], g[kCW], wp[kCW], wv[kCW];
+#pragma unroll
+        for (int i = 0; i < kCW; ++i) {
+            const int off = kB * ((kW * i + wave) * 512 + 8 * lane);
+            x[i].load(xr, off, kNtLoad);
+            if (post) wp[i].load(pr, off, 0);
+            r[i].load(rr, off, kNtLoad);
+            if (gated) g[i].load(gr, off, a.gate_row ? kNtLoad : 0);
+            wv[i].load(wr, off, 0);
+        }
         float v[kCW][8];   // x, then r'
         float p = 0.f;
 #pragma unroll
         for (int i = 0; i < kCW; ++i) {
-            load8<kT>(xr, kB * ((kW * i + wave) * 512 + 8 * lane), v[i]);
+            x[i].floats(v[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) p = fmaf(v[i][j], v[i][j], p);
         }
@@ -145,27 +217,25 @@ __global__ __launch_bounds__(64 * kW) void gated_norm_kernel(const GatedArgs a) 
 #pragma unroll
         for (int i = 0; i < kCW; ++i) {
             const int off = kB * ((kW * i + wave) * 512 + 8 * lane);
-            float r[8], wp[8], g[8], o[8];
-            load8<kT>(rr, off, r);
-            load8<kT>(pr, off, wp);
-            gate8(off, g);
-            new_residual<kT>(st, post, v[i], r, wp, g, o);
-            store8<kT>(ro, off, o);
-            const bool in = off < bytes;   // past the row: 0 * inf may have come out
+            const Eight<kT> o = new_residual<kT>(st, post, gated, v[i], r[i], wp[i], g[i]);
+            o.store(ro, off);
+            o.floats(v[i]);
+            if (off >= bytes) {   // past the row: 0 * inf may have come out
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] = in ? o[j] : 0.f;
-                p = fmaf(v[i][j], v[i][j], p);
+                for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p = fmaf(v[i][j], v[i][j], p);
         }
         const float inv = 1.0f / sqrtf(group_sum<kW>(p, part[1], wave, lane) / (float)a.H + a.eps);
 #pragma unroll
         for (int i = 0; i < kCW; ++i) {
             const int e0 = (kW * i + wave) * 512 + 8 * lane;
             float w8[8], n[8];
-            load8<kT>(wr, kB * e0, w8);
+            wv[i].floats(w8);
+            // (past the row weights are 0 and a NaN of 0 * inf is passed over by the group's maximum)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) n[j] = e0 < a.H ? (v[i][j] * inv) * w8[j] : 0.f;
+            for (int j = 0; j < 8; ++j) n[j] = (v[i][j] * inv) * w8[j];
             put<kT>(a, m, e0, lane, n);
         }
     } else {
@@ -182,16 +252,20 @@ __global__ __launch_bounds__(64 * kW) void gated_norm_kernel(const GatedArgs a) 
         }
         auto residual = [&](int c, float (&o)[8]) {
             const int off = kB * (c * 512 + 8 * lane);
-            float x[8], r[8], wp[8], g[8];
-            load8<kT>(xr, off, x);
-            load8<kT>(rr, off, r);
-            load8<kT>(pr, off, wp);
-            gate8(off, g);
-            new_residual<kT>(st, post, x, r, wp, g, o);
+            Eight<kT> x, r, wp, g;
+            x.load(xr, off, 0);
+            r.load(rr, off, 0);
+            if (post) wp.load(pr, off, 0);
+            if (gated) g.load(gr, off, 0);
+            float xf[8];
+            x.floats(xf);
+            const Eight<kT> out = new_residual<kT>(st, post, gated, xf, r, wp, g);
+            out.floats(o);
             if (off >= bytes) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = 0.f;
             }
+            return out;
         };
         p = 0.f;
         for (int c = wave; c < chunks; c += kW) {
@@ -204,11 +278,10 @@ __global__ __launch_bounds__(64 * kW) void gated_norm_kernel(const GatedArgs a) 
         for (int c = wave; c < chunks; c += kW) {
             const int e0 = c * 512 + 8 * lane;
             float o[8], w8[8], n[8];
-            residual(c, o);
-            store8<kT>(ro, kB * e0, o);
+            residual(c, o).store(ro, kB * e0);
             load8<kT>(wr, kB * e0, w8);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) n[j] = e0 < a.H ? (o[j] * inv) * w8[j] : 0.f;
+            for (int j = 0; j < 8; ++j) n[j] = (o[j] * inv) * w8[j];
             put<kT>(a, m, e0, lane, n);
         }
     }
@@ -222,7 +295,9 @@ void launch_cfg(const GatedArgs& a, hipStream_t st) {
 template <int kT>
 void launch_gated(const GatedArgs& a, hipStream_t st) {
     const int chunks = (a.H + 511) / 512;
-    if (chunks <= 4) launch_cfg<4, 1, kT>(a, st);
+    if (chunks <= 1) launch_cfg<1, 1, kT>(a, st);
+    else if (chunks <= 2) launch_cfg<2, 1, kT>(a, st);
+    else if (chunks <= 4) launch_cfg<4, 1, kT>(a, st);
     else if (chunks <= 8) launch_cfg<8, 1, kT>(a, st);
     else if (chunks <= 16) launch_cfg<8, 2, kT>(a, st);
     else if (chunks <= 32) launch_cfg<8, 4, kT>(a, st);
