@@ -21,6 +21,9 @@
 // bits mapped to unsigned integers of the same order, 0 for taken or absent.
 #include "kbn_common.h"
 
+#include <type_traits>
+#include <utility>
+
 namespace kbn {
 namespace {
 
@@ -41,6 +44,7 @@ struct TopkArgs {
     float* w;
     void* ids;
     int id64;
+    int vec, vec_bias;       // rows, bias take loads of four
 };
 
 // Bits in the values' order; -0 and 0 are one value.
@@ -88,15 +92,11 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
     else return (float)static_cast<const _Float16*>(p)[i];
 }
 
+// Token t by the whole wavefront; `mine`: 64 V words of LDS of its own.
 // K: uint32_t where c is the logit, uint64_t where it is score + bias.
 template <int V, int kL, typename K>
-__global__ __launch_bounds__(64 * kWaves) void router_topk_kernel(const TopkArgs a) {
-    __shared__ uint64_t choice[kWaves][64 * V];   // used with groups only
+__device__ __forceinline__ void route_token(const TopkArgs& a, int t, int lane, uint64_t* mine) {
     constexpr bool kBias = sizeof(K) == 8;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x * kWaves + wave;
-    if (t >= a.T) return;   // no barrier follows: each wavefront uses its own part of the LDS
     const float low = -__builtin_inff();
     float l[V];
 #pragma unroll
@@ -138,7 +138,6 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_kernel(const TopkArgs
         if (e >= a.E) key[j] = 0;
     }
     if (a.G > 1) {
-        uint64_t* mine = choice[wave];
 #pragma unroll
         for (int j = 0; j < V; ++j) mine[lane * V + j] = key[j];
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -147,10 +146,16 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_kernel(const TopkArgs
         uint64_t rank = 0;
         if (lane < a.G) {
             uint64_t best = 0, second = 0;
-            for (int i = 0; i < a.per; ++i) {
-                const uint64_t v = mine[lane * a.per + i];
-                second = v > best ? best : (v > second ? v : second);
-                best = v > best ? v : best;
+            // eight at a time: one by one each read waits for the last
+            for (int i0 = 0; i0 < a.per; i0 += 8) {
+                uint64_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = i0 + i < a.per ? mine[lane * a.per + i0 + i] : 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    second = v[i] > best ? best : (v[i] > second ? v[i] : second);
+                    best = v[i] > best ? v[i] : best;
+                }
             }
             rank = best;
             if (kBias && a.per > 1) {
@@ -230,6 +235,393 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_kernel(const TopkArgs
     }
 }
 
+template <int V, int kL, typename K>
+__global__ __launch_bounds__(64 * kWaves) void router_topk_kernel(const TopkArgs a) {
+    __shared__ uint64_t choice[kWaves][64 * V];   // used with groups only
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x * kWaves + wave;
+    if (t >= a.T) return;   // no barrier follows: each wavefront uses its own part of the LDS
+    route_token<V, kL, K>(a, t, lane, choice[wave]);
+}
+
+// ---- Four tokens a wavefront ------------------------------------------------
+// Sixteen lanes a token, lane n holding experts 4 (n + 16 jj) + i in register 4 jj
+// + i (coalesced loads; V = 16 experts a lane at 256).  A key is a choice value in
+// its upper bits and the expert's number in its lower kIB: a value and its owner at
+// once, never equal to another, and sorting is maxima and minima.  Each lane sorts
+// its best eight; four exchanges across the 16 lanes keep the best eight of the
+// token, in order, in every lane, and the best of what was left out.
+//
+// 16-bit logits (no bias) leave the lower bits of a float empty: nothing is lost.
+// Other values go as places between the row's smallest and largest, 24 bits of
+// them, from fp32 scores.  Where neighbours in the order are further apart than the
+// errors of both, the order is the exact one.  Where some are not, the eight and the
+// best one left out are ordered by their 64-bit values, a lane each; that is exact
+// if the last one taken is above whatever else was left out.  A token for which
+// that does not hold either, or whose last kept and first dropped group are too
+// close, is routed again by the whole wavefront in 64 bits (route_token).  (Cut
+// floats in the keys, 2^-15 of the value: 0.5% of tokens took the last way, and at
+// some 7 us a wavefront 1000 tokens 14 us.)
+constexpr int kFastK = 8;
+
+// Exchange with another of the row's 16 lanes: 0 x ^ 1, 1 x ^ 2, 2 the other half of
+// eight, 3 the other eight (after the first two and three all lanes of four and
+// eight hold the same, so mirrors serve).
+template <int kStep>
+__device__ __forceinline__ uint32_t from_other(uint32_t v) {
+    constexpr int ctrl = kStep == 0 ? 0xB1 : kStep == 1 ? 0x4E : kStep == 2 ? 0x141 : 0x128;   // row_half_mirror, row_ror:8
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, false);
+}
+template <int kStep>
+__device__ __forceinline__ float from_other(float v) { return __uint_as_float(from_other<kStep>(__float_as_uint(v))); }
+
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>{}); }
+
+__device__ __forceinline__ void order2(uint32_t& a, uint32_t& b) {   // a >= b
+    const uint32_t hi = max(a, b), lo = min(a, b);
+    a = hi;
+    b = lo;
+}
+// Descending order of eight keys (19 exchanges).
+__device__ __forceinline__ void sort8(uint32_t (&k)[8]) {
+    order2(k[0], k[1]); order2(k[2], k[3]); order2(k[4], k[5]); order2(k[6], k[7]);
+    order2(k[0], k[2]); order2(k[1], k[3]); order2(k[4], k[6]); order2(k[5], k[7]);
+    order2(k[1], k[2]); order2(k[5], k[6]); order2(k[0], k[4]); order2(k[3], k[7]);
+    order2(k[1], k[5]); order2(k[2], k[6]);
+    order2(k[1], k[4]); order2(k[3], k[6]);
+    order2(k[2], k[4]); order2(k[3], k[5]);
+    order2(k[3], k[4]);
+}
+// The best eight of two descending eights, descending, and the best of the rest.
+__device__ __forceinline__ void merge8(uint32_t (&k)[8], const uint32_t (&o)[8], uint32_t& rest) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest = max(rest, min(k[i], o[7 - i]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = max(k[i], o[7 - i]);
+    // the maxima rise and then fall (or the other way round): halves, quarters, pairs
+    order2(k[0], k[4]); order2(k[1], k[5]); order2(k[2], k[6]); order2(k[3], k[7]);
+    order2(k[0], k[2]); order2(k[1], k[3]); order2(k[4], k[6]); order2(k[5], k[7]);
+    order2(k[0], k[1]); order2(k[2], k[3]); order2(k[4], k[5]); order2(k[6], k[7]);
+}
+
+// Largest number of groups: a lane has one.
+constexpr int kFastGroups = 16;
+
+template <int V, int kL, bool kBias>
+__global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const TopkArgs a) {
+    constexpr int Q = V / 4;                                   // quads of experts a lane
+    constexpr int kIB = V == 4 ? 6 : V == 8 ? 7 : V == 16 ? 8 : 9;
+    constexpr uint32_t kIds = (1u << kIB) - 1;
+    // 16-bit logits leave the cut bits empty: nothing is lost
+    constexpr bool kExact = !kBias && kL != kL32;
+    // upper parts of keys: 0 no expert; -inf; values
+    constexpr uint32_t kMaskedPart = kExact ? Masked<uint32_t>::key >> kIB : 1u;
+    constexpr float kPlaces = kIB == 9 ? 8388604.f : 16777212.f;   // 2^(32 - kIB), 2^24 at most, less four
+    __shared__ uint64_t scratch[kWaves][16 * V];               // quads of four tokens, or one token's choice
+    const int lane = threadIdx.x & 63, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t0 = (blockIdx.x * kWaves + wave) * 4;
+    if (t0 >= a.T) return;                                     // no barrier follows
+    const int t = min(t0 + (lane >> 4), a.T - 1);              // past the end: the last token again, not stored
+    const float low = -__builtin_inff();
+    float f[V];
+#pragma unroll
+    for (int jj = 0; jj < Q; ++jj) {
+        const int e = 4 * (n + 16 * jj);
+        const int64_t at = (int64_t)t * a.ld + e;
+        if (a.vec) {
+            if constexpr (kL == kL32) {
+                typedef float f4 __attribute__((ext_vector_type(4)));
+                f4 v{low, low, low, low};
+                if (e < a.E) v = *reinterpret_cast<const f4*>(static_cast<const float*>(a.l) + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[4 * jj + i] = v[i];
+            } else {
+                u32x2 v{0u, 0u};
+                if (e < a.E) v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.l) + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint16_t h = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+                    const float x = kL == kL16b ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+                    f[4 * jj + i] = e < a.E ? x : low;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[4 * jj + i] = e + i < a.E ? load_logit<kL>(a.l, at + i) : low;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = f[j] != f[j] ? low : fminf(f[j], 3.4028234663852886e38f);
+    // Choice values in fp32 and how far they may be from the exact ones: err + 2^-23
+    // of the value.  exp2(x) of |x| < 128 with x off by 2^-24 of itself and the
+    // instruction by 2^-23, u / (1 + u)^2 (1 + |x|) < 0.6, a sum and a reciprocal of
+    // 2^-24 and 2^-23: a sigmoid is off by less than 2^-21.  A softmax adds its sum's
+    // V + 4 roundings: 2^-18.
+    float err = 0.f;
+    if constexpr (kBias) {
+        constexpr float kLog2e = 1.4426950408889634f;
+        float bias[V];
+        if (a.vec_bias) {
+            typedef float f4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int jj = 0; jj < Q; ++jj) {
+                const f4 v = *reinterpret_cast<const f4*>(a.bias + min(4 * (n + 16 * jj), a.E - 4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bias[4 * jj + i] = v[i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) bias[j] = a.bias[min(4 * (n + 16 * (j / 4)) + (j & 3), a.E - 1)];
+        }
+        if (a.sigmoid) {
+            err = 0x1p-21f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * f[j]));
+                f[j] = f[j] == low ? low : s + bias[j];
+            }
+        } else {
+            err = 0x1p-18f;
+            float top = low, sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) top = fmaxf(top, f[j]);
+            top = fmaxf(top, from_other<0>(top));
+            top = fmaxf(top, from_other<1>(top));
+            top = fmaxf(top, from_other<2>(top));
+            top = fmaxf(top, from_other<3>(top));
+            top = top == low ? 0.f : top;
+            float u[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                u[j] = __builtin_amdgcn_exp2f(kLog2e * (f[j] - top));
+                sum += u[j];
+            }
+            sum += from_other<0>(sum);
+            sum += from_other<1>(sum);
+            sum += from_other<2>(sum);
+            sum += from_other<3>(sum);
+            const float over = __builtin_amdgcn_rcpf(sum);
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = f[j] == low ? low : u[j] * over + bias[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = f[j] != f[j] ? low : f[j];
+    }
+    bool groups = true, sure = true;   // the kept groups, the order are the exact ones
+    if (a.G > 1) {
+        // a quad's best, and its two best with a bias; lane g then ranks group g
+        float* const quads = reinterpret_cast<float*>(scratch[wave]) + (lane >> 4) * (16 * Q * 2);
+#pragma unroll
+        for (int jj = 0; jj < Q; ++jj) {
+            const float b1 = fmaxf(f[4 * jj], f[4 * jj + 1]), s1 = fminf(f[4 * jj], f[4 * jj + 1]);
+            const float b2 = fmaxf(f[4 * jj + 2], f[4 * jj + 3]), s2 = fminf(f[4 * jj + 2], f[4 * jj + 3]);
+            *reinterpret_cast<f32x2*>(&quads[2 * (n + 16 * jj)]) = f32x2{fmaxf(b1, b2), fmaxf(fminf(b1, b2), fmaxf(s1, s2))};
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const int quads_of = a.per / 4;   // quads a group
+        float best = low, second = low;
+        for (int i0 = 0; i0 < quads_of; i0 += 4) {
+            f32x2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = *reinterpret_cast<const f32x2*>(&quads[2 * min(n * quads_of + min(i0 + i, quads_of - 1), 16 * Q - 1)]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i0 + i < quads_of) {
+                    second = fmaxf(fminf(best, v[i].x), fmaxf(second, v[i].y));
+                    best = fmaxf(best, v[i].x);
+                }
+        }
+        const float rank = n < a.G ? (kBias ? best + second : best) : low;
+        int before = 0;   // groups that come before this lane's
+        auto compare = [&](float other, int shift) {
+            const int g = (n + 16 - shift) & 15;   // row_ror: lane n gets lane n - shift
+            before += (int)(other > rank) | ((int)(other == rank) & (int)(g < n));
+        };
+        each<15>([&](auto i) {
+            constexpr int shift = decltype(i)::value + 1;
+            compare(__uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(rank), 0x120 + shift, 0xF, 0xF, false)),
+                    shift);
+        });
+        const bool kept = n < a.G && before < a.kept;
+        const uint32_t keep = (uint32_t)(__ballot(kept) >> (lane & 48)) & 0xFFFFu;
+        if constexpr (kBias) {   // (a group's rank is exact without one)
+            float least = kept ? rank : __builtin_inff(), most = kept || n >= a.G ? low : rank;
+            float size = n < a.G ? fmaxf(fabsf(best), fabsf(second)) : 0.f;   // of the sums' terms
+            auto both = [&](float l, float m, float z) {
+                least = fminf(least, l);
+                most = fmaxf(most, m);
+                size = fmaxf(size, z);
+            };
+            both(from_other<0>(least), from_other<0>(most), from_other<0>(size));
+            both(from_other<1>(least), from_other<1>(most), from_other<1>(size));
+            both(from_other<2>(least), from_other<2>(most), from_other<2>(size));
+            both(from_other<3>(least), from_other<3>(most), from_other<3>(size));
+            // two sums of two terms, each off by err + 2^-23 of itself, and rounded
+            if (a.kept < a.G) groups = least - most > 4.f * err + 0x1p-20f * size;
+        }
+#pragma unroll
+        for (int jj = 0; jj < Q; ++jj) {
+            const int quad = n + 16 * jj;
+            const int g = a.per == 4 ? quad : (int)__umulhi(4u * (uint32_t)quad, a.per_magic);
+            const bool in = g < 16 && (keep >> (g & 15) & 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[4 * jj + i] = in ? f[4 * jj + i] : low;
+        }
+    }
+    float lo = __builtin_inff(), hi = low, scale = 0.f;
+    if constexpr (!kExact) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            lo = f[j] == low ? lo : fminf(lo, f[j]);
+            hi = fmaxf(hi, f[j]);
+        }
+        lo = fminf(lo, from_other<0>(lo));
+        hi = fmaxf(hi, from_other<0>(hi));
+        lo = fminf(lo, from_other<1>(lo));
+        hi = fmaxf(hi, from_other<1>(hi));
+        lo = fminf(lo, from_other<2>(lo));
+        hi = fmaxf(hi, from_other<2>(hi));
+        lo = fminf(lo, from_other<3>(lo));
+        hi = fmaxf(hi, from_other<3>(hi));
+        // (one value, none or an infinite one: all in one place, told apart below)
+        scale = hi - lo > 0x1p-100f && hi - lo < __builtin_inff() ? kPlaces * 0.99999f / (hi - lo) : 0.f;
+    }
+    auto part = [&](float v) -> uint32_t {
+        if constexpr (kExact) return order_key(v) >> kIB;
+        const uint32_t q = 2u + (uint32_t)fmaxf((v - lo) * scale, 0.f);   // (of -inf too: a select, no branch)
+        return v == low ? kMaskedPart : q;
+    };
+    uint32_t k[8], rest = 0;
+#pragma unroll
+    for (int b = 0; b < (V + 7) / 8; ++b) {
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (8 * b + j >= V) {
+                o[j] = 0;
+                continue;
+            }
+            const int jj = 2 * b + j / 4, e = 4 * (n + 16 * jj) + (j & 3);
+            o[j] = (part(f[8 * b + j]) << kIB | (kIds - (uint32_t)e)) & (e < a.E ? ~0u : 0u);
+        }
+        sort8(o);
+        if (b == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = o[j];
+        } else {
+            merge8(k, o, rest);
+        }
+    }
+    auto join = [&](auto step) {
+        constexpr int S = decltype(step)::value;
+        uint32_t o[8];
+        rest = max(rest, from_other<S>(rest));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = from_other<S>(k[j]);
+        merge8(k, o, rest);
+    };
+    join(std::integral_constant<int, 0>{});
+    join(std::integral_constant<int, 1>{});
+    join(std::integral_constant<int, 2>{});
+    join(std::integral_constant<int, 3>{});
+    float off = 0.f;   // of a fp32 choice value
+    if constexpr (!kExact) {
+        if constexpr (kBias) off = err + 0x1p-22f * fmaxf(fabsf(lo), fabsf(hi));
+        // a place is off by less than three: the difference, its product, the cut
+        const uint32_t apart = 4u + (uint32_t)fminf(2.f * off * scale, 0x1p30f);
+        int far = 1, values = 1;   // neighbours are far enough apart; all taken are values
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t mine = k[i] >> kIB, next = (i < 7 ? k[i + 1] : rest) >> kIB;
+            // (a value comes before -inf and before nothing)
+            far &= (int)(i >= a.k) | (int)(next <= kMaskedPart) | (int)(mine > next + apart);
+            values &= (int)(i >= a.k) | (int)(mine > kMaskedPart);
+        }
+        // one exact value on the whole row is in order of the numbers; -inf is left to route_token
+        sure = values & (far | ((int)!kBias & (int)(hi == lo)));
+    }
+    // lane n's expert: the n-th of the order, lane 8 the best one left out
+    uint32_t key = n < 8 ? k[0] : n == 8 ? rest : 0u;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) key = n == i ? k[i] : key;
+    const int id = min((int)(kIds - (key & kIds)), a.E - 1);
+    const bool valid = kExact ? (key >> kIB) != 0 && (key >> kIB) != kMaskedPart : (key >> kIB) > kMaskedPart;
+    const float l = fminf(load_logit<kL>(a.l, (int64_t)t * a.ld + id), 3.4028234663852886e38f);
+    double s = 0.0;   // a sigmoid
+    if (a.sigmoid && valid) s = 1.0 / (1.0 + exp(-(double)l));
+    int place = n;
+    if constexpr (!kExact) {
+        if (__any(!sure) && (!kBias || a.sigmoid)) {
+            double c = -__builtin_inf();
+            if (valid) c = kBias ? s + (double)a.bias[id] : (double)l;
+            const int mine = valid ? id : 0x7FFFFFFF;
+            int better = 0;
+            auto compare = [&](auto ctrl) {
+                constexpr int kCtrl = 0x120 + decltype(ctrl)::value;   // row_ror
+                const uint64_t b = (uint64_t)__double_as_longlong(c);
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, kCtrl, 0xF, 0xF, false);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), kCtrl, 0xF, 0xF, false);
+                const int other = __builtin_amdgcn_update_dpp(0, mine, kCtrl, 0xF, 0xF, false);
+                const double v = __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+                better += (int)(v > c) | ((int)(v == c) & (int)(other < mine));
+            };
+            each<15>([&](auto i) { compare(std::integral_constant<int, decltype(i)::value + 1>{}); });
+            place = valid ? better : 15;
+            double last = valid && better == a.k - 1 ? c : -__builtin_inf();
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) last = fmax(last, __shfl_xor(last, d, 64));
+            // nothing else that was left out is above this
+            const double most = (double)lo + ((double)(rest >> kIB) + 2.0) * ((double)hi - (double)lo) / (double)(kPlaces * 0.9999f) + (double)off;
+            const bool above = (rest >> kIB) <= kMaskedPart ? last > -__builtin_inf() : scale > 0.f && last > most;
+            sure = sure || above;
+        }
+        sure = sure && groups;
+    }
+    const bool taken = place < a.k && n <= 8;
+    const bool counts = taken && valid;
+    if (!a.sigmoid) {
+        float top = counts ? l : low;
+        top = fmaxf(top, from_other<0>(top));
+        top = fmaxf(top, from_other<1>(top));
+        top = fmaxf(top, from_other<2>(top));
+        top = fmaxf(top, from_other<3>(top));
+        if (counts) s = exp((double)l - (double)top);
+    }
+    s = counts ? s : 0.0;
+    if (a.renorm) {
+        double all = s;
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) all += __shfl_xor(all, d, 64);
+        s = all > 0.0 ? s / all : 0.0;
+    }
+    if (taken && sure && t0 + (lane >> 4) < a.T) {
+        const int64_t o = (int64_t)t * a.k + place;
+        a.w[o] = (float)(s * (double)a.scale);
+        if (a.id64) static_cast<int64_t*>(a.ids)[o] = id;
+        else static_cast<int32_t*>(a.ids)[o] = id;
+    }
+    if constexpr (!kExact) {
+        const uint64_t unsure = __ballot(!sure);
+        for (int i = 0; i < 4; ++i)
+            if ((unsure >> (16 * i) & 1) && t0 + i < a.T) {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                route_token<Q, kL, std::conditional_t<kBias, uint64_t, uint32_t>>(a, t0 + i, lane, scratch[wave]);
+            }
+    }
+}
+
 template <int V, typename K>
 void launch(const TopkArgs& a, int dtype, hipStream_t st) {
     const dim3 grid((unsigned)((a.T + kWaves - 1) / kWaves)), block(64 * kWaves);
@@ -245,6 +637,28 @@ void launch_for(const TopkArgs& a, int dtype, hipStream_t st) {
     else if (a.E <= 256) launch<4, K>(a, dtype, st);
     else if (a.E <= 512) launch<8, K>(a, dtype, st);
     else launch<16, K>(a, dtype, st);
+}
+
+template <int V, bool kBias>
+void launch_rows(const TopkArgs& a, int dtype, hipStream_t st) {
+    const dim3 grid((unsigned)((a.T + 4 * kWaves - 1) / (4 * kWaves))), block(64 * kWaves);
+    if (dtype == kL16b) router_topk_rows_kernel<V, kL16b, kBias><<<grid, block, 0, st>>>(a);
+    else if (dtype == kL16f) router_topk_rows_kernel<V, kL16f, kBias><<<grid, block, 0, st>>>(a);
+    else router_topk_rows_kernel<V, kL32, kBias><<<grid, block, 0, st>>>(a);
+}
+
+template <bool kBias>
+void launch_rows_for(const TopkArgs& a, int dtype, hipStream_t st) {
+    if (a.E <= 64) launch_rows<4, kBias>(a, dtype, st);
+    else if (a.E <= 128) launch_rows<8, kBias>(a, dtype, st);
+    else if (a.E <= 256) launch_rows<16, kBias>(a, dtype, st);
+    else launch_rows<32, kBias>(a, dtype, st);
+}
+
+// What the four-token kernel covers: up to eight experts a token, quads that lie
+// in one group, and weights that need no sum over the row.
+bool rows_cover(const TopkArgs& a) {
+    return a.k <= kFastK && a.E <= 512 && (a.G == 1 || (a.G <= kFastGroups && a.per % 4 == 0)) && (a.sigmoid || a.renorm);
 }
 
 }  // namespace
@@ -287,8 +701,12 @@ extern "C" int kbn_moe_router_topk(const void* logits, int dtype, int64_t ld, co
     a.w = weights;
     a.ids = ids;
     a.id64 = id_bytes == 8;
+    const int64_t size = dtype == kL32 ? 4 : 2;
+    a.vec = E % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0 && (T == 1 || ld % 4 == 0);
+    a.vec_bias = E % 4 == 0 && aligned16(bias);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (bias) launch_for<uint64_t>(a, dtype, st);
+    if (rows_cover(a)) bias ? launch_rows_for<true>(a, dtype, st) : launch_rows_for<false>(a, dtype, st);
+    else if (bias) launch_for<uint64_t>(a, dtype, st);
     else launch_for<uint32_t>(a, dtype, st);
     KBN_CHECK_LAUNCH(what);
     return 0;
