@@ -7,12 +7,14 @@
 // workgroups, fp32 partial sums [S, T, R]) and out (the partial sums added in
 // order, so results do not depend on which workgroup ends first).
 //
-// Tokens go by windows, of 256 (of 64 where there are more than 64 adapters, so
-// that few tokens share one).  A workgroup finds the window's adapters in order
-// of appearance and works on chunks of one adapter's tokens, which need not be
-// neighbours: a decode batch reads each adapter once a window, a window inside one
-// prompt has one adapter and full chunks.  Nothing has to be known of the ids on
-// the host.
+// Tokens go by windows, of 256 (of 64 where there are more than 63 adapters, so
+// that few tokens share one).  A workgroup works on chunks of one adapter's tokens
+// in a window, which need not be neighbours: a decode batch reads each adapter once
+// a window, a window inside one prompt has one adapter and full chunks.  It finds its
+// chunks by counting each adapter's tokens, a lane an adapter (adapter after adapter
+// in order of appearance, each waits for the last: 5 us of 15 for 32 tokens of 24
+// adapters), or in order of appearance where adapters are more than lanes.  Nothing
+// has to be known of the ids on the host.
 //
 // h enters the second product as the sum of two bf16 numbers (16 bits of its
 // significand, 2^-16 of the value lost, far below the output's own rounding).
@@ -46,16 +48,33 @@ struct LoraArgs {
     int blocks;          // 256-column blocks of a workgroup of the second launch
 };
 
-// A window of kWords x 64 tokens: lane i's adapter of each 64, the window's
-// adapters in order of appearance, and chunks of their tokens.  kNone: the tokens
-// without an adapter come as those of adapter -1, else they do not come.
-template <int kWords, bool kNone>
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_up_to(int v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(v, d, 64);
+        v += lane >= d ? o : 0;
+    }
+    return v;
+}
+
+// A window of kWords x 64 tokens (lane i has the adapter of token i of each 64; -1:
+// none, -2: no token), and its chunks of at most kSize tokens of one adapter, by
+// number.  kNone: the tokens without an adapter come too, as those of adapter -1.
+// kMode 0: chunks in order of their adapters' appearance; 1 (64 tokens) and 2 (256):
+// at most 63 adapters, in order of their numbers.
+constexpr int kIndexed = 63;
+constexpr int words_of(int mode) { return mode == 2 ? 4 : 1; }
+template <int kMode, int kSize, bool kNone>
 struct Window {
+    static constexpr int kWords = words_of(kMode);
     int t0;
     int id[kWords];
-    uint64_t left[kWords];    // tokens whose adapter was not yet taken
-    uint64_t now[kWords];     // tokens of the adapter that is
-    int adapter, n;           // it, and how many
+    int count, end;           // by number: this lane's adapter's tokens, chunks up to it
+    uint64_t left;            // by appearance: tokens whose adapter was not yet passed
+    int passed;               // chunks of those that were
+    uint64_t now[kWords];     // tokens of the chunk's adapter
+    int adapter, from, n;     // it, and the chunk's tokens among them
     __device__ __forceinline__ Window(const LoraArgs& a, int w, int lane) {
         t0 = w * 64 * kWords;
 #pragma unroll
@@ -64,35 +83,61 @@ struct Window {
             int64_t v = -1;
             if (t < a.T) v = a.id64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t)static_cast<const int32_t*>(a.ids)[t];
             id[k] = t >= a.T ? -2 : v >= 0 && v < a.L ? (int)v : -1;
-            left[k] = __ballot(id[k] >= (kNone ? -1 : 0));
+        }
+        if constexpr (kMode > 0) {
+            count = 0;
+#pragma unroll 4
+            for (int l = kNone ? -1 : 0; l < a.L; ++l) {
+                const int c = tokens_of(l);
+                count = (lane == (l & 63)) ? c : count;   // (none: the last lane)
+            }
+            end = lanes_up_to((count + kSize - 1) / kSize, lane);
+        } else {
+            left = __ballot(id[0] >= (kNone ? -1 : 0));
+            passed = 0;
         }
     }
-    // The next adapter; false if there is none.
-    __device__ __forceinline__ bool next() {
-        bool found = false;
+    __device__ __forceinline__ int tokens_of(int l) const {
+        int c = 0;
 #pragma unroll
-        for (int k = 0; k < kWords; ++k)
-            if (!found && left[k]) {
-                adapter = __builtin_amdgcn_readlane(id[k], (int)__builtin_ctzll(left[k]));
-                found = true;
+        for (int k = 0; k < kWords; ++k) c += (int)__builtin_popcountll(__ballot(id[k] == l));
+        return c;
+    }
+    // Chunk p, numbers rising from call to call; false if there is none.
+    __device__ __forceinline__ bool seek(int p) {
+        int all;
+        if constexpr (kMode > 0) {
+            const uint64_t at = __ballot(end > p);
+            if (!at) return false;
+            const int l = (int)__builtin_ctzll(at);
+            all = __builtin_amdgcn_readlane(count, l);
+            from = (p - (__builtin_amdgcn_readlane(end, l) - (all + kSize - 1) / kSize)) * kSize;
+            adapter = l == 63 ? -1 : l;
+        } else {
+            for (;;) {
+                if (!left) return false;
+                adapter = __builtin_amdgcn_readlane(id[0], (int)__builtin_ctzll(left));
+                const uint64_t m = __ballot(id[0] == adapter);
+                all = (int)__builtin_popcountll(m);
+                const int chunks = (all + kSize - 1) / kSize;
+                from = (p - passed) * kSize;
+                if (p < passed + chunks) break;
+                passed += chunks;
+                left &= ~m;
             }
-        if (!found) return false;
-        n = 0;
-#pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-            now[k] = __ballot(id[k] == adapter);
-            left[k] &= ~now[k];
-            n += __builtin_popcountll(now[k]);
         }
+        n = min(kSize, all - from);
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) now[k] = __ballot(id[k] == adapter);
         return true;
     }
-    // Writes tokens from .. from + count - 1 of now, as places in the window (one wavefront).
-    __device__ __forceinline__ void list(int from, int count, int lane, uint8_t* to) const {
+    // Writes the chunk's tokens as places in the window (one wavefront).
+    __device__ __forceinline__ void list(int lane, uint8_t* to) const {
         int before = -from;
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
             const int at = before + (int)__builtin_popcountll(now[k] & ((1ull << lane) - 1));
-            if ((now[k] >> lane & 1) && at >= 0 && at < count) to[at] = (uint8_t)(64 * k + lane);
+            if ((now[k] >> lane & 1) && at >= 0 && at < n) to[at] = (uint8_t)(64 * k + lane);
             before += (int)__builtin_popcountll(now[k]);
         }
     }
@@ -127,27 +172,21 @@ __device__ __forceinline__ void shrink_tile(const LoraArgs& a, int t0, int place
 }
 
 // grid (splits, windows, slots x rank chunks)
-template <int kD, int kTR, int kWords>
+template <int kD, int kTR, int kMode>
 __global__ __launch_bounds__(64 * kStreamWaves) void lora_shrink_kernel(const LoraArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[Stream<4, kTR, 2, kD, kD>::kSmem];
     const int lane = threadIdx.x & 63;
     const int parts = (a.R + kRankChunk - 1) / kRankChunk;
     const int r0 = blockIdx.z % parts * kRankChunk;
-    int skip = blockIdx.z / parts;   // chunks until this workgroup's next one
-    Window<kWords, false> win(a, blockIdx.y, lane);
-    while (win.next()) {
-        for (int from = 0; from < win.n; from += kChunk) {
-            if (skip-- > 0) continue;
-            skip = a.slots1 - 1;
-            const int n = min(kChunk, win.n - from);
-            if (threadIdx.x < 64) win.list(from, n, lane, smem);
-            __syncthreads();
-            const int list = smem[min(lane, n - 1)];
-            __syncthreads();
-            if (n <= 16) shrink_tile<kD, 1, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
-            else if (n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
-            else shrink_tile<kD, 4, kTR>(a, win.t0, 64 * kWords, n, list, win.adapter, r0, blockIdx.x, smem);
-        }
+    Window<kMode, kChunk, false> win(a, blockIdx.y, lane);
+    for (int p = blockIdx.z / parts; win.seek(p); p += a.slots1) {
+        if (threadIdx.x < 64) win.list(lane, smem);
+        __syncthreads();
+        const int n = win.n, list = smem[min(lane, n - 1)];
+        __syncthreads();
+        if (n <= 16) shrink_tile<kD, 1, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
+        else if (n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
+        else shrink_tile<kD, 4, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
     }
 }
 
@@ -210,7 +249,7 @@ __device__ __forceinline__ u32x2 added(const u32x2& was, float v0, float v1, flo
 // h comes from LDS, summed over the splits and cut in two by the workgroup.
 // kKS: steps of 32 ranks whose rows of B are asked for ahead of h (0: any rank).
 // kVec: base and out go four columns at a time.
-template <int kD, int kKS, int kWords, bool kVec>
+template <int kD, int kKS, int kMode, bool kVec>
 __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const LoraArgs a) {
     constexpr int kRow = (kKS ? 32 * kKS : kMaxRank) + 8;   // values of a row of h: an odd number of 16-byte slots
     constexpr int kTM = kRows / 16;
@@ -219,7 +258,8 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = lane & 15, q = lane >> 4;
-    Window<kWords, true> win(a, blockIdx.y, lane);
+    constexpr int kWords = words_of(kMode);
+    Window<kMode, kRows, true> win(a, blockIdx.y, lane);
     const uint16_t* const base = static_cast<const uint16_t*>(a.base) + (int64_t)win.t0 * a.ld_b;
     uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)win.t0 * a.ld_o;
     const int rows = (int)min((int64_t)64 * kWords, (int64_t)a.T - win.t0);
@@ -231,186 +271,183 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
 #pragma unroll
     for (int k = 0; k < (kKS ? kKS : 1); ++k) wo[k] = 32 * k + 8 * q < a.R ? (4 * row * a.R + 32 * k + 8 * q) * 2 : kOob;
     uint8_t* const mine = places[wave];
-    int skip = blockIdx.z;
-    while (win.next()) {
-        for (int from = 0; from < win.n; from += kRows) {
-            if (skip-- > 0) continue;
-            skip = a.slots2 - 1;
-            const int n = min(kRows, win.n - from), tiles = (n + 15) / 16;
-            const bool copy = win.adapter < 0;
-            if (copy && a.base == a.out) continue;
-            win.list(from, n, lane, mine);   // each wavefront for itself
-            wave_lds_fence();
-            const __amdgpu_buffer_rsrc_t br = rsrc(static_cast<const uint8_t*>(a.b) + (int64_t)win.adapter * a.N * a.R * 2,
-                                                   copy ? 0 : (int)((int64_t)a.N * a.R * 2));
-            // h of the chunk's tokens, eight ranks of one a thread: asked for first,
-            // as everything waits for it
-            const int octets = (a.R + 31) / 32 * 4;
-            const float sc = a.scaling && !copy ? a.scaling[win.adapter] : 1.f;
-            f32x4 u[kMaxSplits][2];
-            auto load_h = [&](int s) {
-                const int i = s / octets, r = s % octets * 8;
-                const bool in = i < n && r < a.R && !copy;
-                const float* hp = a.h + (in ? (int64_t)(win.t0 + mine[i & (kRows - 1)]) * a.R + r : 0);
+    for (int p = blockIdx.z; win.seek(p); p += a.slots2) {
+        const int n = win.n, tiles = (n + 15) / 16;
+        const bool copy = win.adapter < 0;
+        if (copy && a.base == a.out) continue;
+        win.list(lane, mine);   // each wavefront for itself
+        wave_lds_fence();
+        const __amdgpu_buffer_rsrc_t br = rsrc(static_cast<const uint8_t*>(a.b) + (int64_t)win.adapter * a.N * a.R * 2,
+                                               copy ? 0 : (int)((int64_t)a.N * a.R * 2));
+        // h of the chunk's tokens, eight ranks of one a thread: asked for first,
+        // as everything waits for it
+        const int octets = (a.R + 31) / 32 * 4;
+        const float sc = a.scaling && !copy ? a.scaling[win.adapter] : 1.f;
+        f32x4 u[kMaxSplits][2];
+        auto load_h = [&](int s) {
+            const int i = s / octets, r = s % octets * 8;
+            const bool in = i < n && r < a.R && !copy;
+            const float* hp = a.h + (in ? (int64_t)(win.t0 + mine[i & (kRows - 1)]) * a.R + r : 0);
 #pragma unroll
-                for (int k = 0; k < kMaxSplits; ++k) {
-                    u[k][0] = u[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (k < a.splits && in) {
-                        u[k][0] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R);
-                        u[k][1] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R + 4);
-                    }
+            for (int k = 0; k < kMaxSplits; ++k) {
+                u[k][0] = u[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (k < a.splits && in) {
+                    u[k][0] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R);
+                    u[k][1] = *reinterpret_cast<const f32x4*>(hp + (int64_t)k * a.T * a.R + 4);
                 }
-            };
-            // summed over the splits, scaled, cut in two; zeros past the rank and past the tokens
-            auto put_h = [&](int s) {
-                const int i = s / octets, r = s % octets * 8;
-                float v[8];
+            }
+        };
+        // summed over the splits, scaled, cut in two; zeros past the rank and past the tokens
+        auto put_h = [&](int s) {
+            const int i = s / octets, r = s % octets * 8;
+            float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = u[0][j / 4][j & 3];
+            for (int j = 0; j < 8; ++j) v[j] = u[0][j / 4][j & 3];
 #pragma unroll
-                for (int k = 1; k < kMaxSplits; ++k)
-                    if (k < a.splits) {
+            for (int k = 1; k < kMaxSplits; ++k)
+                if (k < a.splits) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] += u[k][j / 4][j & 3];
-                    }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= sc;
-                u32x4 hi, lo;
-                split8(v, hi, lo);
-                if (i < 16 * tiles) {
-                    *reinterpret_cast<u32x4*>(&part[0][i * kRow + r]) = hi;
-                    *reinterpret_cast<u32x4*>(&part[1][i * kRow + r]) = lo;
+                    for (int j = 0; j < 8; ++j) v[j] += u[k][j / 4][j & 3];
                 }
-            };
-            if constexpr (kKS > 0) load_h(threadIdx.x);   // 32 tokens x 8 octets at most
-            // a lane's tokens in base and out: 4 q + i of each 16 of the chunk
-            int bo_at[kTM][4], oo_at[kTM][4];
 #pragma unroll
-            for (int m = 0; m < kTM; ++m)
+            for (int j = 0; j < 8; ++j) v[j] *= sc;
+            u32x4 hi, lo;
+            split8(v, hi, lo);
+            if (i < 16 * tiles) {
+                *reinterpret_cast<u32x4*>(&part[0][i * kRow + r]) = hi;
+                *reinterpret_cast<u32x4*>(&part[1][i * kRow + r]) = lo;
+            }
+        };
+        if constexpr (kKS > 0) load_h(threadIdx.x);   // 32 tokens x 8 octets at most
+        // a lane's tokens in base and out: 4 q + i of each 16 of the chunk
+        int bo_at[kTM][4], oo_at[kTM][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = 16 * m + 4 * q + i, t = mine[min(at, n - 1)];
-                    bo_at[m][i] = at < n ? (t * (int)a.ld_b + 4 * row) * 2 : kOob;
-                    oo_at[m][i] = at < n ? (t * (int)a.ld_o + 4 * row) * 2 : kOob;
-                }
-            struct Strip {
-                u32x2 was[kTM][4];
-                u32x4 w[kKS ? kKS : 1][4];
-            };
-            auto load_b = [&](int n0, int k, u32x4 (&to)[4]) __attribute__((always_inline)) {
-                const int off = kKS ? wo[kKS ? k : 0] : 32 * k + 8 * q < a.R ? (4 * row * a.R + 32 * k + 8 * q) * 2 : kOob;
+        for (int m = 0; m < kTM; ++m)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) to[j] = __builtin_amdgcn_raw_buffer_load_b128(br, off, (n0 + j) * a.R * 2, 0);
-            };
-            auto ask = [&](int n0, Strip& t) __attribute__((always_inline)) {
-                if constexpr (kKS > 0) {
+            for (int i = 0; i < 4; ++i) {
+                const int at = 16 * m + 4 * q + i, t = mine[min(at, n - 1)];
+                bo_at[m][i] = at < n ? (t * (int)a.ld_b + 4 * row) * 2 : kOob;
+                oo_at[m][i] = at < n ? (t * (int)a.ld_o + 4 * row) * 2 : kOob;
+            }
+        struct Strip {
+            u32x2 was[kTM][4];
+            u32x4 w[kKS ? kKS : 1][4];
+        };
+        auto load_b = [&](int n0, int k, u32x4 (&to)[4]) __attribute__((always_inline)) {
+            const int off = kKS ? wo[kKS ? k : 0] : 32 * k + 8 * q < a.R ? (4 * row * a.R + 32 * k + 8 * q) * 2 : kOob;
 #pragma unroll
-                    for (int k = 0; k < kKS; ++k) load_b(n0, k, t.w[k]);
-                }
-                if constexpr (kVec) {   // (past N a row's columns are the next row's: the last strip masks them)
-                    const bool in = n0 + 4 * row < a.N;
+            for (int j = 0; j < 4; ++j) to[j] = __builtin_amdgcn_raw_buffer_load_b128(br, off, (n0 + j) * a.R * 2, 0);
+        };
+        auto ask = [&](int n0, Strip& t) __attribute__((always_inline)) {
+            if constexpr (kKS > 0) {
 #pragma unroll
-                    for (int m = 0; m < kTM; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            t.was[m][i] = __builtin_amdgcn_raw_buffer_load_b64(bi, in ? bo_at[m][i] : kOob, n0 * 2, 0);
-                }
-            };
-            auto finish = [&](int n0, Strip& t) __attribute__((always_inline)) {
-                f32x4 acc[kTM][4];
+                for (int k = 0; k < kKS; ++k) load_b(n0, k, t.w[k]);
+            }
+            if constexpr (kVec) {   // (past N a row's columns are the next row's: the last strip masks them)
+                const bool in = n0 + 4 * row < a.N;
 #pragma unroll
                 for (int m = 0; m < kTM; ++m)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                auto step = [&](int kk, u32x4 (&b)[4]) __attribute__((always_inline)) {
-                    u32x4 bl[4];
-                    if constexpr (kD == kG16f) {   // as two bf16 numbers (exact): h may pass fp16's range
+                    for (int i = 0; i < 4; ++i)
+                        t.was[m][i] = __builtin_amdgcn_raw_buffer_load_b64(bi, in ? bo_at[m][i] : kOob, n0 * 2, 0);
+            }
+        };
+        auto finish = [&](int n0, Strip& t) __attribute__((always_inline)) {
+            f32x4 acc[kTM][4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float wf[8];
-                            to_floats<kG16f>(Raw8<kG16f>{{b[j]}}, wf);
-                            split8(wf, b[j], bl[j]);
-                        }
-                    }
+            for (int m = 0; m < kTM; ++m)
 #pragma unroll
-                    for (int m = 0; m < kTM; ++m) {
-                        if (m >= tiles) continue;
-                        const u32x4 hh = *reinterpret_cast<const u32x4*>(&part[0][(16 * m + row) * kRow + 32 * kk + 8 * q]);
-                        const u32x4 hl = *reinterpret_cast<const u32x4*>(&part[1][(16 * m + row) * kRow + 32 * kk + 8 * q]);
+                for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            auto step = [&](int kk, u32x4 (&b)[4]) __attribute__((always_inline)) {
+                u32x4 bl[4];
+                if constexpr (kD == kG16f) {   // as two bf16 numbers (exact): h may pass fp16's range
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if constexpr (kD == kG16f) acc[m][j] = mma<false>(hh, bl[j], acc[m][j]);
-                            acc[m][j] = mma<false>(hl, b[j], acc[m][j]);
-                            acc[m][j] = mma<false>(hh, b[j], acc[m][j]);
-                        }
-                    }
-                };
-                if constexpr (kKS > 0) {
-#pragma unroll
-                    for (int kk = 0; kk < kKS; ++kk) step(kk, t.w[kk]);
-                } else if (!copy) {
-                    for (int kk = 0; 32 * kk < a.R; ++kk) {
-                        load_b(n0, kk, t.w[0]);
-                        step(kk, t.w[0]);
+                    for (int j = 0; j < 4; ++j) {
+                        float wf[8];
+                        to_floats<kG16f>(Raw8<kG16f>{{b[j]}}, wf);
+                        split8(wf, b[j], bl[j]);
                     }
                 }
-                const int c = n0 + 4 * row;
 #pragma unroll
                 for (int m = 0; m < kTM; ++m) {
                     if (m >= tiles) continue;
+                    const u32x4 hh = *reinterpret_cast<const u32x4*>(&part[0][(16 * m + row) * kRow + 32 * kk + 8 * q]);
+                    const u32x4 hl = *reinterpret_cast<const u32x4*>(&part[1][(16 * m + row) * kRow + 32 * kk + 8 * q]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (kVec) {
-                            const u32x2 y = copy ? t.was[m][i] : added<kD>(t.was[m][i], acc[m][0][i], acc[m][1][i], acc[m][2][i], acc[m][3][i]);
-                            __builtin_amdgcn_raw_buffer_store_b64(y, bo, c < a.N ? oo_at[m][i] : kOob, n0 * 2, 0);
-                        } else if (16 * m + 4 * q + i < n) {
-                            const int64_t at = mine[16 * m + 4 * q + i];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c + e < a.N) {
-                                    const uint16_t v = base[at * a.ld_b + c + e];
-                                    out[at * a.ld_o + c + e] = copy ? v : value_to(kD, value_of(kD, v) + acc[m][e][i]);
-                                }
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (kD == kG16f) acc[m][j] = mma<false>(hh, bl[j], acc[m][j]);
+                        acc[m][j] = mma<false>(hl, b[j], acc[m][j]);
+                        acc[m][j] = mma<false>(hh, b[j], acc[m][j]);
                     }
                 }
             };
-            Strip one, two;
-            ask(first, one);
-            __syncthreads();   // part of the last chunk is done with
             if constexpr (kKS > 0) {
-                put_h(threadIdx.x);
-            } else {
-                for (int s = threadIdx.x; s < 16 * tiles * octets; s += 64 * kStreamWaves) {
-                    load_h(s);
-                    put_h(s);
+#pragma unroll
+                for (int kk = 0; kk < kKS; ++kk) step(kk, t.w[kk]);
+            } else if (!copy) {
+                for (int kk = 0; 32 * kk < a.R; ++kk) {
+                    load_b(n0, kk, t.w[0]);
+                    step(kk, t.w[0]);
                 }
             }
-            __syncthreads();
-            // the next strip is asked for before this one is done
-            const int end = min(a.N, (int)(blockIdx.x + 1) * a.blocks * kColumns);
-            for (int n0 = first; n0 < end; n0 += 2 * kColumns) {
-                const int n1 = n0 + kColumns;
-                if (n1 < end) ask(n1, two);
-                finish(n0, one);
-                if (n1 >= end) break;
-                if (n1 + kColumns < end) ask(n1 + kColumns, one);
-                finish(n1, two);
+            const int c = n0 + 4 * row;
+#pragma unroll
+            for (int m = 0; m < kTM; ++m) {
+                if (m >= tiles) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (kVec) {
+                        const u32x2 y = copy ? t.was[m][i] : added<kD>(t.was[m][i], acc[m][0][i], acc[m][1][i], acc[m][2][i], acc[m][3][i]);
+                        __builtin_amdgcn_raw_buffer_store_b64(y, bo, c < a.N ? oo_at[m][i] : kOob, n0 * 2, 0);
+                    } else if (16 * m + 4 * q + i < n) {
+                        const int64_t at = mine[16 * m + 4 * q + i];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.N) {
+                                const uint16_t v = base[at * a.ld_b + c + e];
+                                out[at * a.ld_o + c + e] = copy ? v : value_to(kD, value_of(kD, v) + acc[m][e][i]);
+                            }
+                    }
+                }
             }
+        };
+        Strip one, two;
+        ask(first, one);
+        __syncthreads();   // part of the last chunk is done with
+        if constexpr (kKS > 0) {
+            put_h(threadIdx.x);
+        } else {
+            for (int s = threadIdx.x; s < 16 * tiles * octets; s += 64 * kStreamWaves) {
+                load_h(s);
+                put_h(s);
+            }
+        }
+        __syncthreads();
+        // the next strip is asked for before this one is done
+        const int end = min(a.N, (int)(blockIdx.x + 1) * a.blocks * kColumns);
+        for (int n0 = first; n0 < end; n0 += 2 * kColumns) {
+            const int n1 = n0 + kColumns;
+            if (n1 < end) ask(n1, two);
+            finish(n0, one);
+            if (n1 >= end) break;
+            if (n1 + kColumns < end) ask(n1 + kColumns, one);
+            finish(n1, two);
         }
     }
 }
 
-// Windows of words x 64 tokens, workgroups a window that share its chunks in each
+// How a window finds its chunks, workgroups a window that share its chunks in each
 // launch, K splits of the first and 256-column blocks of a workgroup of the second.
 struct LoraPlan {
-    int words, windows, slots1, slots2, splits, blocks;
+    int mode, windows, slots1, slots2, splits, blocks;
 };
 LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     LoraPlan p;
-    p.words = L > 64 || T <= 64 ? 1 : 4;
-    const int64_t size = std::min<int64_t>(T, 64 * p.words), cus = cu_count();
-    p.windows = (int)((T + 64 * p.words - 1) / (64 * p.words));
+    // (up to eight tokens are passed one by one sooner than 24 adapters are counted)
+    p.mode = L > kIndexed || T <= 8 ? 0 : T <= 64 ? 1 : 2;
+    const int64_t tokens = 64 * words_of(p.mode);
+    const int64_t size = std::min<int64_t>(T, tokens), cus = cu_count();
+    p.windows = (int)((T + tokens - 1) / tokens);
     // chunks a window can have: full ones, and a last one of each adapter; in many
     // windows (prompts) mostly the full ones, and the rest waits its turn
     const int64_t adapters = std::min(L, size), last = p.windows > 2 ? std::min<int64_t>(adapters, 2) : adapters;
@@ -428,19 +465,19 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     return p;
 }
 
-template <int kD, int kWords>
+template <int kD, int kMode>
 void launch_lora(const LoraArgs& a, const LoraPlan& p, bool vec, hipStream_t st) {
     const int parts = (a.R + kRankChunk - 1) / kRankChunk;
     const dim3 grid((unsigned)a.splits, (unsigned)p.windows, (unsigned)(a.slots1 * parts)), block(64 * kStreamWaves);
-    if (a.R <= 16) lora_shrink_kernel<kD, 1, kWords><<<grid, block, 0, st>>>(a);
-    else if (a.R <= 32) lora_shrink_kernel<kD, 2, kWords><<<grid, block, 0, st>>>(a);
-    else lora_shrink_kernel<kD, 4, kWords><<<grid, block, 0, st>>>(a);
+    if (a.R <= 16) lora_shrink_kernel<kD, 1, kMode><<<grid, block, 0, st>>>(a);
+    else if (a.R <= 32) lora_shrink_kernel<kD, 2, kMode><<<grid, block, 0, st>>>(a);
+    else lora_shrink_kernel<kD, 4, kMode><<<grid, block, 0, st>>>(a);
     const int cols = kColumns * a.blocks;
     const dim3 egrid((unsigned)((a.N + cols - 1) / cols), (unsigned)p.windows, (unsigned)a.slots2);
-    if (!vec) lora_expand_kernel<kD, 0, kWords, false><<<egrid, block, 0, st>>>(a);
-    else if (a.R <= 32) lora_expand_kernel<kD, 1, kWords, true><<<egrid, block, 0, st>>>(a);
-    else if (a.R <= 64) lora_expand_kernel<kD, 2, kWords, true><<<egrid, block, 0, st>>>(a);
-    else lora_expand_kernel<kD, 0, kWords, true><<<egrid, block, 0, st>>>(a);
+    if (!vec) lora_expand_kernel<kD, 0, kMode, false><<<egrid, block, 0, st>>>(a);
+    else if (a.R <= 32) lora_expand_kernel<kD, 1, kMode, true><<<egrid, block, 0, st>>>(a);
+    else if (a.R <= 64) lora_expand_kernel<kD, 2, kMode, true><<<egrid, block, 0, st>>>(a);
+    else lora_expand_kernel<kD, 0, kMode, true><<<egrid, block, 0, st>>>(a);
 }
 
 }  // namespace
@@ -504,8 +541,15 @@ extern "C" int kbn_lora_add(const void* x, int dtype, int64_t ld_x, const void* 
     const bool vec = N % 4 == 0 && aligned8(base) && aligned8(out) && ld_base % 4 == 0 && ld_out % 4 == 0 && ld_base < (1 << 22) &&
             ld_out < (1 << 22);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == kG16b) p.words == 1 ? launch_lora<kG16b, 1>(a, p, vec, st) : launch_lora<kG16b, 4>(a, p, vec, st);
-    else p.words == 1 ? launch_lora<kG16f, 1>(a, p, vec, st) : launch_lora<kG16f, 4>(a, p, vec, st);
+    if (dtype == kG16b) {
+        if (p.mode == 0) launch_lora<kG16b, 0>(a, p, vec, st);
+        else if (p.mode == 1) launch_lora<kG16b, 1>(a, p, vec, st);
+        else launch_lora<kG16b, 2>(a, p, vec, st);
+    } else {
+        if (p.mode == 0) launch_lora<kG16f, 0>(a, p, vec, st);
+        else if (p.mode == 1) launch_lora<kG16f, 1>(a, p, vec, st);
+        else launch_lora<kG16f, 2>(a, p, vec, st);
+    }
     KBN_CHECK_LAUNCH(what);
     return 0;
 }
