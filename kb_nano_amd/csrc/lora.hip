@@ -460,7 +460,8 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cus + busy - 1) / busy, few, kMaxSplits, units / kStreamWaves}));
     // of the second launch's workgroups a CU holds two, and one takes about 5 us
     // whatever its columns: one round of them
-    const int64_t cols = (N + kColumns - 1) / kColumns, all = p.windows * std::min<int64_t>(p.slots2, (size + kRows - 1) / kRows + adapters);
+    const int64_t cols = (N + kColumns - 1) / kColumns;
+    const int64_t all = p.windows * std::min<int64_t>(p.slots2, (size + kRows - 1) / kRows + adapters);
     p.blocks = (int)std::max<int64_t>(1, std::min(cols, (all * cols + 2 * cus - 1) / (2 * cus)));
     return p;
 }

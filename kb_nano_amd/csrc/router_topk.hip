@@ -357,8 +357,9 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
             for (int i = 0; i < 4; ++i) f[4 * jj + i] = e + i < a.E ? load_logit<kL>(a.l, at + i) : low;
         }
     }
+    // (the larger of a NaN and -inf is -inf; as a median of three the compiler drops the -inf)
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = f[j] != f[j] ? low : fminf(f[j], 3.4028234663852886e38f);
+    for (int j = 0; j < V; ++j) f[j] = fminf(fmaxf(f[j], low), 3.4028234663852886e38f);
     // Choice values in fp32 and how far they may be from the exact ones: err + 2^-23
     // of the value.  exp2(x) of |x| < 128 with x off by 2^-24 of itself and the
     // instruction by 2^-23, u / (1 + u)^2 (1 + |x|) < 0.6, a sum and a reciprocal of
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
             for (int j = 0; j < V; ++j) f[j] = f[j] == low ? low : u[j] * over + bias[j];
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = f[j] != f[j] ? low : f[j];
+        for (int j = 0; j < V; ++j) f[j] = fmaxf(f[j], low);   // a NaN counts as -inf
     }
     bool groups = true, sure = true;   // the kept groups, the order are the exact ones
     if (a.G > 1) {
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
             for (int i = 0; i < 4; ++i) f[4 * jj + i] = in ? f[4 * jj + i] : low;
         }
     }
-    float lo = __builtin_inff(), hi = low, scale = 0.f;
+    float lo = __builtin_inff(), hi = low, scale = 0.f, from = 2.f;
     if constexpr (!kExact) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -493,13 +494,16 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
         hi = fmaxf(hi, from_other<2>(hi));
         lo = fminf(lo, from_other<3>(lo));
         hi = fmaxf(hi, from_other<3>(hi));
-        // (one value, none or an infinite one: all in one place, told apart below)
-        scale = hi - lo > 0x1p-100f && hi - lo < __builtin_inff() ? kPlaces * 0.99999f / (hi - lo) : 0.f;
+        // (one value, none, an infinite one, or values close together far from 0, whose
+        // places would be off by more than is left at the end: all in one place)
+        const float range = hi - lo;
+        const bool fits = range > 0x1p-100f && range < __builtin_inff() && fmaxf(fabsf(lo), fabsf(hi)) < 64.f * range;
+        scale = fits ? kPlaces * 0.9999f / range : 0.f;
+        from = fits ? 2.f - lo * scale : 2.f;
     }
     auto part = [&](float v) -> uint32_t {
         if constexpr (kExact) return order_key(v) >> kIB;
-        const uint32_t q = 2u + (uint32_t)fmaxf((v - lo) * scale, 0.f);   // (of -inf too: a select, no branch)
-        return v == low ? kMaskedPart : q;
+        return (uint32_t)fmaxf(fmaf(v, scale, from), 1.f);   // (-inf, and its NaN with a scale of 0, in place 1)
     };
     uint32_t k[8], rest = 0;
 #pragma unroll
@@ -537,7 +541,8 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
     float off = 0.f;   // of a fp32 choice value
     if constexpr (!kExact) {
         if constexpr (kBias) off = err + 0x1p-22f * fmaxf(fabsf(lo), fabsf(hi));
-        // a place is off by less than three: the difference, its product, the cut
+        // a place is off by less than three: the sum, the scale, the cut (all of a row by
+        // their origin's rounding too, the same)
         const uint32_t apart = 4u + (uint32_t)fminf(2.f * off * scale, 0x1p30f);
         int far = 1, values = 1;   // neighbours are far enough apart; all taken are values
 #pragma unroll
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
 #pragma unroll
             for (int d = 1; d < 16; d *= 2) last = fmax(last, __shfl_xor(last, d, 64));
             // nothing else that was left out is above this
-            const double most = (double)lo + ((double)(rest >> kIB) + 2.0) * ((double)hi - (double)lo) / (double)(kPlaces * 0.9999f) + (double)off;
+            const double most = ((double)(rest >> kIB) + 4.0 - (double)from) / (double)scale + (double)off;
             const bool above = (rest >> kIB) <= kMaskedPart ? last > -__builtin_inf() : scale > 0.f && last > most;
             sure = sure || above;
         }
