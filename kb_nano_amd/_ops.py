@@ -1257,6 +1257,9 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     _mx_rows(what, "output", out, (T, N))
     if _overlaps(base, out) and (base.data_ptr() != out.data_ptr() or _ld(base) != _ld(out)):
         raise ValueError(f"{what}: output overlaps base (only exactly in place is allowed)")
+    for t, name in ((lora_b, "lora_b"), (adapter_ids, "adapter_ids"), (scaling, "scaling")):   # read as outputs are written
+        if t is not None and _overlaps(t, out):
+            raise ValueError(f"{what}: output overlaps {name}")
     if T == 0:
         return
     x = _near(x, LORA_FAR_ROWS)
@@ -1267,6 +1270,8 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), base.data_ptr(), _ld(base), lora_a.data_ptr(), lora_b.data_ptr(),
         adapter_ids.data_ptr(), adapter_ids.element_size(), scaling.data_ptr() if scaling is not None else None, T, N, K, L, R,
         out.data_ptr(), _ld(out), buf.data_ptr(), nbytes, _stream(x)), what)
+    if out.data_ptr() == base.data_ptr() and not out.is_inference():   # written through raw pointers: tell torch
+        torch.autograd.graph.increment_version(out)
 
 
 def fp8_block_requant(w_in: torch.Tensor, s_in: torch.Tensor | None, w_out: torch.Tensor, s_out: torch.Tensor,

@@ -44,6 +44,24 @@ def test_strips_and_splits(gpu_device, T, N, K, R):
             assert_lora(LoraAdd()(*args(d)), *args(d), f"{T}x{N}")
 
 
+def test_in_place_reads_its_input_first_and_tells_autograd(gpu_device):
+    """base may be x itself (the first launch has read it all); what is saved of base counts as changed."""
+    from kb_nano_amd import LoraAdd
+    d = make(70, 256, 256, 4, 16, BF16, 5, gpu_device)
+    want = LoraAdd()(d["x"], d["x"], d["a"], d["b"], d["ids"], d["s"])
+    x = d["x"].clone()
+    before = x._version
+    assert LoraAdd()(x, x, d["a"], d["b"], d["ids"], d["s"], inplace=True) is x
+    assert torch.equal(x, want) and x._version == before + 1
+    with torch.inference_mode():   # which keeps no versions
+        x = d["x"].clone()
+        assert torch.equal(LoraAdd()(x, x, d["a"], d["b"], d["ids"], d["s"], inplace=True), want)
+    # B, ids and scaling are read while the output is written
+    both = torch.zeros(4 * 256 * 16, dtype=BF16, device=gpu_device)
+    with pytest.raises(ValueError, match="overlaps lora_b"):
+        LoraAdd()(d["x"][:8], both[:2048].view(8, 256), d["a"], both.view(4, 256, 16), d["ids"][:8], d["s"], inplace=True)
+
+
 def test_zeros_keep_their_signs_in_rows_without_an_adapter(gpu_device):
     from kb_nano_amd import LoraAdd
     d = make(70, 64, 64, 2, 8, BF16, 1, gpu_device)
