@@ -16,6 +16,12 @@
 // adapters), or in order of appearance where adapters are more than lanes.  Nothing
 // has to be known of the ids on the host.
 //
+// Bound by rows, base and out for prompts: 4096 tokens of 8 adapters in runs, 7168 x
+// 16384, rank 32: 24 to 33 us (4.1 to 5.6 TB/s) and 33 us (3.5 TB/s: the products of a
+// strip are not all hidden behind the next one's loads).  A decode batch is bound by
+// the chain of two launches (ids, list, rows; ids, list, h, B): 32 tokens of 24
+// adapters, 8192 x 8192, rank 16, 6.3 + 5.2 us.
+//
 // h enters the second product as the sum of two bf16 numbers (16 bits of its
 // significand, 2^-16 of the value lost, far below the output's own rounding).
 #include "row_stream.h"
@@ -25,7 +31,7 @@
 namespace kbn {
 namespace {
 
-constexpr int kChunk = 64;        // tokens of one workgroup of the first launch
+constexpr int kChunk = 64;        // most tokens of one workgroup of the first launch
 constexpr int kRankChunk = 64;    // ranks of one workgroup of the first launch
 constexpr int kMaxSplits = 4;     // more gain nothing: the second launch reads them all back
 
@@ -171,22 +177,22 @@ __device__ __forceinline__ void shrink_tile(const LoraArgs& a, int t0, int place
     __syncthreads();   // smem is used again by the next chunk
 }
 
-// grid (splits, windows, slots x rank chunks)
-template <int kD, int kTR, int kMode>
+// grid (splits, windows, slots x rank chunks); chunks of kSize tokens
+template <int kD, int kTR, int kMode, int kSize>
 __global__ __launch_bounds__(64 * kStreamWaves) void lora_shrink_kernel(const LoraArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[Stream<4, kTR, 2, kD, kD>::kSmem];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[Stream<kSize / 16, kTR, 2, kD, kD>::kSmem];
     const int lane = threadIdx.x & 63;
     const int parts = (a.R + kRankChunk - 1) / kRankChunk;
     const int r0 = blockIdx.z % parts * kRankChunk;
-    Window<kMode, kChunk, false> win(a, blockIdx.y, lane);
+    Window<kMode, kSize, false> win(a, blockIdx.y, lane);
     for (int p = blockIdx.z / parts; win.seek(p); p += a.slots1) {
         if (threadIdx.x < 64) win.list(lane, smem);
         __syncthreads();
         const int n = win.n, list = smem[min(lane, n - 1)];
         __syncthreads();
         if (n <= 16) shrink_tile<kD, 1, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
-        else if (n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
-        else shrink_tile<kD, 4, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
+        else if (kSize == 32 || n <= 32) shrink_tile<kD, 2, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
+        else shrink_tile<kD, kSize / 16, kTR>(a, win.t0, 64 * words_of(kMode), n, list, win.adapter, r0, blockIdx.x, smem);
     }
 }
 
@@ -440,9 +446,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
 }
 
 // How a window finds its chunks, workgroups a window that share its chunks in each
-// launch, K splits of the first and 256-column blocks of a workgroup of the second.
+// launch, tokens of a chunk and K splits of the first and 256-column blocks of a
+// workgroup of the second.
 struct LoraPlan {
-    int mode, windows, slots1, slots2, splits, blocks;
+    int mode, windows, slots1, slots2, chunk, splits, blocks;
 };
 LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     LoraPlan p;
@@ -455,12 +462,16 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     // windows (prompts) mostly the full ones, and the rest waits its turn
     const int64_t adapters = std::min(L, size), last = p.windows > 2 ? std::min<int64_t>(adapters, 2) : adapters;
     const int64_t full1 = size / kChunk, full2 = size / kRows + 1;   // (and the tokens without an adapter)
-    p.slots1 = (int)std::max<int64_t>(1, full1 + last);
     p.slots2 = (int)std::max<int64_t>(1, full2 + last);
     const int64_t parts = (R + kRankChunk - 1) / kRankChunk, units = (K + kStreamK - 1) / kStreamK;
     const int64_t busy = p.windows * std::max<int64_t>(std::max<int64_t>(1, full1), p.windows > 2 ? 1 : adapters * 2 / 3) * parts;
     const int64_t few = std::max<int64_t>(1, 65536 / (std::min<int64_t>(T, kRows) * R * 4));   // that a chunk reads back
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cus + busy - 1) / busy, few, kMaxSplits, units / kStreamWaves}));
+    // where chunks of 64 leave half of the CUs idle, chunks of 32 (777 tokens of runs
+    // of 90, 4608 x 7168, rank 64: 23.8 us, with 64 26.1; 4096 tokens in runs of 700,
+    // 7168 x 16384, rank 32, which 64 fill the CUs with: 72.9 and 69.0)
+    p.chunk = p.mode == 2 && p.windows * full1 * parts * p.splits <= cus / 2 ? 32 : kChunk;
+    p.slots1 = (int)std::max<int64_t>(1, size / p.chunk + last);
     // of the second launch's workgroups a CU holds two, and one takes about 5 us
     // whatever its columns: one round of them
     const int64_t cols = (N + kColumns - 1) / kColumns;
@@ -469,13 +480,19 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t L, int64_t R, int64_t N) {
     return p;
 }
 
+template <int kD, int kMode, int kSize>
+void launch_shrink(const LoraArgs& a, const dim3& grid, hipStream_t st) {
+    const dim3 block(64 * kStreamWaves);
+    if (a.R <= 16) lora_shrink_kernel<kD, 1, kMode, kSize><<<grid, block, 0, st>>>(a);
+    else if (a.R <= 32) lora_shrink_kernel<kD, 2, kMode, kSize><<<grid, block, 0, st>>>(a);
+    else lora_shrink_kernel<kD, 4, kMode, kSize><<<grid, block, 0, st>>>(a);
+}
 template <int kD, int kMode>
 void launch_lora(const LoraArgs& a, const LoraPlan& p, bool vec, hipStream_t st) {
     const int parts = (a.R + kRankChunk - 1) / kRankChunk;
     const dim3 grid((unsigned)a.splits, (unsigned)p.windows, (unsigned)(a.slots1 * parts)), block(64 * kStreamWaves);
-    if (a.R <= 16) lora_shrink_kernel<kD, 1, kMode><<<grid, block, 0, st>>>(a);
-    else if (a.R <= 32) lora_shrink_kernel<kD, 2, kMode><<<grid, block, 0, st>>>(a);
-    else lora_shrink_kernel<kD, 4, kMode><<<grid, block, 0, st>>>(a);
+    if constexpr (kMode == 2) p.chunk == 32 ? launch_shrink<kD, kMode, 32>(a, grid, st) : launch_shrink<kD, kMode, kChunk>(a, grid, st);
+    else launch_shrink<kD, kMode, kChunk>(a, grid, st);
     const int cols = kColumns * a.blocks;
     const dim3 egrid((unsigned)((a.N + cols - 1) / cols), (unsigned)p.windows, (unsigned)a.slots2);
     if (!vec) lora_expand_kernel<kD, 0, kMode, false><<<egrid, block, 0, st>>>(a);
