@@ -13,7 +13,13 @@
 // wavefronts has one token; chunk c of its row is the 512 elements c*512 ..
 // c*512+511 (eight a lane), wavefront w owns chunks w, w + kW, ...  Sums of
 // squares are fp32: over a lane's elements in order, by butterfly over the
-// wavefront, over the wavefronts in order.
+// wavefront, over the wavefronts in order.  A wavefront a chunk up to 4096 columns
+// (4096 x 1024 9.2 us, 12.1 before that and the packing of values in pairs).
+//
+// 4096 x 7168 bf16 with a post norm, a full gate and codes out: 47 us, 264 MB, 5.6
+// TB/s (a copy of 1 GiB: 5.1); 777 x 8192 fp16, a gate for each channel, 14.7 us (3 TB/s:
+// with one round of workgroups the loads, sums and stores of the rows follow each
+// other); one token of 7168 3.9 us, of which 2.4 are a launch.
 #include "norm_common.h"
 
 namespace kbn {

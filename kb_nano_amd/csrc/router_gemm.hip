@@ -1,7 +1,10 @@
 // The router's product: logits[t, e] = sum_h x[t, h] w[e, h] in fp32.
 //
 // Few experts (8 to some hundred) and a long sum: what bounds it is reading w
-// (few tokens) or x (many).  The wavefronts of a workgroup share one tile of
+// (few tokens: 1 x 128 x 4096 2.5 us, of which 2.4 are a launch) or x and w by CUs
+// that share neither (many: 4096 x 256 x 7168 bf16 24.1 us, 470 MB through 256 CUs
+// at 76 B/ns each, 0.62 PFLOP/s; memory alone 13).  Weights in fp32 are bound by the
+// instructions that take them apart (2051 x 256 x 7168 53 us with bf16 rows).  The wavefronts of a workgroup share one tile of
 // logits and split its K, unit by unit; each streams whole 128-byte lines of its
 // units through a private LDS ring by direct loads, so there is no barrier until
 // their sums meet in LDS, in wavefront order.  (Fragments loaded straight into
@@ -165,7 +168,10 @@ struct GatePlan {
 // from 4 to 4096 with (256, 7168), (128, 4096) and (16, 2048), each type: 1.3%
 // above the best of up to 30 choices on average, 14% at most (512 x 256 x 7168:
 // 12.0 us with 32 experts a tile and four splits, 14.7 with 64 and three; 2048
-// tokens 18.8 with 32 and none, 27.4 with 16).
+// tokens 18.8 with 32 and none, 27.4 with 16).  Splits up to two rounds of the CUs,
+// four where the weights are taken apart and a round is long (2051 x 256 x 7168, two
+// splits and none: fp16 with fp32 weights 76 and 90 us, bf16 with those 53 and 58,
+// fp32 99 and 107; bf16 29 and 24).
 GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
     if (T <= (xd == kG32 ? kRowTokens32 : kRowTokens)) return {0, 0, 1};
     const int64_t units = (H + kStreamK - 1) / kStreamK, cus = cu_count();
@@ -178,7 +184,7 @@ GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
         if (te > 1 && 8 * te >= E) break;
         const int64_t tiles = (T + 16 * tm - 1) / (16 * tm) * ((E + 16 * te - 1) / (16 * te));
         for (const int s : {1, 2, 3, 4, 8, 16, 32}) {
-            if (s > 1 && (s > units / kStreamWaves || tiles * s > 2 * cus)) break;
+            if (s > 1 && (s > units / kStreamWaves || tiles * s > (wd == kG32 ? 4 : 2) * cus)) break;
             const double rate = 80.0 + 20.0 * std::max<double>(0.0, 1.0 - (double)(tiles * s) / cus);
             double ns = (double)((tiles * s + cus - 1) / cus) * (16 * tm * bx + 16 * te * bw) * H / s / rate * slow + wide;
             if (s > 1) ns += 2400.0 + 200.0 * ((s + 7) / 8) + 60.0 * s + 8.0 * s * T * E / 4000.0;

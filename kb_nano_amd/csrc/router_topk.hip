@@ -16,7 +16,12 @@
 // of 256 come out in the other order once in some 10^4 tokens: whatever a choice
 // depends on is computed in 64 bits, and so are the few weights.
 //
-// One wavefront a token, expert e = lane * V + j in register j, so the lowest
+// Reads and writes are small (16384 x 256 fp32 logits, top 8 with groups and a bias:
+// 18 MB, 4 us at the rate of a copy): the instructions bound it, some 1100 for four
+// tokens, and for few tokens their latency (that case 18 us, 1 TB/s; one token 5.1;
+// 777 x 128, no groups, 3.9).
+//
+// The general path: one wavefront a token, expert e = lane * V + j in register j, so the lowest
 // index of equal keys is the first lane's first register.  Keys are the values'
 // bits mapped to unsigned integers of the same order, 0 for taken or absent.
 #include "kbn_common.h"
