@@ -534,7 +534,8 @@ int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* 
  * The router's product (no kb_nano counterpart): logits[t, e] = sum_h x[t, h] w[e, h].
  *   x      [T, H], row stride ld_x, w [E, H], row stride ld_w; x_dtype and
  *          w_dtype 0 bf16, 1 fp16, 2 fp32, w of x's type or fp32; rows 16-byte
- *          aligned, strides below 2^23 elements; H % 8 == 0
+ *          aligned, strides below 2^23 elements; H % 8 == 0,
+ *          H <= 2^22, T < 2^24, E <= 65536
  *   out    fp32 [T, E], row stride ld_out
  * fp32 sums of exact products (fp32 operands as three bf16 numbers, products
  * below 2^-24 of the largest left out), in one order for a shape and device.
@@ -576,7 +577,7 @@ int kbn_moe_router_topk(const void* logits, int dtype, int64_t ld, const float* 
  * x, r, r_out and n_out [T, H] of one type (dtype 0 bf16, 1 fp16, 2 fp32), H % 8
  * == 0, rows 16-byte aligned; w and post (or NULL) [H] of that type.  gate (or
  * NULL) has element (t, h) at gate[t * gate_row + h * gate_col], gate_col 0 or 1.
- * r_out may be r.  n leaves as rows (n_out) or as FP8 codes and scales (q_fp8
+ * r_out may be r (no other overlap).  n leaves as rows (n_out) or as FP8 codes and scales (q_fp8
  * [T, H] and scale, as kbn_rmsnorm_fp8_quant quantizes), or both; the other NULL.
  */
 int kbn_gated_add_rmsnorm(const void* x, int dtype, int64_t ld_x, const void* r, int64_t ld_r, const void* w,
@@ -592,7 +593,9 @@ int kbn_gated_add_rmsnorm(const void* x, int dtype, int64_t ld_x, const void* r,
  *   x [T, K], base and out [T, N] (dtype 0 bf16, 1 fp16), lora_a [L, R, K] and
  *   lora_b [L, N, R] contiguous, of that type; ids int32 or int64 (id_bytes 4, 8)
  *   [T]; scaling fp32 [L] or NULL (1).  K % 8 == 0, R % 8 == 0 and at most 256,
- *   adapters of smaller rank padded with zeros.  out may be base.
+ *   adapters of smaller rank padded with zeros.  x and adapters 16-byte aligned,
+ *   x's row stride below 2^22 elements; T <= 65535 * 64, an adapter's B below 2 GiB.
+ *   out may be base, and base x; nothing else that is read may overlap out.
  *   workspace: kbn_lora_add_workspace_bytes(T, K, L, R) bytes (-1 for sizes that
  *   are refused), for this call alone while it runs.
  */
