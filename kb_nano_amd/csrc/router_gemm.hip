@@ -3,8 +3,9 @@
 // Few experts (8 to some hundred) and a long sum: what bounds it is reading w
 // (few tokens: 1 x 128 x 4096 2.5 us, of which 2.4 are a launch) or x and w by CUs
 // that share neither (many: 4096 x 256 x 7168 bf16 24.1 us, 470 MB through 256 CUs
-// at 76 B/ns each, 0.62 PFLOP/s; memory alone 13).  Weights in fp32 are bound by the
-// instructions that take them apart (2051 x 256 x 7168 53 us with bf16 rows).  The wavefronts of a workgroup share one tile of
+// at 76 B/ns each, 0.62 PFLOP/s; memory alone 13), with weights in fp32 the
+// matrix instructions and the barriers of a stage (2051 x 256 x 7168 with bf16 rows
+// 34 us, three products each: 0.66 PFLOP/s).  The wavefronts of a workgroup share one tile of
 // logits and split its K, unit by unit; each streams whole 128-byte lines of its
 // units through a private LDS ring by direct loads, so there is no barrier until
 // their sums meet in LDS, in wavefront order.  (Fragments loaded straight into
@@ -67,6 +68,112 @@ __global__ __launch_bounds__(64 * kStreamWaves) void router_gemm_tile_kernel(con
                 if (t + i < nt) out[(t0 + t + i) * ld + e0 + e] = v[i];
         }
     }
+}
+
+// Many tokens and weights in fp32: 128 tokens x 128 experts a workgroup, whose
+// wavefronts (64 x 32 each) meet both operands' pieces in LDS.  Each value is taken
+// apart once a workgroup, on its way there: a thread has eight values of a row of
+// each operand a stage (32 K) and holds those of the next kAhead stages (one or three:
+// the same times within 3%).  (In the tiles above each wavefront takes its
+// own K's values apart: 2051 x 256 x 7168 with fp32 weights 58 us, here 34.)
+constexpr int kWideT = 128, kWideE = 128, kWideK = 32, kWideThreads = 512, kAhead = 2;
+
+template <int kX>
+__global__ __launch_bounds__(kWideThreads) void router_gemm_wide_kernel(const GateArgs a) {
+    constexpr int PX = kX == kG32 ? 3 : kX == kG16f ? 2 : 1, PW = 3;
+    constexpr int bx = bytes_of<kX>();
+    __shared__ __attribute__((aligned(16))) u32x4 lx[2][PX][kWideT * 4];   // rows of four 16-byte chunks
+    __shared__ __attribute__((aligned(16))) u32x4 lw[2][PW][kWideE * 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int te = (a.E + kWideE - 1) / kWideE;
+    const int split = blockIdx.x % a.splits, tile_e = blockIdx.x / a.splits % te, tile_t = blockIdx.x / a.splits / te;
+    const int t0 = tile_t * kWideT, e0 = tile_e * kWideE;
+    const int nt = min(kWideT, a.T - t0), ne = min(kWideE, a.E - e0);
+    // a wavefront's 16 rows of each operand
+    const int row = tid >> 2, oct = tid & 3, row0 = 16 * wave;
+    const __amdgpu_buffer_rsrc_t xr = rsrc(static_cast<const uint8_t*>(a.x) + (int64_t)(t0 + row0) * a.ld_x * bx,
+                                           nt > row0 ? (int)(((int64_t)(min(16, nt - row0) - 1) * a.ld_x + a.H) * bx) : 0);
+    const __amdgpu_buffer_rsrc_t wr = rsrc(static_cast<const uint8_t*>(a.w) + (int64_t)(e0 + row0) * a.ld_w * 4,
+                                           ne > row0 ? (int)(((int64_t)(min(16, ne - row0) - 1) * a.ld_w + a.H) * 4) : 0);
+    const int units = (a.H + kWideK - 1) / kWideK;
+    const int from = (int)((int64_t)units * split / a.splits), end = (int)((int64_t)units * (split + 1) / a.splits);
+    const int xo = row < nt ? (row - row0) * (int)a.ld_x * bx : kOob, wo = row < ne ? (row - row0) * (int)a.ld_w * 4 : kOob;
+    const int put = 4 * row + (oct ^ (row >> 1 & 3));   // chunk c of row r lies in slot c ^ (r / 2) % 4
+    Raw8<kX> xs[kAhead];
+    Raw8<kG32> ws[kAhead];
+    // (a stage past the split's end and values past the row's read zeros)
+    auto ask = [&](int u, Raw8<kX>& x, Raw8<kG32>& w) __attribute__((always_inline)) {
+        const int k = u * kWideK + 8 * oct;
+        const bool in = u < end && k < a.H;
+        x = load_raw8<kX>(xr, in && xo != kOob ? xo + k * bx : kOob);
+        w = load_raw8<kG32>(wr, in && wo != kOob ? wo + k * 4 : kOob);
+    };
+    auto give = [&](int buf, const Raw8<kX>& x, const Raw8<kG32>& w) __attribute__((always_inline)) {
+        const Pieces<PX> px = pieces_of<kX, PX>(x);
+        const Pieces<PW> pw = pieces_of<kG32, PW>(w);
+#pragma unroll
+        for (int i = 0; i < PX; ++i) lx[buf][i][put] = px.p[i];
+#pragma unroll
+        for (int i = 0; i < PW; ++i) lw[buf][i][put] = pw.p[i];
+    };
+    f32x4 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int tw = 64 * (wave & 1), ew = 32 * (wave >> 1);
+    const int fr = lane & 15, at = 4 * fr + ((lane >> 4) ^ (fr >> 1 & 3));   // (16 rows on, the same slot)
+    auto products = [&](int buf) __attribute__((always_inline)) {
+        u32x4 x[PX][4], w[PW][2];
+#pragma unroll
+        for (int m = 0; m < PX; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[m][i] = lx[buf][m][4 * (tw + 16 * i) + at];
+#pragma unroll
+        for (int n = 0; n < PW; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w[n][j] = lw[buf][n][4 * (ew + 16 * j) + at];
+#pragma unroll
+        for (int sum = 2; sum >= 0; --sum) {   // the smallest products first
+#pragma unroll
+            for (int m = 0; m < PX; ++m) {
+                const int n = sum - m;
+                if (n < 0 || n >= PW) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = mma<false>(x[m][i], w[n][j], acc[i][j]);
+            }
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) ask(from + d, xs[d], ws[d]);
+    give(0, xs[0], ws[0]);
+    ask(from + kAhead, xs[0], ws[0]);
+    __syncthreads();
+    // stage u lies in buffer (u - from) % 2; its successor is given while it is multiplied
+    for (int u = from; u < end;) {
+#pragma unroll
+        for (int d = 1; d <= 2 * kAhead; ++d) {
+            if (u >= end) break;
+            give(d & 1, xs[d % kAhead], ws[d % kAhead]);
+            ask(u + 1 + kAhead, xs[d % kAhead], ws[d % kAhead]);
+            products((d - 1) & 1);
+            __syncthreads();
+            ++u;
+        }
+    }
+    float* const out = a.splits > 1 ? a.sums + (int64_t)split * a.T * a.E : a.out;
+    const int64_t ld = a.splits > 1 ? a.E : a.ld_o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = tw + 16 * i + 4 * (lane >> 4) + k, e = ew + 16 * j + fr;
+                if (t < nt && e < ne) out[(t0 + t) * ld + e0 + e] = acc[i][j][k];
+            }
 }
 
 // out = the sums of the splits, in order; eight of them asked for at a time
@@ -156,42 +263,59 @@ __global__ __launch_bounds__(64 * kRowWaves) void router_gemm_rows_kernel(const 
 // 4096 3.7, 5.3, 5.4, 6.5; fp32 rows 5.5, 9.7, 11.3, 11.7 and 4.0, 6.0, 6.8, 8.2).
 constexpr int kRowTokens = 16, kRowTokens32 = 12;
 
-// Tiles of 16 tm x 16 te logits, K in `splits` parts; tm = 0: the rows kernel.
+// Tiles of 16 tm x 16 te logits, K in `splits` parts; tm = 0: the rows kernel, 8: the wide one.
 struct GatePlan {
     int tm, te, splits;
 };
 
+// The second launch of a split product, in ns.
+double sum_price(int64_t T, int64_t E, int s) { return s > 1 ? 2400.0 + 200.0 * ((s + 7) / 8) + 60.0 * s + 8.0 * s * T * E / 4000.0 : 0.0; }
+
 // The cheapest of the tile widths and splits by what one takes in ns: the bytes
 // of a CU's workgroups, of which a lone CU takes 100 a ns and each of 256 at
-// work 80 (half where fp32 values are taken apart), a price on wide tiles (one
-// workgroup a CU), and with splits the second launch.  Fitted to 13 token counts
-// from 4 to 4096 with (256, 7168), (128, 4096) and (16, 2048), each type: 1.3%
-// above the best of up to 30 choices on average, 14% at most (512 x 256 x 7168:
-// 12.0 us with 32 experts a tile and four splits, 14.7 with 64 and three; 2048
-// tokens 18.8 with 32 and none, 27.4 with 16).  Splits up to two rounds of the CUs,
-// four where the weights are taken apart and a round is long (2051 x 256 x 7168, two
-// splits and none: fp16 with fp32 weights 76 and 90 us, bf16 with those 53 and 58,
-// fp32 99 and 107; bf16 29 and 24).
+// work 80, a price on wide tiles (one workgroup a CU), and with splits the second
+// launch.  Fitted to 13 token counts from 4 to 4096 with (256, 7168), (128, 4096) and
+// (16, 2048): 1.3% above the best of up to 30 choices on average, 14% at most (512 x
+// 256 x 7168: 12.0 us with 32 experts a tile and four splits, 14.7 with 64 and three;
+// 2048 tokens 18.8 with 32 and none, 27.4 with 16).
+// With fp32 weights the bytes cost more by the work of taking the values apart, by
+// the rows' type and the tile's width; the wide kernel goes by what a stage takes a
+// lone workgroup of a CU and each two (of fp32 rows LDS holds one).  Fitted to 10
+// token counts from 61 to 4096 with those and three more sizes: 1.2% on average, 15%
+// at most (2051 x 256 x 7168, wide and not: bf16 rows 34 and 53 us, fp16 44 and 76,
+// fp32 51 and 99; 777 x 128 x 4096 bf16 15 and 12).
 GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
     if (T <= (xd == kG32 ? kRowTokens32 : kRowTokens)) return {0, 0, 1};
     const int64_t units = (H + kStreamK - 1) / kStreamK, cus = cu_count();
-    const int tm = xd == kG32 ? 2 : 4, most = wd == kG32 ? 2 : 4;
-    const double bx = xd == kG32 ? 4 : 2, bw = wd == kG32 ? 4 : 2, slow = wd == kG32 ? 2.0 : 1.0;
+    const bool apart = wd == kG32;
+    const int tm = xd == kG32 ? 2 : 4, most = apart ? 2 : 4;
+    const double bx = xd == kG32 ? 4 : 2, bw = apart ? 4 : 2;
+    const double slow[3][2] = {{1.13, 1.44}, {1.97, 2.29}, {1.6, 1.81}};   // bf16, fp16, fp32 rows; 16, 32 experts
     GatePlan best{tm, 1, 1};
     double least = 1e30;
-    double wide = 0.0;
-    for (int te = 1; te <= most; te *= 2, wide += 900.0) {
+    for (int te = 1, i = 0; te <= most; te *= 2, ++i) {
         if (te > 1 && 8 * te >= E) break;
         const int64_t tiles = (T + 16 * tm - 1) / (16 * tm) * ((E + 16 * te - 1) / (16 * te));
         for (const int s : {1, 2, 3, 4, 8, 16, 32}) {
-            if (s > 1 && (s > units / kStreamWaves || tiles * s > (wd == kG32 ? 4 : 2) * cus)) break;
+            if (s > 1 && (s > units / kStreamWaves || tiles * s > 2 * cus)) break;
             const double rate = 80.0 + 20.0 * std::max<double>(0.0, 1.0 - (double)(tiles * s) / cus);
-            double ns = (double)((tiles * s + cus - 1) / cus) * (16 * tm * bx + 16 * te * bw) * H / s / rate * slow + wide;
-            if (s > 1) ns += 2400.0 + 200.0 * ((s + 7) / 8) + 60.0 * s + 8.0 * s * T * E / 4000.0;
+            const double ns = (double)((tiles * s + cus - 1) / cus) * (16 * tm * bx + 16 * te * bw) * H / s / rate *
+                    (apart ? slow[xd][i] : 1.0) + (apart ? 3900.0 : 900.0 * i) + sum_price(T, E, s);
             if (ns < least) {
                 least = ns;
                 best = {tm, te, s};
             }
+        }
+    }
+    if (!apart) return best;
+    const double start[] = {1000.0, 2900.0, 3900.0}, one[] = {835.0, 1065.0, 1150.0}, two[] = {1120.0, 1550.0, 2300.0};
+    const int64_t tiles = (T + kWideT - 1) / kWideT * ((E + kWideE - 1) / kWideE), stages = (H + kWideK - 1) / kWideK;
+    for (int s = 1; s <= 32 && 4 * s <= stages && (s == 1 || tiles * s <= 2 * cus); ++s) {
+        const int64_t n = (tiles * s + cus - 1) / cus;
+        const double ns = start[xd] + (double)stages / s * ((double)(n / 2) * two[xd] + (double)(n % 2) * one[xd]) + sum_price(T, E, s);
+        if (ns < least) {
+            least = ns;
+            best = {8, 8, s};
         }
     }
     return best;
@@ -211,7 +335,9 @@ void launch(GateArgs a, const GatePlan& p, hipStream_t st) {
     constexpr int kTM = kX == kG32 ? 2 : 4;
     const int64_t tiles = (int64_t)((a.T + 16 * p.tm - 1) / (16 * p.tm)) * ((a.E + 16 * p.te - 1) / (16 * p.te));
     const dim3 grid((unsigned)(tiles * p.splits)), block(64 * kStreamWaves);
-    if (p.te == 1) router_gemm_tile_kernel<kTM, 1, 2, kX, kW><<<grid, block, 0, st>>>(a);
+    if (p.tm == 8) {
+        if constexpr (kW == kG32) router_gemm_wide_kernel<kX><<<grid, dim3(kWideThreads), 0, st>>>(a);
+    } else if (p.te == 1) router_gemm_tile_kernel<kTM, 1, 2, kX, kW><<<grid, block, 0, st>>>(a);
     else if (p.te == 2) router_gemm_tile_kernel<kTM, 2, 2, kX, kW><<<grid, block, 0, st>>>(a);
     else if constexpr (kW != kG32) router_gemm_tile_kernel<kTM, 4, 2, kX, kW><<<grid, block, 0, st>>>(a);
     if (p.splits > 1) {

@@ -98,6 +98,33 @@ def test_every_tile_and_split(gpu_device, T, E, x_dtype, w_dtype):
     assert_gate(MoeRouterGemm()(x, w), x, w, f"{T}x{E}")
 
 
+@pytest.mark.parametrize("T,E,H,x_dtype", [(1101, 250, 7176, F32), (1101, 250, 7176, BF16), (1101, 250, 7176, F16), (2051, 129, 7168, F32),
+                                           (2049, 256, 7168, BF16), (4096, 320, 2056, F16), (20000, 256, 520, F32)])
+def test_many_tokens_and_weights_in_fp32(gpu_device, T, E, H, x_dtype):
+    """Tiles of 128 x 128 that end inside tokens, experts and K; with and without splits; rows with gaps; NaN behind the rows."""
+    from kb_nano_amd import MoeRouterGemm
+    print(f"router wide {T} x {E} x {H} {x_dtype}", flush=True)
+    gap = 24
+    x, w = randn((T + 1, H + gap), x_dtype, T, gpu_device), randn((E + 1, H + gap), F32, E, gpu_device, 0.02)
+    x[T], w[E], x[:, H:], w[:, H:] = float("nan"), float("nan"), float("nan"), float("nan")
+    x, w = x[:T, :H], w[:E, :H]
+    out = MoeRouterGemm()(x, w)
+    assert_gate(out, x, w, f"{T}x{E}x{H}")
+    assert all(torch.equal(out, MoeRouterGemm()(x, w)) for _ in range(3))
+    small = MoeRouterGemm()(x[:61], w)   # other tiles: the same sums in another order
+    assert_gate(small, x[:61], w, "first rows")
+
+
+def test_weights_far_apart(gpu_device):
+    """Weight rows further apart than 128 of them fit into 32-bit offsets."""
+    from kb_nano_amd import MoeRouterGemm
+    H, ld = 7168, (1 << 22) + 8
+    x, buf = randn((2051, H), BF16, 1, gpu_device), torch.empty(129 * ld, dtype=F32, device=gpu_device)
+    w = buf.view(129, ld)[:, :H]
+    w.copy_(randn((129, H), F32, 2, gpu_device, 0.02))
+    assert_gate(MoeRouterGemm()(x, w), x, w, "far")
+
+
 def test_product_does_not_depend_on_the_run(gpu_device):
     """Splits meet in one order: the same bits on every run, beside other work."""
     from kb_nano_amd import MoeRouterGemm
