@@ -221,7 +221,6 @@ constexpr int kStrip = 64;                          // output columns of a wavef
 constexpr int kColumns = kStreamWaves * kStrip;     // of a workgroup's block
 constexpr int kRows = 32;                           // tokens of one workgroup of the second launch
 constexpr int kMaxRank = 256;
-constexpr int kNt = 2;                              // buffer cache policy: non-temporal
 
 // A wavefront's LDS writes come before its reads that follow.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -350,15 +349,16 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
 #pragma unroll
                 for (int k = 0; k < kKS; ++k) load_b(n0, k, t.w[k]);
             }
-            // (past N a row's columns are the next row's: the last strip masks them;
-            // nothing reads base again: 2048 tokens of 32 adapters 61.9 us without the hint, 56.7 with)
+            // (past N a row's columns are the next row's: the last strip masks them.  No
+            // non-temporal hints: base is mostly just written, x read by other products too;
+            // 2048 tokens of 8 adapters, 10240 x 8192, warm 50.2 us, base with the hint 55.1)
             if constexpr (kVec) {
                 const bool in = n0 + 4 * row < a.N;
 #pragma unroll
                 for (int m = 0; m < kTM; ++m)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        t.was[m][i] = __builtin_amdgcn_raw_buffer_load_b64(bi, in ? bo_at[m][i] : kOob, n0 * 2, kNt);
+                        t.was[m][i] = __builtin_amdgcn_raw_buffer_load_b64(bi, in ? bo_at[m][i] : kOob, n0 * 2, 0);
             }
         };
         auto finish = [&](int n0, Strip& t) __attribute__((always_inline)) {
