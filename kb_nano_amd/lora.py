@@ -22,7 +22,8 @@ class LoraAdd(nn.Module):
     adapter_ids[t]``, ``base[t]`` for ids outside [0, L) (requests without an
     adapter, padding).  ``x [..., K]`` and ``base [..., N]`` bf16 or fp16, adapters
     of the same type, ids int32 or int64 ``[...]``, scaling fp32 [L].  fp32 sums, one
-    rounding at the end.  Returns a new tensor, or with ``inplace`` base itself."""
+    rounding at the end.  Returns a new tensor, or with ``inplace`` base itself (which
+    may be x, and must not overlap lora_b, ids or scaling)."""
 
     def forward(self, x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter_ids: torch.Tensor, scaling: torch.Tensor | None = None, inplace: bool = False) -> torch.Tensor:
