@@ -328,6 +328,10 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
     // upper parts of keys: 0 no expert; -inf; values
     constexpr uint32_t kMaskedPart = kExact ? Masked<uint32_t>::key >> kIB : 1u;
     constexpr float kPlaces = kIB == 9 ? 8388604.f : 16777212.f;   // 2^(32 - kIB), 2^24 at most, less four
+    // The row's smallest value is meant to lie here; the rounding of the origin below (terms
+    // up to 64 kPlaces < 2^30: two of 32 at most) moves the whole row by up to 64 places,
+    // so no value reaches the place of -inf, and none the end: 0.0001 kPlaces > 838 are left.
+    constexpr float kFirstPlace = 68.f;
     __shared__ uint64_t scratch[kWaves][16 * V];               // quads of four tokens, or one token's choice
     const int lane = threadIdx.x & 63, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -484,7 +488,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
             for (int i = 0; i < 4; ++i) f[4 * jj + i] = in ? f[4 * jj + i] : low;
         }
     }
-    float lo = __builtin_inff(), hi = low, scale = 0.f, from = 2.f;
+    float lo = __builtin_inff(), hi = low, scale = 0.f, from = 2.f;   // (places 2 and up; 1: -inf)
     if constexpr (!kExact) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(64 * kWaves) void router_topk_rows_kernel(const Top
         const float range = hi - lo;
         const bool fits = range > 0x1p-100f && range < __builtin_inff() && fmaxf(fabsf(lo), fabsf(hi)) < 64.f * range;
         scale = fits ? kPlaces * 0.9999f / range : 0.f;
-        from = fits ? 2.f - lo * scale : 2.f;
+        from = fits ? kFirstPlace - lo * scale : 2.f;
     }
     auto part = [&](float v) -> uint32_t {
         if constexpr (kExact) return order_key(v) >> kIB;
