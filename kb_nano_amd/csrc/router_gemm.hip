@@ -17,7 +17,9 @@
 // fp32 operands go through the 16-bit matrix instruction as well: a float is
 // the exact sum of three bf16 numbers (8 + 8 + 8 bits of its significand, cut
 // off by clearing low bits), and the products of pieces down to 2^-16 of the
-// largest are added, as good as fp32 products.
+// largest are added, as good as fp32 products.  Products of leading pieces have a
+// sum of their own, which alone counts where it is not finite (an infinity's lower
+// pieces are no numbers): 1 to 3% of the time, and half of the error.
 #include "row_stream.h"
 
 #include <algorithm>
@@ -73,14 +75,16 @@ __global__ __launch_bounds__(64 * kStreamWaves) void router_gemm_tile_kernel(con
 // Many tokens and weights in fp32: 128 tokens x 128 experts a workgroup, whose
 // wavefronts (64 x 32 each) meet both operands' pieces in LDS.  Each value is taken
 // apart once a workgroup, on its way there: a thread has eight values of a row of
-// each operand a stage (32 K) and holds those of the next kAhead stages (one or three:
-// the same times within 3%).  (In the tiles above each wavefront takes its
+// each operand a stage (32 K) and holds those of the next kAhead stages (one, two or three:
+// the same times within 3%; of fp16 rows one, with which two workgroups fit a CU's
+// registers).  (In the tiles above each wavefront takes its
 // own K's values apart: 2051 x 256 x 7168 with fp32 weights 58 us, here 34.)
-constexpr int kWideT = 128, kWideE = 128, kWideK = 32, kWideThreads = 512, kAhead = 2;
+constexpr int kWideT = 128, kWideE = 128, kWideK = 32, kWideThreads = 512;
 
 template <int kX>
-__global__ __launch_bounds__(kWideThreads) void router_gemm_wide_kernel(const GateArgs a) {
+__global__ __launch_bounds__(kWideThreads, kX == kG32 ? 1 : 4) void router_gemm_wide_kernel(const GateArgs a) {
     constexpr int PX = kX == kG32 ? 3 : kX == kG16f ? 2 : 1, PW = 3;
+    constexpr int kAhead = kX == kG16f ? 1 : 2;
     constexpr int bx = bytes_of<kX>();
     __shared__ __attribute__((aligned(16))) u32x4 lx[2][PX][kWideT * 4];   // rows of four 16-byte chunks
     __shared__ __attribute__((aligned(16))) u32x4 lw[2][PW][kWideE * 4];
@@ -116,33 +120,36 @@ __global__ __launch_bounds__(kWideThreads) void router_gemm_wide_kernel(const Ga
 #pragma unroll
         for (int i = 0; i < PW; ++i) lw[buf][i][put] = pw.p[i];
     };
-    f32x4 acc[4][2];
+    f32x4 acc[2][4][2];   // products of leading pieces, of others
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[c][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int tw = 64 * (wave & 1), ew = 32 * (wave >> 1);
     const int fr = lane & 15, at = 4 * fr + ((lane >> 4) ^ (fr >> 1 & 3));   // (16 rows on, the same slot)
     auto products = [&](int buf) __attribute__((always_inline)) {
-        u32x4 x[PX][4], w[PW][2];
-#pragma unroll
-        for (int m = 0; m < PX; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[m][i] = lx[buf][m][4 * (tw + 16 * i) + at];
+        u32x4 w[PW][2];
 #pragma unroll
         for (int n = 0; n < PW; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) w[n][j] = lw[buf][n][4 * (ew + 16 * j) + at];
 #pragma unroll
-        for (int sum = 2; sum >= 0; --sum) {   // the smallest products first
+        for (int m = PX - 1; m >= 0; --m) {   // the smallest products first
+            u32x4 x[4];
 #pragma unroll
-            for (int m = 0; m < PX; ++m) {
-                const int n = sum - m;
-                if (n < 0 || n >= PW) continue;
+            for (int i = 0; i < 4; ++i) x[i] = lx[buf][m][4 * (tw + 16 * i) + at];
+#pragma unroll
+            for (int n = 2 - m; n >= 0; --n) {
+                if (n >= PW) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = mma<false>(x[m][i], w[n][j], acc[i][j]);
+                    for (int j = 0; j < 2; ++j) {
+                        f32x4& to = acc[m + n > 0 ? 1 : 0][i][j];
+                        to = mma<false>(x[i], w[n][j], to);
+                    }
             }
         }
     };
@@ -168,12 +175,14 @@ __global__ __launch_bounds__(kWideThreads) void router_gemm_wide_kernel(const Ga
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
+            const f32x4 v = joined(acc[0][i][j], acc[1][i][j]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int t = tw + 16 * i + 4 * (lane >> 4) + k, e = ew + 16 * j + fr;
-                if (t < nt && e < ne) out[(t0 + t) * ld + e0 + e] = acc[i][j][k];
+                if (t < nt && e < ne) out[(t0 + t) * ld + e0 + e] = v[k];
             }
+        }
 }
 
 // out = the sums of the splits, in order; eight of them asked for at a time

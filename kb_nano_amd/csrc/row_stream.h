@@ -72,13 +72,26 @@ __device__ __forceinline__ Pieces<kP> pieces_of(const Raw8<kD>& r) {
             for (int i = 0; i < 4; ++i) {
                 const uint32_t a = __float_as_uint(f[2 * i]), b = __float_as_uint(f[2 * i + 1]);
                 o.p[k][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);   // the upper halves
-                if (k + 1 < kP) {   // (an infinity leaves a NaN here: its row has no finite result either way)
+                if (k + 1 < kP) {   // (an infinity leaves a NaN here: see joined)
                     f[2 * i] -= __uint_as_float(a & 0xFFFF0000u);
                     f[2 * i + 1] -= __uint_as_float(b & 0xFFFF0000u);
                 }
             }
     }
     return o;
+}
+
+// A sum of products of leading pieces and the sum of all others, which counts only where
+// the first is finite: leading pieces are infinite where the values are, and give the
+// formula's infinities and NaN, while lower pieces are 0 or NaN beside them.
+__device__ __forceinline__ f32x4 joined(const f32x4& lead, const f32x4& rest) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool finite = (__float_as_uint(lead[i]) & 0x7F800000u) != 0x7F800000u;
+        v[i] = lead[i] + (finite ? rest[i] : 0.f);
+    }
+    return v;
 }
 
 template <bool kHalf>
@@ -181,11 +194,14 @@ struct Stream {
                 });
             }
         };
-        f32x4 acc[kTM][kTE];
+        constexpr int kAcc = PX + PW > 2 ? 2 : 1;   // products of leading pieces, of others
+        f32x4 acc[kAcc][kTM][kTE];
 #pragma unroll
-        for (int i = 0; i < kTM; ++i)
+        for (int c = 0; c < kAcc; ++c)
 #pragma unroll
-            for (int j = 0; j < kTE; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < kTM; ++i)
+#pragma unroll
+                for (int j = 0; j < kTE; ++j) acc[c][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         const int row = lane & 15, q = lane >> 4;
         for (int d = 0; d < kDepth; ++d) issue(d, from + wave + d * kStreamWaves);
         int buf = 0;
@@ -222,7 +238,10 @@ struct Stream {
 #pragma unroll
                         for (int i = 0; i < kTM; ++i)
 #pragma unroll
-                            for (int j = 0; j < kTE; ++j) acc[i][j] = mma<kHalf>(px[i].p[m], pw[j].p[n], acc[i][j]);
+                            for (int j = 0; j < kTE; ++j) {
+                                f32x4& to = acc[sum > 0 ? 1 : 0][i][j];
+                                to = mma<kHalf>(px[i].p[m], pw[j].p[n], to);
+                            }
                     }
                 }
             }
@@ -233,7 +252,11 @@ struct Stream {
 #pragma unroll
         for (int i = 0; i < kTM; ++i)
 #pragma unroll
-            for (int j = 0; j < kTE; ++j) part[((wave * kTM + i) * kTE + j) * 64 + lane] = acc[i][j];
+            for (int j = 0; j < kTE; ++j) {
+                f32x4 v = acc[0][i][j];
+                if constexpr (kAcc == 2) v = joined(v, acc[1][i][j]);
+                part[((wave * kTM + i) * kTE + j) * 64 + lane] = v;
+            }
         __syncthreads();
     }
 

@@ -17,8 +17,8 @@ class MoeRouterGemm(nn.Module):
     """``forward(hidden_states, weight) -> logits``: bf16, fp16 or fp32 hidden
     states ``[..., H]`` (H % 8 == 0) times ``weight [E, H]`` (of their type or
     fp32, as checkpoints keep it), fp32 logits ``[..., E]`` from fp32 sums: no
-    rounding between the product and the choice of experts.  An infinity among fp32
-    operands gives infinite or NaN logits."""
+    rounding between the product and the choice of experts.  Infinities give the
+    formula's infinities and NaN, whatever the types and the number of tokens."""
 
     def forward(self, hidden_states: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         if _ops._host is not None and not torch.compiler.is_compiling():
