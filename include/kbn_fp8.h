@@ -537,8 +537,10 @@ int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* 
  *          aligned, strides below 2^23 elements; H % 8 == 0,
  *          H <= 2^22, T < 2^24, E <= 65536
  *   out    fp32 [T, E], row stride ld_out
- * fp32 sums of exact products (fp32 operands as three bf16 numbers, products
- * below 2^-24 of the largest left out), in one order for a shape and device.
+ * fp32 sums of products, in one order for a shape and device; products are exact
+ * but for fp32 w with fp32 or fp16 x and more tokens than 12 or 16, whose lowest
+ * parts are left out (operands as three and two bf16 numbers): up to 2^-21 of a
+ * product.  Infinities are the formula's.
  *   workspace: kbn_moe_router_gemm_workspace_bytes(...) bytes (0: none needed, -1
  *   for sizes that are refused), for this call alone while it runs.
  */

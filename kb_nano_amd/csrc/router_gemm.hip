@@ -16,10 +16,12 @@
 //
 // fp32 operands go through the 16-bit matrix instruction as well: a float is
 // the exact sum of three bf16 numbers (8 + 8 + 8 bits of its significand, cut
-// off by clearing low bits), and the products of pieces down to 2^-16 of the
-// largest are added, as good as fp32 products.  Products of leading pieces have a
-// sum of their own, which alone counts where it is not finite (an infinity's lower
-// pieces are no numbers): 1 to 3% of the time, and half of the error.
+// off by clearing low bits: the second is below 2^-7 of it, the third below 2^-15).
+// Of two such numbers the products of second and third pieces, up to 2^-22 each, are
+// left out, always towards 0: up to 2^-21 of a product, 2^-24.7 on average (an fp32
+// product's rounding: up to 2^-24).  Products of leading pieces have a sum of their own,
+// which alone counts where it is not finite (an infinity's lower pieces are no numbers):
+// 1 to 3% of the time, and half of the error.
 #include "row_stream.h"
 
 #include <algorithm>
