@@ -22,8 +22,10 @@
 // the chain of two launches (ids, list, rows; ids, list, h, B): 32 tokens of 24
 // adapters, 8192 x 8192, rank 16, 6.3 + 5.2 us.
 //
-// h enters the second product as the sum of two bf16 numbers (16 bits of its
-// significand, 2^-16 of the value lost, far below the output's own rounding).
+// h enters the second product as the sum of two bf16 numbers, each rounded to nearest:
+// off by 2^-17 at most, far below the output's own rounding (cut off instead, by up to
+// 2^-15, always towards 0).  fp16 B is the sum of two as well, exactly, and all four
+// products are added.
 #include "row_stream.h"
 
 #include <algorithm>
@@ -204,7 +206,7 @@ __device__ __forceinline__ uint16_t value_to(int d, float f) {
     return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-// Eight fp32 values as two bf16 numbers each, cut off (their sum is off by 2^-16 at most).
+// Eight values of an fp16 row as two bf16 numbers each, cut off: 8 and 3 bits, exact.
 __device__ __forceinline__ void split8(const float (&f)[8], u32x4& hi, u32x4& lo) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -214,6 +216,28 @@ __device__ __forceinline__ void split8(const float (&f)[8], u32x4& hi, u32x4& lo
         const uint32_t la = fa ? __float_as_uint(f[2 * i] - __uint_as_float(a & 0xFFFF0000u)) : 0u;
         const uint32_t lb = fb ? __float_as_uint(f[2 * i + 1] - __uint_as_float(b & 0xFFFF0000u)) : 0u;
         lo[i] = __builtin_amdgcn_perm(lb, la, 0x07060302u);
+    }
+}
+
+// Eight fp32 values as two bf16 numbers each, rounded to nearest: what the first leaves
+// is 2^-8 of the value at most, what the second leaves 2^-9 of that.  (The first is cut off
+// where rounding would make an infinity of it.)
+__device__ __forceinline__ void round8(const float (&f)[8], u32x4& hi, u32x4& lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bf16x2 near = __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), bf16x2);
+        const uint32_t both = __builtin_bit_cast(uint32_t, near);
+        float left[2];
+        uint32_t first[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float v = f[2 * i + j];
+            const uint32_t u = __float_as_uint(v), size = u & 0x7FFFFFFFu;
+            first[j] = size < 0x7F7F8000u ? (j ? both & 0xFFFF0000u : both << 16) : u & 0xFFFF0000u;
+            left[j] = size < 0x7F800000u ? v - __uint_as_float(first[j]) : 0.f;
+        }
+        hi[i] = __builtin_amdgcn_perm(first[1], first[0], 0x07060302u);
+        lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{left[0], left[1]}), bf16x2));
     }
 }
 
@@ -318,7 +342,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] *= sc;
             u32x4 hi, lo;
-            split8(v, hi, lo);
+            round8(v, hi, lo);
             if (i < 16 * tiles) {
                 *reinterpret_cast<u32x4*>(&part[0][i * kRow + r]) = hi;
                 *reinterpret_cast<u32x4*>(&part[1][i * kRow + r]) = lo;
@@ -384,7 +408,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void lora_expand_kernel(const Lo
                     const u32x4 hl = *reinterpret_cast<const u32x4*>(&part[1][(16 * m + row) * kRow + 32 * kk + 8 * q]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if constexpr (kD == kG16f) acc[m][j] = mma<false>(hh, bl[j], acc[m][j]);
+                        if constexpr (kD == kG16f) {   // the smallest products first
+                            acc[m][j] = mma<false>(hl, bl[j], acc[m][j]);
+                            acc[m][j] = mma<false>(hh, bl[j], acc[m][j]);
+                        }
                         acc[m][j] = mma<false>(hl, b[j], acc[m][j]);
                         acc[m][j] = mma<false>(hh, b[j], acc[m][j]);
                     }

@@ -21,8 +21,10 @@ class LoraAdd(nn.Module):
     ``base[t] + scaling[a] * lora_b[a] @ (lora_a[a] @ x[t])`` for ``a =
     adapter_ids[t]``, ``base[t]`` for ids outside [0, L) (requests without an
     adapter, padding).  ``x [..., K]`` and ``base [..., N]`` bf16 or fp16, adapters
-    of the same type, ids int32 or int64 ``[...]``, scaling fp32 [L].  fp32 sums, one
-    rounding at the end.  Returns a new tensor, or with ``inplace`` base itself (which
+    of the same type, ids int32 or int64 ``[...]``, scaling fp32 [L].  fp32 sums; the
+    scaled ``lora_a[a] @ x[t]`` enters the second product as two bf16 numbers (2^-17 of it
+    at most is lost), and the result is rounded once.  An infinity in x or an adapter
+    leaves infinities or NaN in its tokens' rows.  Returns a new tensor, or with ``inplace`` base itself (which
     may be x, and must not overlap lora_b, ids or scaling)."""
 
     def forward(self, x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
