@@ -565,7 +565,8 @@ PyObject* gated_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!x || !r || !w || !plain_or_none(args[3], post) || !plain_or_none(args[4], gate) || !number_of(args[5], rs) ||
             !number_of(args[6], eps) || !plain_thread())
             Py_RETURN_NONE;
-        const bool rows = args[7] == Py_True, codes = args[8] == Py_True;
+        const int rows = PyObject_IsTrue(args[7]), codes = PyObject_IsTrue(args[8]);   // any object, as in Python
+        if (rows < 0 || codes < 0) return nullptr;
         const at::ScalarType type = x->scalar_type();
         const int code = value_code(type);
         const int64_t dev = x->get_device();
