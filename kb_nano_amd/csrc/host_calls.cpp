@@ -644,7 +644,7 @@ PyObject* lora_add(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t T = xr.n, K = xr.k, N = br.k, L = a->size(0), R = a->size(1);
         if (a->size(2) != K || b->size(0) != L || b->size(1) != N || b->size(2) != R || K % 8 || L < 1 ||
             (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->get_device() != dev || ids->numel() != T ||
-            !ids->is_contiguous() || (sc && !is_vector(*sc, at::kFloat, dev, L)) || !launch_stream(dev, st))
+            !ids->is_contiguous() || (ids->dim() != 1 && ids->sizes() != x->sizes().slice(0, x->dim() - 1)) || (sc && !is_vector(*sc, at::kFloat, dev, L)) || !launch_stream(dev, st))
             Py_RETURN_NONE;
         const int64_t bytes = kbn_lora_add_workspace_bytes(T, K, L, R);
         if (bytes <= 0) Py_RETURN_NONE;

@@ -16,16 +16,29 @@ from . import _ops
 from .fp8_linear import Fp8Linear
 
 
+def _flat_ids(ids: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """``ids [T]`` in the order of x's rows.  Where both have several dimensions they have to be the same
+    (ones aside): ids [S, B] beside x [B, S, K] would give tokens each other's adapters."""
+    if ids.dim() == 1:
+        return ids
+    if ids.shape != x.shape[:-1]:
+        mine, rows = [n for n in ids.shape if n != 1], [n for n in x.shape[:-1] if n != 1]
+        if len(mine) > 1 and len(rows) > 1 and mine != rows:
+            raise ValueError(f"lora_add: adapter_ids {tuple(ids.shape)} and x {tuple(x.shape)} have other rows")
+    return ids.reshape(-1)
+
+
 class LoraAdd(nn.Module):
     """``forward(x, base, lora_a, lora_b, adapter_ids, scaling=None, inplace=False)``:
     ``base[t] + scaling[a] * lora_b[a] @ (lora_a[a] @ x[t])`` for ``a =
     adapter_ids[t]``, ``base[t]`` for ids outside [0, L) (requests without an
     adapter, padding).  ``x [..., K]`` and ``base [..., N]`` bf16 or fp16, adapters
-    of the same type, ids int32 or int64 ``[...]``, scaling fp32 [L].  fp32 sums; the
-    scaled ``lora_a[a] @ x[t]`` enters the second product as two bf16 numbers (2^-17 of it
-    at most is lost), and the result is rounded once.  An infinity in x or an adapter
-    leaves infinities or NaN in its tokens' rows.  Returns a new tensor, or with ``inplace`` base itself (which
-    may be x, and must not overlap lora_b, ids or scaling)."""
+    of the same type, ids int32 or int64 ``[...]`` or flat ``[T]``, scaling fp32
+    [L].  fp32 sums; the scaled ``lora_a[a] @ x[t]`` enters the second product as two
+    bf16 numbers (2^-17 of it at most is lost), and the result is rounded once.  An
+    infinity in x or an adapter leaves infinities or NaN in its tokens' rows.  Returns
+    a new tensor, or with ``inplace`` base itself (which may be x, and must not overlap
+    lora_b, ids or scaling)."""
 
     def forward(self, x: torch.Tensor, base: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter_ids: torch.Tensor, scaling: torch.Tensor | None = None, inplace: bool = False) -> torch.Tensor:
@@ -43,7 +56,7 @@ class LoraAdd(nn.Module):
             b2 = base.view(-1, base.shape[-1]) if inplace else base.reshape(-1, base.shape[-1])
         # (the compiler's ops write to no tensor that they also read)
         out = b2 if inplace and not tracing else torch.empty(b2.shape, dtype=base.dtype, device=base.device)
-        args = (x2, b2, lora_a, lora_b, adapter_ids.reshape(-1), scaling, out)
+        args = (x2, b2, lora_a, lora_b, _flat_ids(adapter_ids, x), scaling, out)
         if tracing:
             torch.ops.kb_nano_lora.add(*args)
             if inplace:

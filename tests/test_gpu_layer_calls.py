@@ -1,5 +1,5 @@
-"""Calls of the gated norms and the adapters beside their plain ones: truth values that are no bool, and the compiled
-forms of the adapters in place."""
+"""Calls of the gated norms and the adapters beside their plain ones: truth values that are no bool, ids of
+several dimensions, and the compiled forms of the adapters in place."""
 import pytest
 import torch
 
@@ -17,6 +17,20 @@ def test_with_rows_goes_by_its_truth_value(gpu_device, yes, no):
     *_, rows = got = GatedAddRMSNormFP8Quant()(x, x, x[0], with_rows=yes)
     assert len(got) == 4 and torch.equal(rows, normed)
     assert len(GatedAddRMSNormFP8Quant()(x, x, x[0], with_rows=no)) == 3
+
+
+def test_ids_of_several_dimensions(gpu_device):
+    from kb_nano_amd import LoraAdd
+    x, base, a, b, ids, s = args(make(12, 64, 128, 4, 8, BF16, 3, gpu_device))
+    out = LoraAdd()(x, base, a, b, ids, s)
+    x3, b3 = x.view(3, 4, 128), base.view(3, 4, 64)
+    for i in (ids.view(3, 4), ids):
+        assert torch.equal(LoraAdd()(x3, b3, a, b, i, s).view(12, 64), out)
+    assert torch.equal(LoraAdd()(x, base, a, b, ids.view(3, 4), s), out)
+    for i in (ids.view(4, 3), ids.view(3, 4).t(), ids.view(2, 6)):
+        for inplace in (False, True):
+            with pytest.raises(ValueError, match="adapter_ids"):
+                LoraAdd()(x3, b3, a, b, i, s, inplace)
 
 
 def _compiled(fn):
