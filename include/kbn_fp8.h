@@ -536,7 +536,7 @@ int kbn_few_token_experts(const void* x, int x_dtype, int64_t ld_x, const void* 
  *          w_dtype 0 bf16, 1 fp16, 2 fp32, w of x's type or fp32; rows 16-byte
  *          aligned, strides below 2^23 elements; H % 8 == 0,
  *          H <= 2^22, T < 2^24, E <= 65536
- *   out    fp32 [T, E], row stride ld_out
+ *   out    fp32 [T, E], row stride ld_out; overlaps neither x nor w
  * fp32 sums of products, in one order for a shape and device; products are exact
  * but for fp32 w with fp32 or fp16 x and more tokens than 12 or 16, whose lowest
  * parts are left out (operands as three and two bf16 numbers): up to 2^-21 of a
@@ -562,7 +562,8 @@ int kbn_moe_router_gemm(const void* x, int x_dtype, int64_t ld_x, const void* w,
  *   values (groups and experts) go to the lower index.
  *   weights  fp32 [T, top_k]: the experts' scores, over their sum if
  *            renormalize (0 where that is 0), times scale
- *   ids      int32 or int64 (id_bytes 4, 8) [T, top_k]
+ *   ids      int32 or int64 (id_bytes 4, 8) [T, top_k]; no output overlaps another
+ *            or what is read
  * Experts of logit -inf or NaN are masked: taken only where no other is left,
  * with weight 0.  +inf counts as the largest float.  Choice values and weights
  * are computed in 64 bits.

@@ -1081,13 +1081,44 @@ def few_token_experts(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tenso
         T, topk, E, H, inter, out.data_ptr(), _ld(out), buf.data_ptr(), nbytes, _stream(x)), what)
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    lo = t.data_ptr()
+    if t.is_contiguous():
+        return lo, lo + t.nbytes
+    return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the storage byte ranges spanned by two tensors intersect."""
-    def span(t):
-        lo = t.data_ptr()
-        return lo, lo + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
+def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two sets of contiguous rows of one stride lie beside each other: columns of one buffer."""
+    def rows(t):
+        return t.dim() == 2 and t.shape[0] > 1 and (t.stride(1) == 1 or t.shape[1] == 1)
+    if not rows(a) or not rows(b):
+        return False
+    step, width_a, width_b = (a.stride(0) * a.element_size(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size())
+    if step <= 0 or b.stride(0) * b.element_size() != step:
+        return False
+    at = (b.data_ptr() - a.data_ptr()) % step
+    return width_a <= at and at + width_b <= step
+
+
+def _apart(what: str, outs: dict, reads: dict) -> None:
+    """Outputs overlap neither each other nor what is read (other workgroups may still
+    read it); by name, None for those that are not there, none of them empty."""
+    seen = [(n, t, *_span(t)) for n, t in reads.items() if t is not None]
+    for name, o in outs.items():
+        if o is None:
+            continue
+        lo, hi = _span(o)
+        for other, t, a, b in seen:
+            if a < hi and lo < b and not _beside(o, t):
+                raise ValueError(f"{what}: {name} overlaps {other}")
+        seen.append((name, o, lo, hi))
 
 
 def moe_router_gemm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) -> None:
@@ -1111,6 +1142,7 @@ def moe_router_gemm(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) ->
     _mx_rows(what, "output", out, (T, E))
     if T == 0:
         return
+    _apart(what, {"output": out}, {"hidden states": x, "weight": weight})
     x, weight = _near(x), _near(weight)
     L = lib()
     xc, wc = _QUANT_IN[x.dtype], _QUANT_IN[weight.dtype]
@@ -1157,6 +1189,9 @@ def moe_router_topk(logits: torch.Tensor, top_k: int, scoring: str, bias: torch.
     for t, name in ((weights, "weights"), (ids, "ids")):
         if tuple(t.shape) != (T, top_k) or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be contiguous {(T, top_k)}, got {tuple(t.shape)}")
+    if T == 0:
+        return
+    _apart(what, {"weights": weights, "ids": ids}, {"logits": logits, "bias": bias})
     check(lib().kbn_moe_router_topk(
         logits.data_ptr(), _QUANT_IN[logits.dtype], _ld(logits), bias.data_ptr() if bias is not None else None, T, E, top_k,
         1 if scoring == "sigmoid" else 0, num_groups, topk_groups, 1 if renormalize else 0, float(scale), weights.data_ptr(),
@@ -1207,6 +1242,9 @@ def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
             raise ValueError(f"{what}: output_scales must be {(T, -(-H // GROUP))}, got {tuple(out_scale.shape)}")
     if T == 0:
         return
+    in_place = residual_out.data_ptr() == residual.data_ptr() and _ld(residual_out) == _ld(residual)
+    _apart(what, {"residual output": residual_out, "output": out, "output_fp8": out_fp8, "output_scales": out_scale},
+           {"input": x, "residual": None if in_place else residual, "weight": weight, "post_weight": post_weight, "gate": gate})
     check(lib().kbn_gated_add_rmsnorm(
         x.data_ptr(), _QUANT_IN[x.dtype], _ld(x), residual.data_ptr(), _ld(residual), weight.data_ptr(),
         post_weight.data_ptr() if post_weight is not None else None, gate.data_ptr() if gate is not None else None, *gs,
