@@ -17,10 +17,11 @@
 // has to be known of the ids on the host.
 //
 // Bound by rows, base and out for prompts: 4096 tokens of 8 adapters in runs, 7168 x
-// 16384, rank 32: 24 to 33 us (4.1 to 5.6 TB/s) and 33 us (3.5 TB/s: the products of a
-// strip are not all hidden behind the next one's loads).  A decode batch is bound by
-// the chain of two launches (ids, list, rows; ids, list, h, B): 32 tokens of 24
-// adapters, 8192 x 8192, rank 16, 6.3 + 5.2 us.
+// 16384, rank 32: 25 to 43 us (134 MB of x at 3.1 to 5.4 TB/s, by what of it the
+// memory-side cache holds) and 32 to 34 us (3.5 TB/s: the products of a strip are not all
+// hidden behind the next one's loads).  A decode batch is bound by the chain of two
+// launches (ids, list, rows; ids, list, h, B): 32 tokens of 24 adapters, 8192 x 8192,
+// rank 16, 6 to 6.6 + 5.4 to 7 us.
 //
 // h enters the second product as the sum of two bf16 numbers, each rounded to nearest:
 // off by 2^-17 at most, far below the output's own rounding (cut off instead, by up to

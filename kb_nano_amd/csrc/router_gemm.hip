@@ -5,7 +5,7 @@
 // that share neither (many: 4096 x 256 x 7168 bf16 24.1 us, 470 MB through 256 CUs
 // at 76 B/ns each, 0.62 PFLOP/s; memory alone 13), with weights in fp32 the
 // matrix instructions and the barriers of a stage (2051 x 256 x 7168 with bf16 rows
-// 34 us, three products each: 0.66 PFLOP/s).  The wavefronts of a workgroup share one tile of
+// 36 us, three products each: 0.63 PFLOP/s).  The wavefronts of a workgroup share one tile of
 // logits and split its K, unit by unit; each streams whole 128-byte lines of its
 // units through a private LDS ring by direct loads, so there is no barrier until
 // their sums meet in LDS, in wavefront order.  (Fragments loaded straight into
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void router_gemm_tile_kernel(con
 // each operand a stage (32 K) and holds those of the next kAhead stages (one, two or three:
 // the same times within 3%; of fp16 rows one, with which two workgroups fit a CU's
 // registers).  (In the tiles above each wavefront takes its
-// own K's values apart: 2051 x 256 x 7168 with fp32 weights 58 us, here 34.)
+// own K's values apart: 2051 x 256 x 7168 with fp32 weights 58 us, here 36.)
 constexpr int kWideT = 128, kWideE = 128, kWideK = 32, kWideThreads = 512;
 
 template <int kX>
@@ -294,7 +294,8 @@ double sum_price(int64_t T, int64_t E, int s) { return s > 1 ? 2400.0 + 200.0 * 
 // lone workgroup of a CU and each two (of fp32 rows LDS holds one).  Fitted to 10
 // token counts from 61 to 4096 with those and three more sizes: 1.2% on average, 15%
 // at most (2051 x 256 x 7168, wide and not: bf16 rows 34 and 53 us, fp16 44 and 76,
-// fp32 51 and 99; 777 x 128 x 4096 bf16 15 and 12).
+// fp32 51 and 99; 777 x 128 x 4096 bf16 15 and 12; before leading pieces had sums of
+// their own, which cost both alike).
 GatePlan gate_plan(int64_t T, int64_t E, int64_t H, int xd, int wd) {
     if (T <= (xd == kG32 ? kRowTokens32 : kRowTokens)) return {0, 0, 1};
     const int64_t units = (H + kStreamK - 1) / kStreamK, cus = cu_count();

@@ -17,9 +17,10 @@
 // depends on is computed in 64 bits, and so are the few weights.
 //
 // Reads and writes are small (16384 x 256 fp32 logits, top 8 with groups and a bias:
-// 18 MB, 4 us at the rate of a copy): the instructions bound it, some 1100 for four
-// tokens, and for few tokens their latency (that case 18 us, 1 TB/s; one token 5.1;
-// 777 x 128, no groups, 3.9).
+// 18 MB, 4 us at the rate of a copy).  That case takes 18 us (1 TB/s): 14 the four-token
+// way, some 1100 instructions a wavefront, and 4 to 5 the last way of the 1 to 7 tokens
+// that need it, which ends after all others.  Few tokens take the latency of their
+// instructions (one token 5.4; 777 x 128, no groups, 3.8).
 //
 // The general path: one wavefront a token, expert e = lane * V + j in register j, so the lowest
 // index of equal keys is the first lane's first register.  Keys are the values'

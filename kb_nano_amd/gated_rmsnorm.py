@@ -60,7 +60,9 @@ class GatedAddRMSNorm(nn.Module):
     """``forward(input, residual, weight, post_weight=None, gate=None,
     residual_scale=1.0, eps=1e-6) -> (normed, residual')``, both new tensors of
     input's shape ``[..., H]``.  ``gate`` broadcasts against input: [H] a value for
-    each channel, [..., 1] for each token, [..., H] for each element."""
+    each channel, [..., 1] for each token, [..., H] for each element.  Others ([B, 1, H],
+    one for each sequence) are spread to a [T, H] of their own first: one launch and
+    two such tensors of traffic more."""
 
     def forward(self, input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
                 post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
