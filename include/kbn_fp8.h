@@ -599,6 +599,8 @@ int kbn_gated_add_rmsnorm(const void* x, int dtype, int64_t ld_x, const void* r,
  *   adapters of smaller rank padded with zeros.  x and adapters 16-byte aligned,
  *   x's row stride below 2^22 elements; T <= 65535 * 64, an adapter's B below 2 GiB.
  *   out may be base, and base x; nothing else that is read may overlap out.
+ * fp32 sums; scaling * A x enters the second product as two bf16 numbers (2^-17 of it
+ * at most is lost).
  *   workspace: kbn_lora_add_workspace_bytes(T, K, L, R) bytes (-1 for sizes that
  *   are refused), for this call alone while it runs.
  */

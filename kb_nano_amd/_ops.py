@@ -1095,13 +1095,14 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two sets of contiguous rows of one stride lie beside each other: columns of one buffer."""
-    def rows(t):
-        return t.dim() == 2 and t.shape[0] > 1 and (t.stride(1) == 1 or t.shape[1] == 1)
-    if not rows(a) or not rows(b):
-        return False
-    step, width_a, width_b = (a.stride(0) * a.element_size(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size())
-    if step <= 0 or b.stride(0) * b.element_size() != step:
+    """Whether two sets of rows (contiguous, or of one value each) of one stride lie
+    beside each other: columns of one buffer."""
+    def rows(t):   # (stride, width) in bytes
+        if t.dim() != 2 or t.shape[0] < 2 or (t.stride(1) not in (0, 1) and t.shape[1] > 1):
+            return 0, 0
+        return t.stride(0) * t.element_size(), (t.shape[1] if t.stride(1) else 1) * t.element_size()
+    (step, width_a), (step_b, width_b) = rows(a), rows(b)
+    if step == 0 or step != step_b:
         return False
     at = (b.data_ptr() - a.data_ptr()) % step
     return width_a <= at and at + width_b <= step

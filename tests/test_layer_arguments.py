@@ -117,6 +117,12 @@ def test_columns_of_one_buffer_do_not_overlap(no_launch):
     d["q"], d["s"] = packed[:, :256].view(torch.float8_e4m3fn), packed[:, 256:].view(F32)
     with pytest.raises(AssertionError, match="launched"):
         run_norm(no_launch, d)
+    wide = torch.zeros(4, 1032, dtype=BF16)      # a gate for each token beside the rows
+    e = {**d, **{k: wide[:, 256 * i:256 * (i + 1)] for i, k in enumerate(("x", "r", "r_out", "n_out"))}}
+    with pytest.raises(AssertionError, match="launched"):
+        run_norm(no_launch, {**e, "gate": wide[:, 1024:1025].expand(4, 256)})
+    with pytest.raises(ValueError, match="overlaps gate"):
+        run_norm(no_launch, {**e, "gate": wide[:, 1000:1001].expand(4, 256)})
     for k, v in (("n_out", store[:, 504:760]), ("r_out", store[:, 8:264]), ("n_out", store[:, 248:504]), ("x", store[:, 760:1016]),
                  ("s", packed[:, 248:256].view(F32))):
         e = {**d, k: v}
